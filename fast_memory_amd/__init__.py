@@ -9,8 +9,10 @@ from .hash_attention import attention_hash, attention_hash_varlen, attention_has
 from .memory import (Memory, MemoryBatch, calc_ref_centroids, compute_centroids, fit_projection, init_centroids, kmeans_spherical, learn_emb_proj,  # noqa: F401
                      merge, ring_attention_masked_backward, ring_attention_masked_forward, update_out_and_lse)
 
-from .autograd import attention_hash_varlen_op, local_attention_backward, ring_cross_attention_approx  # noqa: F401,E402
+from .autograd import attention_hash_varlen_op, local_attention, local_attention_backward, ring_cross_attention_approx  # noqa: F401,E402
+from .ops import ScoreTerms  # noqa: F401,E402
+from .paged import PagedCache  # noqa: F401,E402
 
-__all__ = ["attention_hash_varlen_op", "local_attention_backward", "ring_cross_attention_approx", "attention_hash", "attention_hash_varlen", "attention_hash_varlen_backward", "Memory", "MemoryBatch", "calc_ref_centroids", "compute_centroids", "fit_projection",
+__all__ = ["PagedCache", "ScoreTerms", "local_attention", "attention_hash_varlen_op", "local_attention_backward", "ring_cross_attention_approx", "attention_hash", "attention_hash_varlen", "attention_hash_varlen_backward", "Memory", "MemoryBatch", "calc_ref_centroids", "compute_centroids", "fit_projection",
            "init_centroids", "kmeans_spherical", "learn_emb_proj", "merge", "ring_attention_masked_backward", "ring_attention_masked_forward",
            "update_out_and_lse"]

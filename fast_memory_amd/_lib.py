@@ -18,6 +18,8 @@ FM_MAX_D = 256
 FM_QTILE = 64
 FM_STATIC_SCRATCH_BYTES = 32 << 20
 FM_FUSED_STATUS_INTS = 66
+FM_CACHE_META_INTS = 16
+FM_CACHE_MAX_PAGE = 4096
 
 P = c_void_p
 
@@ -63,6 +65,19 @@ SIGNATURES = {
     "fm_decode_hash_attn": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_float, P, P, P, P, c_int, P]),
     "fm_local_attn_fwd": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
                                   c_int, P]),
+    "fm_cache_book_ints": (c_size_t, [c_int] * 3),
+    "fm_cache_workspace": (c_size_t, [c_int] * 2),
+    "fm_cache_append": (c_int, [P, P, P] + [c_int] * 6 + [P, P] + [c_int64] * 4 + [P, c_int, c_int, P, c_size_t, P]),
+    "fm_cache_fork": (c_int, [P, P, P] + [c_int] * 6 + [P, c_int, P, c_size_t, P]),
+    "fm_cache_drop": (c_int, [P] + [c_int] * 4 + [P, P]),
+    "fm_cache_compact": (c_int, [P, P, P] + [c_int] * 7 + [P, c_size_t, P]),
+    "fm_local_attn_terms_fwd_workspace": (c_size_t, [c_int] * 6),
+    "fm_local_attn_terms_fwd": (c_int, [P] * 5 + [c_float] + [P] * 4 + [c_int] * 5 + [c_float, c_int, c_int, P, c_size_t, P]),
+    "fm_local_attn_terms_bwd_workspace": (c_size_t, [c_int] * 6),
+    "fm_local_attn_terms_bwd": (c_int, [P] * 10 + [c_float] + [P] * 4 + [c_int] * 5 + [c_float, c_int, c_int, P, c_size_t, P]),
+    "fm_paged_attn_fwd_workspace": (c_size_t, [c_int] * 9),
+    "fm_paged_attn_fwd": (c_int, [P, c_int64, c_int64, P, P, P] + [c_int] * 4 + [P, P, c_int64, c_int64, P, c_int64, c_int64] +
+                          [c_int] * 5 + [c_float, c_float, P, P, c_int, P, c_size_t, P]),
     "fm_lse_merge": (c_int, [P, P, P, P, c_int64, c_int, c_int, P]),
     "fm_l2_normalize": (c_int, [P, P, c_int64, c_int, c_float, c_int, P]),
     "fm_topk_mean": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P]),

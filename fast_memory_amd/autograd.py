@@ -170,13 +170,17 @@ def _causal_prefix_lists(H: int, t0: int, t1: int, S: int, L: int, device):
 
 
 def local_attention_backward(d_out, q, k, v, out, lse, sm_scale: float, causal: bool = True,
-                             staged: Optional[bool] = None):
+                             staged: Optional[bool] = None, terms: Optional[ops.ScoreTerms] = None,
+                             dlse: Optional[torch.Tensor] = None):
     """Gradients of the dense local attention (the ``attention_backward(dout, q, k_self, v_self, out, lse,
     sm_scale, True)`` call at memory.py:368, which the reference does not define).  ``q, out, d_out
     [H*G,S,d]``, ``k, v [H,L,d]``, ``lse [H*G,S]``; ``out`` / ``lse`` may be the merged result.  Returns
     ``(dq [H*G,S,d], dk, dv [H,L,d] fp32)``.
 
-    No kernel of its own: given ``out`` and ``lse`` the backward is a sum over keys, so the causal case is two
+    With ``terms`` (:class:`ops.ScoreTerms`) or ``dlse`` it is the backward of :func:`local_attention`, which has kernels of
+    its own: ``dk`` and ``dv`` come in the inputs' type.
+
+    Without, no kernel of its own: given ``out`` and ``lse`` the backward is a sum over keys, so the causal case is two
     backwards of the gathered attention whose key sets partition every token's prefix.  In the first, blocks of
     8 tokens (with all their G query heads: 8 G queries) share a bucket that lists the keys all of them see; in
     the second every token has a bucket of its own with the up to 7 keys left.  The lists of the first hold
@@ -187,6 +191,12 @@ def local_attention_backward(d_out, q, k, v, out, lse, sm_scale: float, causal: 
     ``staged`` is passed on to :func:`attention_hash_varlen_backward`: ``None`` (the default) takes the form
     without atomics for bf16 with d = 128 where a call has at least as many queries as buckets (results do not
     depend on scheduling) and the atomic adds otherwise or when its workspace does not fit."""
+    if terms is not None or dlse is not None:
+        if staged is not None:
+            raise ValueError("local_attention_backward: staged chooses among gathered backwards; there are none with terms or dlse")
+        same = lambda t: t.to(q.dtype).contiguous()
+        return ops.local_attn_terms_bwd(same(d_out), q.contiguous(), k.contiguous(), v.contiguous(), same(out),
+                                        lse.float().contiguous(), sm_scale, causal, terms, dlse)
     HG, S, d = q.shape
     H, L, _ = k.shape
     G = HG // H
@@ -227,13 +237,50 @@ def local_attention_backward(d_out, q, k, v, out, lse, sm_scale: float, causal: 
     return dq.reshape(HG, S, d), dk, dv
 
 
+class _LocalAttentionFunc(torch.autograd.Function):
+    """Local attention with score terms.  Everything the backward reads, the terms' tensors among it, goes through
+    save_for_backward, so that an in-place change between forward and backward is caught."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, sm_scale, causal, softcap, slopes, doc_q, doc_k, prefix):
+        terms = ops.ScoreTerms(softcap, slopes, doc_q, doc_k, prefix)
+        out, lse = ops.local_attn_terms_fwd(q, k, v, sm_scale, causal, terms)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, doc_q, doc_k, prefix)
+        ctx.sm_scale, ctx.causal, ctx.softcap = sm_scale, causal, softcap
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlse):
+        q, k, v, out, lse, slopes, doc_q, doc_k, prefix = ctx.saved_tensors
+        if dout is None and dlse is None:
+            return (None,) * 10
+        dout = torch.zeros_like(q) if dout is None else dout.to(q.dtype).contiguous()
+        dq, dk, dv = ops.local_attn_terms_bwd(dout, q, k, v, out, lse, ctx.sm_scale, ctx.causal,
+                                              ops.ScoreTerms(ctx.softcap, slopes, doc_q, doc_k, prefix), dlse)
+        return (dq, dk, dv) + (None,) * 7
+
+
+def local_attention(q, k, v, sm_scale: float, causal: bool = True, terms: Optional[ops.ScoreTerms] = None):
+    """The local attention (call site memory.py:302-304) with :class:`ops.ScoreTerms`, differentiable in ``q``, ``k`` and
+    ``v`` through ``out`` and ``lse``: ``q [H*G,S,d]``, ``k, v [H,L,d]`` -> ``(out [H*G,S,d], lse [H*G,S] fp32)``.  The
+    gradients do not depend on scheduling."""
+    t = ops.ScoreTerms() if terms is None else terms
+    if t.slopes is not None and t.slopes.requires_grad:
+        raise ValueError("slopes receive no gradient: pass them detached")
+    return _LocalAttentionFunc.apply(q.contiguous(), k.contiguous(), v.contiguous(), float(sm_scale), bool(causal),
+                                     float(t.softcap), t.slopes, t.doc_q, t.doc_k, t.prefix)
+
+
 # ------------------------------------------------------------------ the module forward as one Function
 class _ApproxCrossAttentionFunc(torch.autograd.Function):
     """``_RingApproxCrossAttentionFunc`` (memory.py:234-418) with a world of one: no all-reduce, all-to-all,
     all-gather or ring steps; the key window is all of ``k``."""
 
     @staticmethod
-    def forward(ctx, q, kq, k_self, v_self, k, v, rnd_centroids, sm_scale, n_hashes, n_results, centroid_topk):
+    def forward(ctx, q, kq, k_self, v_self, k, v, rnd_centroids, sm_scale, n_hashes, n_results, centroid_topk,
+                softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, with_terms=False):
         from .memory import Memory, compute_centroids, update_out_and_lse
         batch_size, n_heads, seq_len, d_qkv = q.shape
         assert batch_size == 1
@@ -248,8 +295,11 @@ class _ApproxCrossAttentionFunc(torch.autograd.Function):
         mem = Memory.build(k[0], v[0], A, min(int(n_results), context_len))                 # memory.py:260-278
         q3 = q[0].reshape(k_heads, n_groups * seq_len, d_qkv).contiguous()
         q_hashes = mem.hash(q3)                                                             # memory.py:280-283
-        block_out, block_lse = ops.local_attn_fwd(q[0].contiguous(), k_self[0].contiguous(), v_self[0].contiguous(),
-                                                  sm_scale, True)                           # memory.py:302-304
+        local = (q[0].contiguous(), k_self[0].contiguous(), v_self[0].contiguous(), sm_scale, True)
+        if with_terms:
+            block_out, block_lse = ops.local_attn_terms_fwd(*local, ops.ScoreTerms(softcap, slopes, doc_q, doc_k, prefix))
+        else:
+            block_out, block_lse = ops.local_attn_fwd(*local)                               # memory.py:302-304
         out, lse = update_out_and_lse(None, None, block_out.reshape(q3.shape), block_lse.reshape(k_heads, -1))
         mo, ml = mem.attend(q3, sm_scale, q_hash=q_hashes)                                  # memory.py:319-321
         out, lse = update_out_and_lse(out.contiguous(), lse.contiguous(), mo, ml)           # memory.py:332
@@ -261,14 +311,17 @@ class _ApproxCrossAttentionFunc(torch.autograd.Function):
         # instead of silently giving gradients against the new contents, and the bucket lists with their
         # key-ordered copy, from which the backward rebuilds a Memory view without building an index again.
         attn_idx = mem._attn_idx if mem._attn_idx is not None else mem.bucket_idx.new_empty(0)
-        ctx.save_for_backward(q, k_self, v_self, q_hashes, out, lse.squeeze(-1), k, v, A, mem.bucket_idx, attn_idx)
+        ctx.with_terms, ctx.softcap = with_terms, softcap
+        ctx.save_for_backward(q, k_self, v_self, q_hashes, out, lse.squeeze(-1), k, v, A, mem.bucket_idx, attn_idx,
+                              slopes, doc_q, doc_k, prefix)
         ctx.mark_non_differentiable(q_hashes)
         return out.reshape(q.shape), q_hashes
 
     @staticmethod
     def backward(ctx, dout, _d_hashes):
         from .memory import Memory
-        q, k_self, v_self, q_hashes, out, lse, k, v, A, bucket_idx, attn_idx = ctx.saved_tensors
+        q, k_self, v_self, q_hashes, out, lse, k, v, A, bucket_idx, attn_idx, *term_tensors = ctx.saved_tensors
+        terms = ops.ScoreTerms(ctx.softcap, *term_tensors) if ctx.with_terms else None
         sm_scale = ctx.sm_scale
         mem = Memory(k[0], v[0], A, bucket_idx)
         if attn_idx.numel():
@@ -280,18 +333,18 @@ class _ApproxCrossAttentionFunc(torch.autograd.Function):
         # memory.py:367-369: the local part, with the merged out / lse
         dq, dk_self, dv_self = local_attention_backward(dout[0].to(q.dtype).contiguous(), q[0].contiguous(),
                                                         k_self[0], v_self[0], out.reshape(n_heads, seq_len, d_qkv),
-                                                        lse.reshape(n_heads, seq_len), sm_scale, True)
+                                                        lse.reshape(n_heads, seq_len), sm_scale, True, terms=terms)
         # memory.py:386-393: the memory part
         mq, dk, dv = mem.attend_backward(dout3, q3, out, lse, sm_scale, q_hash=q_hashes)
         dq = dq.float() + mq.reshape(n_heads, seq_len, d_qkv).float()
         cast = lambda t, like: t.to(like.dtype).reshape(like.shape)
         return (cast(dq, q), None, cast(dk_self, k_self), cast(dv_self, v_self), cast(dk, mem.keys.unsqueeze(0)),
-                cast(dv, mem.values.unsqueeze(0)), None, None, None, None, None)
+                cast(dv, mem.values.unsqueeze(0))) + (None,) * 11
 
 
 def ring_cross_attention_approx(q, kq, k_self, v_self, k, v, rnd_centroids, sm_scale, n_hashes, n_results, *,
                                 centroid_topk: int, sampling_method: Optional[str] = None,
-                                return_hashes: bool = False):
+                                return_hashes: bool = False, local_terms: Optional[ops.ScoreTerms] = None):
     """Drop-in for ``ring_cross_attention_approx`` (memory.py:421-425) on one device.
 
     :param q: ``[1, n_heads, seq_len, d]``
@@ -300,9 +353,11 @@ def ring_cross_attention_approx(q, kq, k_self, v_self, k, v, rnd_centroids, sm_s
     :param k, v: ``[1, k_heads, context_len, d]`` the memory
     :param rnd_centroids: ``[n_hashes, d]`` initial centroids (memory.py:489-493)
     :param centroid_topk: the reference's ``consts.centroid_topk`` (memory.py:220)
+    :param local_terms: :class:`ops.ScoreTerms` of the local attention (the memory's scores have none)
     :return: ``out [1, n_heads, seq_len, d]`` in q's dtype; differentiable in ``q``, ``k_self``, ``v_self``,
         ``k`` and ``v`` (``kq`` and the centroids receive no gradient, memory.py:418).
     """
     out, hashes = _ApproxCrossAttentionFunc.apply(q, kq, k_self, v_self, k, v, rnd_centroids, float(sm_scale),
-                                                  int(n_hashes), int(n_results), int(centroid_topk))
+                                                  int(n_hashes), int(n_results), int(centroid_topk),
+                                                  *(local_terms or ops.ScoreTerms()), local_terms is not None)
     return (out, hashes) if return_hashes else out

@@ -1,0 +1,129 @@
+// C entry points of the local attention with score terms and of the attention over a paged cache.
+#include <math.h>
+
+#include "terms_api.hpp"
+
+namespace fm {
+
+extern std::atomic<int> g_force_generic;
+
+static bool cap_ok(float sm_scale, float softcap) {
+  return softcap == 0.f || (softcap > 0.f && isfinite(softcap * kLog2e) && isfinite(sm_scale / softcap));
+}
+
+static int terms_check(const char* name, const FwdArgs& a) {
+  FM_REQUIRE(a.H >= 1 && a.G >= 1 && a.S >= 1 && a.L >= 1 && a.d >= 1 && a.d <= FM_MAX_D, FM_ERR_ARG,
+             "%s: H=%d G=%d S=%d L=%d d=%d", name, a.H, a.G, a.S, a.L, a.d);
+  FM_REQUIRE(dtype_ok(a.dtype), FM_ERR_ARG, "%s: dtype=%d", name, a.dtype);
+  FM_REQUIRE(a.sm_scale > 0.f && isfinite(a.sm_scale), FM_ERR_ARG, "%s: sm_scale=%g", name, double(a.sm_scale));
+  FM_REQUIRE(cap_ok(a.sm_scale, a.t.softcap), FM_ERR_ARG, "%s: softcap=%g", name, double(a.t.softcap));
+  FM_REQUIRE((a.t.doc_q == nullptr) == (a.t.doc_k == nullptr), FM_ERR_ARG, "%s: doc_q and doc_k come together", name);
+  FM_REQUIRE(a.q && a.k && a.v && a.out && a.lse, FM_ERR_ARG, "%s: null pointer", name);
+  FM_REQUIRE(int64_t(a.H) * a.G <= 65535 && int64_t(a.H) * a.G * a.S <= 0x7fffffffLL && int64_t(a.H) * a.L <= 0x7fffffffLL &&
+                 a.S <= (1 << 24) && a.L <= (1 << 24),
+             FM_ERR_UNSUPPORTED, "%s: H*G=%lld S=%d L=%d", name, (long long)a.H * a.G, a.S, a.L);
+  return FM_OK;
+}
+
+template <template <typename> class F, typename... A>
+static int by_type(int dtype, A&&... a) {
+  if (dtype == FM_F32) return F<float>::run(a...);
+  if (dtype == FM_BF16) return F<bf16_t>::run(a...);
+  return F<f16_t>::run(a...);
+}
+template <typename T>
+struct FwdRows {
+  static int run(const FwdArgs& a, hipStream_t st) { return terms_fwd_rows<T>(a, st); }
+};
+template <typename T>
+struct BwdRows {
+  static int run(const BwdArgs& a, float* delta, hipStream_t st) {
+    int rc = terms_delta<T>(a, delta, st);
+    return rc ? rc : terms_bwd_rows<T>(a, delta, st);
+  }
+};
+template <typename T>
+struct PagedRows {
+  static int run(const PagedArgs& a, hipStream_t st) { return paged_attn_rows<T>(a, st); }
+};
+
+static size_t delta_bytes(int H, int G, int S) { return align_up(size_t(H) * G * S * 4, 256); }
+
+}  // namespace fm
+
+extern "C" size_t fm_local_attn_terms_fwd_workspace(int H, int G, int S, int L, int d, int dtype) {
+  if (H < 1 || G < 1 || S < 1 || L < 1 || d < 1) return 0;
+  (void)dtype;
+  return 256;
+}
+
+extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void* v, void* out, float* lse, float softcap,
+                                       const float* slopes, const int32_t* doc_q, const int32_t* doc_k,
+                                       const int32_t* prefix, int H, int G, int S, int L, int d, float sm_scale, int causal,
+                                       int dtype, void* ws, size_t ws_bytes, void* stream) {
+  using namespace fm;
+  const FwdArgs a{q, k, v, out, lse, {slopes, doc_q, doc_k, prefix, softcap, causal != 0}, H, G, S, L, d, dtype, sm_scale};
+  int rc = terms_check("fm_local_attn_terms_fwd", a);
+  if (rc) return rc;
+  const size_t need = fm_local_attn_terms_fwd_workspace(H, G, S, L, d, dtype);
+  FM_REQUIRE(ws, FM_ERR_ARG, "fm_local_attn_terms_fwd: null pointer");
+  FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_fwd: workspace %zu < %zu", ws_bytes, need);
+  return by_type<FwdRows>(dtype, a, as_stream(stream));
+}
+
+extern "C" size_t fm_local_attn_terms_bwd_workspace(int H, int G, int S, int L, int d, int dtype) {
+  if (H < 1 || G < 1 || S < 1 || L < 1 || d < 1) return 0;
+  (void)dtype;
+  return fm::delta_bytes(H, G, S);
+}
+
+extern "C" int fm_local_attn_terms_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
+                                       const void* dout, const float* dlse, void* dq, void* dk, void* dv, float softcap,
+                                       const float* slopes, const int32_t* doc_q, const int32_t* doc_k,
+                                       const int32_t* prefix, int H, int G, int S, int L, int d, float sm_scale, int causal,
+                                       int dtype, void* ws, size_t ws_bytes, void* stream) {
+  using namespace fm;
+  const BwdArgs a{{q, k, v, const_cast<void*>(out), const_cast<float*>(lse), {slopes, doc_q, doc_k, prefix, softcap, causal != 0},
+                   H, G, S, L, d, dtype, sm_scale},
+                  dout, dlse, dq, dk, dv};
+  int rc = terms_check("fm_local_attn_terms_bwd", a.f);
+  if (rc) return rc;
+  FM_REQUIRE(dout && dq && dk && dv && ws, FM_ERR_ARG, "fm_local_attn_terms_bwd: null pointer");
+  const size_t need = fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dtype);
+  FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_bwd: workspace %zu < %zu", ws_bytes, need);
+  return by_type<BwdRows>(dtype, a, static_cast<float*>(ws), as_stream(stream));
+}
+
+extern "C" size_t fm_paged_attn_fwd_workspace(int rows, int T, int max_new, int H, int G, int d, int width, int page, int dtype) {
+  if (rows < 1 || T < 1 || H < 1 || G < 1 || d < 1 || width < 1 || page < 1) return 0;
+  (void)max_new;
+  (void)dtype;
+  return 256;
+}
+
+extern "C" int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head, const void* k_pages, const void* v_pages,
+                                 const int32_t* book, int n_pages, int rows, int width, int page, const int32_t* cu, void* out,
+                                 int64_t out_token, int64_t out_head, float* lse, int64_t lse_token, int64_t lse_head, int T,
+                                 int max_new, int H, int G, int d, float sm_scale, float softcap, const float* slopes,
+                                 const int32_t* prefix, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  using namespace fm;
+  FM_REQUIRE(n_pages >= 1 && rows >= 1 && width >= 1 && H >= 1 && G >= 1 && d >= 1 && d <= FM_MAX_D && T >= 0 && max_new >= 0,
+             FM_ERR_ARG, "fm_paged_attn_fwd: n_pages=%d rows=%d width=%d H=%d G=%d d=%d T=%d max_new=%d", n_pages, rows, width, H,
+             G, d, T, max_new);
+  FM_REQUIRE(page <= FM_CACHE_MAX_PAGE && log2_exact(page) >= 0, FM_ERR_ARG,
+             "fm_paged_attn_fwd: page size %d is no power of two up to %d", page, FM_CACHE_MAX_PAGE);
+  FM_REQUIRE(dtype_ok(dtype), FM_ERR_ARG, "fm_paged_attn_fwd: dtype=%d", dtype);
+  FM_REQUIRE(sm_scale > 0.f && isfinite(sm_scale) && cap_ok(sm_scale, softcap), FM_ERR_ARG,
+             "fm_paged_attn_fwd: sm_scale=%g softcap=%g", double(sm_scale), double(softcap));
+  FM_REQUIRE(int64_t(H) * G <= 65535 && int64_t(T) * H * G <= 0x7fffffffLL && rows <= (1 << 24) &&
+                 (int64_t(width) * page) <= (1 << 24),
+             FM_ERR_UNSUPPORTED, "fm_paged_attn_fwd: T=%d H*G=%lld rows=%d width*page=%lld", T, (long long)H * G, rows,
+             (long long)width * page);
+  if (T == 0) return FM_OK;
+  FM_REQUIRE(q && k_pages && v_pages && book && cu && out && lse && ws, FM_ERR_ARG, "fm_paged_attn_fwd: null pointer");
+  const size_t need = fm_paged_attn_fwd_workspace(rows, T, max_new, H, G, d, width, page, dtype);
+  FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_paged_attn_fwd: workspace %zu < %zu", ws_bytes, need);
+  const PagedArgs a{q, q_token, q_head, k_pages, v_pages, book, n_pages, rows, width, page, log2_exact(page), cu, out, out_token,
+                    out_head, lse, lse_token, lse_head, T, H, G, d, sm_scale, softcap, slopes, prefix, dtype};
+  return by_type<PagedRows>(dtype, a, as_stream(stream));
+}

@@ -379,17 +379,35 @@ class Memory:
         return ops.hash_attn_bwd(q, self.keys, self.values, lists, self.bucket_off, self.bucket_cnt, groups, *args)
 
     def attend_with_local(self, q: torch.Tensor, k_local: torch.Tensor, v_local: torch.Tensor,
-                          sm_scale: float, n_groups: int, causal: bool = True):
+                          sm_scale: float, n_groups: int, causal: bool = True,
+                          terms: Optional["ops.ScoreTerms"] = None):
         """Memory attention LSE-merged with dense attention over local keys
         (memory.py:302-305, 319-332).  q ``[H,G*S,d]`` with ``G = n_groups``;
         k_local, v_local ``[H,L,d]``.  Returns fp32 ``(out [H,G*S,d], lse
-        [H,G*S])``."""
+        [H,G*S])``.  ``terms`` (:class:`ops.ScoreTerms`) are the local part's; the memory's scores have none."""
         H, Sq, d = q.shape
         S = Sq // n_groups
         q = q.contiguous()
-        lo, ll = ops.local_attn_fwd(q.reshape(H * n_groups, S, d), k_local.contiguous(),
-                                    v_local.contiguous(), sm_scale, causal)
+        local = (q.reshape(H * n_groups, S, d), k_local.contiguous(), v_local.contiguous(), sm_scale, causal)
+        lo, ll = ops.local_attn_fwd(*local) if terms is None else ops.local_attn_terms_fwd(*local, terms)
         out, lse = update_out_and_lse(None, None, lo.reshape(H, Sq, d), ll.reshape(H, Sq))
+        mo, ml = self.attend(q, sm_scale)
+        out, lse = update_out_and_lse(out.contiguous(), lse.contiguous(), mo, ml)
+        return out, lse.squeeze(-1)
+
+    def attend_with_cache(self, q: torch.Tensor, cache, row: int, sm_scale: float, n_groups: int,
+                          terms: Optional["ops.ScoreTerms"] = None):
+        """:meth:`attend_with_local` with the local keys in row ``row`` of a :class:`PagedCache`, whose last S tokens
+        are those of ``q [H,G*S,d]`` (append them first).  Returns fp32 ``(out [H,G*S,d], lse [H,G*S])``."""
+        H, Sq, d = q.shape
+        S = Sq // n_groups
+        if not 0 <= row < cache.n_rows:
+            raise ValueError(f"attend_with_cache: row {row} of {cache.n_rows}")
+        q = q.contiguous()
+        cu = torch.zeros(cache.n_rows + 1, dtype=torch.int32, device=q.device)
+        cu[row + 1:] = S
+        lo, ll = cache.attend(q.reshape(H * n_groups, S, d).transpose(0, 1), cu, sm_scale, terms, S)
+        out, lse = update_out_and_lse(None, None, lo.transpose(0, 1).reshape(H, Sq, d), ll.t().reshape(H, Sq))
         mo, ml = self.attend(q, sm_scale)
         out, lse = update_out_and_lse(out.contiguous(), lse.contiguous(), mo, ml)
         return out, lse.squeeze(-1)
@@ -446,6 +464,20 @@ class MemoryBatch:
         lo, ll = ops.local_attn_fwd(q.reshape(n_seq * H * G, 1, d).contiguous(),
                                     k_local.reshape(n_seq * H, L, d).contiguous(),
                                     v_local.reshape(n_seq * H, L, d).contiguous(), sm_scale, True)
+        out, lse = update_out_and_lse(None, None, lo.reshape(n_seq, H, G, d), ll.reshape(n_seq, H, G))
+        out, lse = update_out_and_lse(out.contiguous(), lse.contiguous(), mo, ml)
+        return out, lse.squeeze(-1)
+
+    def attend_with_cache(self, q, cache, sm_scale: float, terms: Optional["ops.ScoreTerms"] = None):
+        """:meth:`attend_with_local` with sequence i's local keys in row i of a :class:`PagedCache` of ``n_seq`` rows,
+        each row's last token being the query's own (append it first)."""
+        n_seq, H, G, d = q.shape
+        if cache.n_rows != n_seq or cache.n_heads != H:
+            raise ValueError(f"attend_with_cache: {n_seq} sequences and {H} heads, the cache has {cache.n_rows} rows and "
+                             f"{cache.n_heads} heads")
+        mo, ml, _ = self.attend(q, sm_scale)
+        cu = torch.arange(n_seq + 1, dtype=torch.int32, device=q.device)
+        lo, ll = cache.attend(q.reshape(n_seq, H * G, d), cu, sm_scale, terms, 1)
         out, lse = update_out_and_lse(None, None, lo.reshape(n_seq, H, G, d), ll.reshape(n_seq, H, G))
         out, lse = update_out_and_lse(out.contiguous(), lse.contiguous(), mo, ml)
         return out, lse.squeeze(-1)

@@ -527,6 +527,204 @@ def local_attn_fwd(q, k, v, sm_scale: float, causal: bool = True):
     return out, lse
 
 
+# --------------------------------------------------------------------- local keys in pages
+def _same_device(*ts) -> None:
+    dev = ts[0].device
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+
+
+def _call(fn, like: torch.Tensor, *args) -> None:
+    """One C call on the current stream of ``like``'s device, which need not be the current device."""
+    if like.device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(like.device):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+
+
+def _row_ints(t: torch.Tensor, n: int, like: torch.Tensor, what: str) -> torch.Tensor:
+    """An int32 vector of n entries on ``like``'s device (int64 is cast at the edge)."""
+    if t.shape != (n,) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: {n} integers, got {tuple(t.shape)} {t.dtype}")
+    _same_device(like, t)
+    return t.to(torch.int32).contiguous()
+
+
+def cache_append_(cache, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor) -> None:
+    """``PagedCache.append`` (fm_cache_append)."""
+    kp = cache.k_pages
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (cache.n_heads, cache.d) or k.dtype != kp.dtype or v.dtype != kp.dtype:
+        raise ValueError(f"append: k and v are [T, {cache.n_heads}, {cache.d}] {kp.dtype}, got {tuple(k.shape)} {k.dtype} and "
+                         f"{tuple(v.shape)} {v.dtype}")
+    _same_device(kp, k, v)
+    cu = _row_ints(cu, cache.n_rows + 1, kp, "append: cu")
+    k = k if k.stride(2) == 1 else k.contiguous()
+    v = v if v.stride(2) == 1 else v.contiguous()
+    ws = _ws(cache._ws_bytes, kp)
+    _call(_lib.load().fm_cache_append, kp, kp.data_ptr(), cache.v_pages.data_ptr(), cache.book.data_ptr(), cache.n_pages,
+          cache.n_rows, cache.width, cache.page_size, cache.n_heads, cache.d, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
+          v.stride(0), v.stride(1), cu.data_ptr(), k.shape[0], _DT[kp.dtype], ws.data_ptr(), ws.numel())
+
+
+def cache_fork_(cache, src: torch.Tensor) -> None:
+    """``PagedCache.fork`` (fm_cache_fork)."""
+    kp = cache.k_pages
+    src = _row_ints(src, cache.n_rows, kp, "fork: src")
+    ws = _ws(cache._ws_bytes, kp)
+    _call(_lib.load().fm_cache_fork, kp, kp.data_ptr(), cache.v_pages.data_ptr(), cache.book.data_ptr(), cache.n_pages, cache.n_rows,
+          cache.width, cache.page_size, cache.n_heads, cache.d, src.data_ptr(), _DT[kp.dtype], ws.data_ptr(), ws.numel())
+
+
+def cache_drop_(cache, pages: torch.Tensor) -> None:
+    """``PagedCache.drop`` (fm_cache_drop)."""
+    pages = _row_ints(pages, cache.n_rows, cache.k_pages, "drop: pages")
+    _call(_lib.load().fm_cache_drop, cache.k_pages, cache.book.data_ptr(), cache.n_pages, cache.n_rows, cache.width, cache.page_size,
+          pages.data_ptr())
+
+
+def cache_compact_(cache) -> None:
+    """``PagedCache.compact`` (fm_cache_compact)."""
+    kp = cache.k_pages
+    ws = _ws(cache._ws_bytes, kp)
+    _call(_lib.load().fm_cache_compact, kp, kp.data_ptr(), cache.v_pages.data_ptr(), cache.book.data_ptr(), cache.n_pages,
+          cache.n_rows, cache.width, cache.page_size, cache.n_heads, cache.d, _DT[kp.dtype], ws.data_ptr(), ws.numel())
+
+
+# --------------------------------------------------------------------- local attention with score terms
+class ScoreTerms(NamedTuple):
+    """What changes the scores ``x_ij = sm_scale q_i.k_j`` of the local attention, in this order:
+
+    * ``softcap`` c > 0: ``x <- c tanh(x / c)``;
+    * ``slopes [n_query_heads]`` fp32: ``x <- x - slope |distance|``, the distance counted with the last query on the
+      last key (``|i + (L - S) - j|``); constants, they receive no gradient;
+    * ``doc_q [S]``, ``doc_k [L]`` int: query i sees key j only where they are equal and not negative (a negative
+      document is padding: it sees nothing and nobody sees it);
+    * ``prefix [S]`` int: query i sees the keys ``j < prefix[i]`` whatever the causal mask says (of its own document,
+      where there are any).  Over a paged cache it is ``[n_rows]``, and a row is a document of its own.
+    """
+    softcap: float = 0.0
+    slopes: Optional[torch.Tensor] = None
+    doc_q: Optional[torch.Tensor] = None
+    doc_k: Optional[torch.Tensor] = None
+    prefix: Optional[torch.Tensor] = None
+
+
+_NO_TERMS = ScoreTerms()
+
+
+def _slopes(terms: ScoreTerms, HG: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    s = terms.slopes
+    if s is None:
+        return None
+    if s.shape != (HG,) or s.dtype != torch.float32:
+        raise ValueError(f"slopes: fp32 [{HG}], got {tuple(s.shape)} {s.dtype}")
+    if s.requires_grad:
+        raise ValueError("slopes receive no gradient: pass them detached")
+    _same_device(like, s)
+    return s.contiguous()
+
+
+def _terms_of(terms: Optional[ScoreTerms], q: torch.Tensor, L: int):
+    """The terms as the C entry points take them, and the tensors that have to live until the call has returned."""
+    t = _NO_TERMS if terms is None else terms
+    HG, S, _ = q.shape
+    slopes = _slopes(t, HG, q)
+    if (t.doc_q is None) != (t.doc_k is None):
+        raise ValueError("doc_q and doc_k come together")
+    doc_q = None if t.doc_q is None else _row_ints(t.doc_q, S, q, "doc_q")
+    doc_k = None if t.doc_k is None else _row_ints(t.doc_k, L, q, "doc_k")
+    prefix = None if t.prefix is None else _row_ints(t.prefix, S, q, "prefix")
+    return (float(t.softcap), _p(slopes), _p(doc_q), _p(doc_k), _p(prefix)), (slopes, doc_q, doc_k, prefix)
+
+
+def _local_shapes(q, k, v):
+    _dev(q, k, v)
+    _same_device(q, k, v)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q [H*G,S,d] and k, v [H,L,d], got {tuple(q.shape)} and {tuple(k.shape)}")
+    HG, S, d = q.shape
+    H, L, _ = k.shape
+    if H == 0 or HG % H or k.shape != v.shape or k.shape[2] != d or not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"q [H*G,S,d] and k, v [H,L,d] of one type, got {tuple(q.shape)} {q.dtype}, {tuple(k.shape)} {k.dtype}, "
+                         f"{tuple(v.shape)} {v.dtype}")
+    return H, HG // H, S, L, d
+
+
+def local_attn_terms_fwd(q, k, v, sm_scale: float, causal: bool = True, terms: Optional[ScoreTerms] = None):
+    """:func:`local_attn_fwd` with :class:`ScoreTerms`: q [H*G,S,d], k,v [H,L,d] -> (out, lse [H*G,S] fp32)."""
+    H, G, S, L, d = _local_shapes(q, k, v)
+    flat, keep = _terms_of(terms, q, L)
+    out = torch.empty_like(q)
+    lse = torch.empty((H * G, S), dtype=torch.float32, device=q.device)
+    lib, dt = _lib.load(), _dt(q)
+    ws = _ws(lib.fm_local_attn_terms_fwd_workspace(H, G, S, L, d, dt), q)
+    _call(lib.fm_local_attn_terms_fwd, q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *flat, H, G, S, L,
+          d, float(sm_scale), int(bool(causal)), dt, ws.data_ptr(), ws.numel())
+    return out, lse
+
+
+def local_attn_terms_bwd(dout, q, k, v, out, lse, sm_scale: float, causal: bool = True, terms: Optional[ScoreTerms] = None,
+                         dlse: Optional[torch.Tensor] = None):
+    """Backward of :func:`local_attn_terms_fwd`: ``(dq, dk, dv)`` in the inputs' type.  ``out`` / ``lse`` are the forward's
+    or the merged ones, ``dlse [H*G,S]`` (optional) the gradient w.r.t. the log-sum-exp."""
+    H, G, S, L, d = _local_shapes(q, k, v)
+    _dev(dout, out, lse)
+    _same_device(q, dout, out, lse, dlse)
+    if dout.shape != q.shape or out.shape != q.shape or lse.shape != q.shape[:2] or not (dout.dtype == out.dtype == q.dtype) \
+            or lse.dtype != torch.float32 or (dlse is not None and dlse.shape != lse.shape):
+        raise ValueError(f"dout and out are like q ({tuple(q.shape)} {q.dtype}), lse and dlse fp32 {tuple(q.shape[:2])}")
+    dlse = _check_dlse(dlse, lse)
+    flat, keep = _terms_of(terms, q, L)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    lib, dt = _lib.load(), _dt(q)
+    ws = _ws(lib.fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dt), q)
+    _call(lib.fm_local_attn_terms_bwd, q, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+          _p(dlse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *flat, H, G, S, L, d, float(sm_scale), int(bool(causal)), dt,
+          ws.data_ptr(), ws.numel())
+    return dq, dk, dv
+
+
+def paged_attn_fwd(q: torch.Tensor, cache, cu: torch.Tensor, sm_scale: float, terms: Optional[ScoreTerms] = None, max_new: int = 0):
+    """``PagedCache.attend`` (fm_paged_attn_fwd).  ``q`` may have any token and head strides (rows of d are dense); ``out``
+    and ``lse`` follow its order."""
+    kp = cache.k_pages
+    if q.dim() != 3 or q.shape[2] != cache.d or q.dtype != kp.dtype or q.shape[1] == 0 or q.shape[1] % cache.n_heads:
+        raise ValueError(f"attend: q is [T, {cache.n_heads} G, {cache.d}] {kp.dtype}, got {tuple(q.shape)} {q.dtype}")
+    if not q.is_cuda:
+        raise RuntimeError("libfastmem operators take GPU tensors only (there is no CPU path)")
+    _same_device(kp, q)
+    T, HG, d = q.shape
+    t = _NO_TERMS if terms is None else terms
+    if t.doc_q is not None or t.doc_k is not None:
+        raise ValueError("attend: a row of the cache is a document of its own; doc_q and doc_k do not apply")
+    slopes = _slopes(t, HG, kp)
+    prefix = None if t.prefix is None else _row_ints(t.prefix, cache.n_rows, kp, "prefix")
+    cu = _row_ints(cu, cache.n_rows + 1, kp, "attend: cu")
+    if int(max_new) < 0:
+        raise ValueError(f"attend: max_new={max_new}")
+    if q.stride(2) != 1 or (q.element_size() * q.stride(0)) % 16 or (q.element_size() * q.stride(1)) % 16 or q.data_ptr() % 16:
+        q = q.contiguous()
+    heads_first = T > 1 and q.stride(0) < q.stride(1)
+    if heads_first:
+        out = torch.empty((HG, T, d), dtype=q.dtype, device=q.device).transpose(0, 1)
+        lse = torch.empty((HG, T), dtype=torch.float32, device=q.device).t()
+    else:
+        out = torch.empty((T, HG, d), dtype=q.dtype, device=q.device)
+        lse = torch.empty((T, HG), dtype=torch.float32, device=q.device)
+    if T == 0:
+        return out, lse
+    lib, dt = _lib.load(), _dt(q)
+    G = HG // cache.n_heads
+    ws = _ws(lib.fm_paged_attn_fwd_workspace(cache.n_rows, T, int(max_new), cache.n_heads, G, d, cache.width, cache.page_size, dt), q)
+    _call(lib.fm_paged_attn_fwd, q, q.data_ptr(), q.stride(0), q.stride(1), kp.data_ptr(), cache.v_pages.data_ptr(),
+          cache.book.data_ptr(), cache.n_pages, cache.n_rows, cache.width, cache.page_size, cu.data_ptr(), out.data_ptr(),
+          out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0), lse.stride(1), T, int(max_new), cache.n_heads, G, d,
+          float(sm_scale), float(t.softcap), _p(slopes), _p(prefix), dt, ws.data_ptr(), ws.numel())
+    return out, lse
+
+
 # --------------------------------------------------------------------- a10
 def lse_merge_(out: torch.Tensor, lse: torch.Tensor, block_out: torch.Tensor, block_lse: torch.Tensor):
     """In-place merge of (block_out, block_lse) into the fp32 running pair (memory.py:54-71)."""

@@ -341,6 +341,105 @@ int fm_local_attn_fwd(const void* q, const void* k, const void* v, void* out, fl
                       int G, int S, int L, int d, float sm_scale, int causal, int dtype,
                       void* stream);
 
+/* ---- local keys in pages ------------------------------------------------------
+ * The reference's local keys are dense tensors of one forward (memory.py:302-304);
+ * these keep them from step to step for many sequences (no counterpart in the
+ * reference).  The pool is k_pages, v_pages [n_pages][H][page][d], `page` a power
+ * of two up to FM_CACHE_MAX_PAGE; `book` is one int32 array on the device of
+ * fm_cache_book_ints(n_pages, rows, width) words:
+ *   meta [FM_CACHE_META_INTS]   zeroed by the caller once; meta[0] counts the calls
+ *                               that were refused on the device, meta[1] names why
+ *                               the first was (fm_cache_reason); the rest is the
+ *                               library's
+ *   length [rows]               tokens of each row (sequence)
+ *   refs [n_pages]              rows that hold a page; 0 = free
+ *   table [rows][width]         pages of each row in order, -1 behind the last
+ * An empty cache is meta, length, refs = 0 and table = -1.  Nothing is read back:
+ * the calls record into a graph, and a request that cannot be met changes nothing
+ * but meta[0] and meta[1].  The calls of one cache follow each other on one stream
+ * (or are ordered by events).  Pages are handed out from the lowest free one up, to
+ * the requests in row order.  Workspace of append, fork and compact:
+ * fm_cache_workspace(n_pages, rows) bytes.
+ *   fm_cache_append   row r receives tokens cu[r] .. cu[r+1] of k_new, v_new (element
+ *                     strides k_token, k_head, ..; rows of d elements are dense);
+ *                     cu [rows+1] ascending from 0, cu[rows] <= T
+ *   fm_cache_fork     src [rows]: row r, which is empty, becomes a copy of row src[r]
+ *                     (< 0: left alone; a source is not itself forked into).  Whole
+ *                     pages are shared, a last partial page is copied
+ *   fm_cache_drop     n_drop [rows]: the first min(n_drop[r], all) pages of row r leave
+ *                     it (its oldest tokens, e.g. those the memory's index has taken
+ *                     over); <= 0: none; a large number empties the row.  A page
+ *                     nobody holds any more is free
+ *   fm_cache_compact  the used pages move to the front of the pool: the i-th free page
+ *                     below their number takes the i-th used one at or above it */
+#define FM_CACHE_META_INTS 16
+#define FM_CACHE_MAX_PAGE 4096
+typedef enum {
+  FM_CACHE_NO_PAGES = 1,   /* fewer free pages than the call needs                      */
+  FM_CACHE_ROW_FULL = 2,   /* a row would outgrow its table of `width` pages            */
+  FM_CACHE_BAD_REQUEST = 3 /* cu not ascending from 0 to T, or a fork into a row that
+                              holds tokens, from itself, from outside or from a target  */
+} fm_cache_reason;
+size_t fm_cache_book_ints(int n_pages, int rows, int width);
+size_t fm_cache_workspace(int n_pages, int rows);
+int fm_cache_append(void* k_pages, void* v_pages, int32_t* book, int n_pages, int rows, int width,
+                    int page, int H, int d, const void* k_new, const void* v_new, int64_t k_token,
+                    int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* cu, int T, int dtype,
+                    void* ws, size_t ws_bytes, void* stream);
+int fm_cache_fork(void* k_pages, void* v_pages, int32_t* book, int n_pages, int rows, int width,
+                  int page, int H, int d, const int32_t* src, int dtype, void* ws, size_t ws_bytes,
+                  void* stream);
+int fm_cache_drop(int32_t* book, int n_pages, int rows, int width, int page, const int32_t* n_drop,
+                  void* stream);
+int fm_cache_compact(void* k_pages, void* v_pages, int32_t* book, int n_pages, int rows, int width,
+                     int page, int H, int d, int dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- local attention with score terms -------------------------------------------
+ * fm_local_attn_fwd (the attention_forward call at memory.py:302) with
+ *   softcap c > 0     scores x become c tanh(x / c)      (0: none)
+ *   slopes [H*G]      then x_ij -= slope |i + (L - S) - j|, fp32 (NULL: none)
+ *   doc_q [S], doc_k [L]   query i sees only keys with doc_k[j] == doc_q[i] (NULL, NULL:
+ *                     all); a negative document is nobody's (padding): such a query
+ *                     sees nothing, such a key is seen by nobody
+ *   prefix [S]        query i sees keys j < prefix[i] whatever `causal` says (NULL: none)
+ * each on its own or together; sm_scale > 0.  A query that sees nothing gets out = 0,
+ * lse = -FLT_MAX.  What is not seen touches no result, NaN and infinities included.
+ * The backward takes the forward's out and lse (or the ones merged with the memory's:
+ * the gradients are then the local keys' share), dlse [H*G,S] fp32 or NULL, and writes
+ * dq, dk, dv in the inputs' type, each rounded once; the same bits every time.
+ * H*G <= 65535, S and L <= 2^24. */
+size_t fm_local_attn_terms_fwd_workspace(int H, int G, int S, int L, int d, int dtype);
+int fm_local_attn_terms_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                            float softcap, const float* slopes, const int32_t* doc_q,
+                            const int32_t* doc_k, const int32_t* prefix, int H, int G, int S, int L,
+                            int d, float sm_scale, int causal, int dtype, void* ws, size_t ws_bytes,
+                            void* stream);
+size_t fm_local_attn_terms_bwd_workspace(int H, int G, int S, int L, int d, int dtype);
+int fm_local_attn_terms_bwd(const void* q, const void* k, const void* v, const void* out,
+                            const float* lse, const void* dout, const float* dlse, void* dq, void* dk,
+                            void* dv, float softcap, const float* slopes, const int32_t* doc_q,
+                            const int32_t* doc_k, const int32_t* prefix, int H, int G, int S, int L,
+                            int d, float sm_scale, int causal, int dtype, void* ws, size_t ws_bytes,
+                            void* stream);
+
+/* ---- attention of new tokens over a paged cache -----------------------------------
+ * The new tokens of row r, which fm_cache_append has put at its end, are q[cu[r]] ..
+ * q[cu[r+1] - 1] (T of them in all; element strides q_token, q_head; head h*G + g reads
+ * KV head h).  A token sees the keys up to its own and, with prefix [rows], the first
+ * prefix[r] keys of its row; softcap and slopes [H*G] as above.  out and lse have strides
+ * of their own; lse is the natural-log LSE for fm_lse_merge with the memory's attention.
+ * A token of no row, or with nothing to see, gets out = 0, lse = -FLT_MAX.  Page numbers
+ * outside the pool are clamped into it, never dereferenced.  max_new: no row has more
+ * new tokens than that (it shapes the launch only; 0 = unknown).  width * page <= 2^24. */
+size_t fm_paged_attn_fwd_workspace(int rows, int T, int max_new, int H, int G, int d, int width,
+                                   int page, int dtype);
+int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head, const void* k_pages,
+                      const void* v_pages, const int32_t* book, int n_pages, int rows, int width,
+                      int page, const int32_t* cu, void* out, int64_t out_token, int64_t out_head,
+                      float* lse, int64_t lse_token, int64_t lse_head, int T, int max_new, int H, int G,
+                      int d, float sm_scale, float softcap, const float* slopes, const int32_t* prefix,
+                      int dtype, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- a10: LSE merge, in place on the running pair ---------------------------
  * update_out_and_lse (memory.py:54-71).  out [Q,d] fp32 and lse [Q] fp32 are
  * updated with block_out [Q,d] (dtype) and block_lse [Q] fp32. */

@@ -1,11 +1,38 @@
 // C entry points of the local attention with score terms and of the attention over a paged cache.
 #include <math.h>
 
-#include "terms_api.hpp"
+#include <initializer_list>
+
+#include "terms_fwd.hpp"
 
 namespace fm {
 
 extern std::atomic<int> g_force_generic;
+extern template int terms_fwd_tiles<64>(const FwdTileArgs&, bool, hipStream_t);
+extern template int terms_fwd_tiles<128>(const FwdTileArgs&, bool, hipStream_t);
+extern template int terms_fwd_tiles<256>(const FwdTileArgs&, bool, hipStream_t);
+
+static bool tiles_take(int d, int dtype) {
+  return g_force_generic != 1 && dtype != FM_F32 && (d == 64 || d == 128 || d == 256);
+}
+
+static int terms_fwd_run(const FwdArgs& a, void* ws, hipStream_t st) {
+  FwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (bf16_t*)a.out, a.lse, a.t, masks_layout(ws, a.S, a.L),
+                a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, 0.f, 0.f, a.sm_scale};
+  if (a.t.softcap > 0.f) {
+    const Score<true> s(a.sm_scale, a.t.softcap);
+    t.in = s.in, t.out_scale = s.out;
+  } else {
+    const Score<false> s(a.sm_scale, 0.f);
+    t.in = s.in, t.out_scale = s.out;
+  }
+  if (t.use_masks) {
+    const int rc = make_masks(t.m, a.t, a.S, a.L, st);
+    if (rc) return rc;
+  }
+  const bool f16 = a.dtype == FM_F16;
+  return a.d == 64 ? terms_fwd_tiles<64>(t, f16, st) : a.d == 128 ? terms_fwd_tiles<128>(t, f16, st) : terms_fwd_tiles<256>(t, f16, st);
+}
 
 static bool cap_ok(float sm_scale, float softcap) {
   return softcap == 0.f || (softcap > 0.f && isfinite(softcap * kLog2e) && isfinite(sm_scale / softcap));
@@ -47,6 +74,13 @@ struct PagedRows {
   static int run(const PagedArgs& a, hipStream_t st) { return paged_attn_rows<T>(a, st); }
 };
 
+// (the tiled kernels read rows of q, k, v in 16-byte pieces, 8 bytes at a time written)
+static bool aligned16(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  return true;
+}
+
 static size_t delta_bytes(int H, int G, int S) { return align_up(size_t(H) * G * S * 4, 256); }
 
 }  // namespace fm
@@ -54,7 +88,7 @@ static size_t delta_bytes(int H, int G, int S) { return align_up(size_t(H) * G *
 extern "C" size_t fm_local_attn_terms_fwd_workspace(int H, int G, int S, int L, int d, int dtype) {
   if (H < 1 || G < 1 || S < 1 || L < 1 || d < 1) return 0;
   (void)dtype;
-  return 256;
+  return fm::masks_layout(nullptr, S, L).bytes;
 }
 
 extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void* v, void* out, float* lse, float softcap,
@@ -68,6 +102,7 @@ extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void*
   const size_t need = fm_local_attn_terms_fwd_workspace(H, G, S, L, d, dtype);
   FM_REQUIRE(ws, FM_ERR_ARG, "fm_local_attn_terms_fwd: null pointer");
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_fwd: workspace %zu < %zu", ws_bytes, need);
+  if (tiles_take(d, dtype) && aligned16({q, k, v, out})) return terms_fwd_run(a, ws, as_stream(stream));
   return by_type<FwdRows>(dtype, a, as_stream(stream));
 }
 

@@ -1,0 +1,370 @@
+// The tiled forward of the attention with score terms (bf16 / fp16, head dimension 64, 128 or 256): 128 query rows per
+// workgroup, 32 per wave, over tiles of 64 keys.  The training forward (terms_fwd.hip) and the chunks over a paged cache
+// (paged_attn.hip) run it; they differ in where a key's row lies and in what a query row is.
+//
+//   S^T = K.Q^T   v_mfma_f32_32x32x16: A = 32 keys of the tile from LDS, B = this wave's queries, in registers for the
+//                 whole sweep.  Lane (query l % 32, half l / 32) ends up with the scores of keys 8 (r / 4) + 4 (l / 32) +
+//                 r % 4: a query is a lane column, its softmax statistics are plain registers and one exchange between
+//                 the halves per tile makes a maximum whole.
+//   O^T += V^T.P^T  same instruction.  Registers 8 s .. 8 s + 7 of a score block are the B operand of step s with the 16
+//                 keys of the step in the order 0-3, 8-11 | 4-7, 12-15, and ds_read_b64_tr_b16 reads V^T in just that
+//                 order out of row-major V: nothing is shuffled or transposed in registers.
+//
+// K and V go from global memory straight into LDS (global_load_lds_dwordx4, two tiles: one read, one on its way), a
+// 1 KiB block of whole rows per load.  16-byte chunk c of row r lies at position c ^ f(r): the lanes that read one chunk
+// of 16 rows (K) and the 4 rows x 64 bytes that half a wave reads of V then hit every bank once.
+//
+// Masks cost only the tiles that have masked places: the others (keys that all queries of a wave see) run without a
+// compare.  Where a tile does have masked places and its values hold a NaN or an infinity, the product 0 x NaN would
+// reach queries that do not see the row: the workgroup notes it and, after the sweep, does its rows again a row at a
+// time (terms.hpp), which visits only what is seen.
+#pragma once
+#include "attn_ring.hpp"
+#include "mma16.hpp"
+#include "terms_api.hpp"
+
+namespace fm {
+
+constexpr int kTQ = 128;  // query rows of a workgroup
+constexpr int kTK = 64;   // keys of a tile
+
+// what the scores have, beside the product: bit 0 the cap, bit 1 the distance bias
+constexpr int kModeCap = 1, kModeBias = 2;
+
+template <int D>
+__device__ __forceinline__ constexpr int tile_swz(int r) {
+  if constexpr (D == 64)
+    return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);  // 8 chunks a row, two rows span the banks
+  else
+    return ((r & 3) << 2) | ((r >> 2) & 3);  // (head dimension 256: among 16 of the 32 chunks)
+}
+
+// 16-bit values that are infinite or NaN: any in the 8 of a register quad
+template <bool F16>
+__device__ __forceinline__ bool any_nonfinite(const uint4& x) {
+  constexpr uint32_t e = F16 ? 0x7c007c00u : 0x7f807f80u, one = F16 ? 0x04000400u : 0x00800080u;
+  const uint32_t a = ((x.x & e) + one) | ((x.y & e) + one) | ((x.z & e) + one) | ((x.w & e) + one);
+  return (a & 0x80008000u) != 0;  // an exponent of all ones carries into the (masked) sign
+}
+
+// One direct load: lane i's 16 bytes from base + voff to LDS byte `lds_addr` + 16 i (both wave-uniform)
+__device__ __forceinline__ void tile_load(uint32_t lds_addr, uint32_t voff, const void* base) { ring_load16(lds_addr, voff, base); }
+
+__device__ __forceinline__ uint4 lds_read16(const lds_char_t* p) {
+  const ring_u32x4 a = *reinterpret_cast<const __attribute__((address_space(3))) ring_u32x4*>(p);
+  return make_uint4(a[0], a[1], a[2], a[3]);
+}
+__device__ __forceinline__ ring_short4 lds_read_tr(const lds_char_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ring_short4*)p);
+}
+__device__ __forceinline__ uint4 tr_pair(const lds_char_t* p, const lds_char_t* q) {
+  union {
+    ring_short4 s[2];
+    uint4 u;
+  } a;
+  a.s[0] = lds_read_tr(p);
+  a.s[1] = lds_read_tr(q);
+  return a.u;
+}
+
+// LDS of one tile of ROWS rows: where a wave's lanes load, and where the operands are read
+template <int D, int ROWS = kTK>
+struct TileLds {
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kBytes = ROWS * kRowBytes;
+  static constexpr int kRowsPerLoad = 1024 / kRowBytes;         // whole rows in a load of 1 KiB
+  static constexpr int kLoads = kBytes / 1024;                   // loads of a tile ..
+  static constexpr int kLoadsPerWave = kLoads / 4;               // .. and of a wave's share: loads w, w + 4, ..
+  // the row of load i this lane fills, and the byte offset in that row it asks global memory for
+  __device__ static __forceinline__ int load_row(int i, int lane) { return i * kRowsPerLoad + lane / (D / 8); }
+  __device__ static __forceinline__ uint32_t load_chunk(int row, int lane) {
+    return uint32_t((lane % (D / 8)) ^ tile_swz<D>(row)) << 4;
+  }
+  // operand of 32 consecutive rows (row = l % 32), contraction step ks: 8 elements from 16 ks + 8 (l / 32)
+  __device__ static __forceinline__ uint4 rows32(const lds_char_t* tile, int row0, int ks, int lane) {
+    const int row = row0 + (lane & 31);
+    return lds_read16(tile + row * kRowBytes + (((2 * ks + (lane >> 5)) ^ tile_swz<D>(row)) << 4));
+  }
+  // transposed operand: dimensions 32 dt + l % 32, contraction over the 16 rows from row0 in the order 0-3, 8-11 | 4-7, 12-15
+  __device__ static __forceinline__ uint4 cols32(const lds_char_t* tile, int row0, int dt, int lane) {
+    const int i = lane & 15, c = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    const int r = row0 + 4 * (lane >> 5) + (i >> 2);
+    const lds_char_t* p = tile + r * kRowBytes + ((c ^ tile_swz<D>(r)) << 4) + (i & 1) * 8;
+    const lds_char_t* q = tile + (r + 8) * kRowBytes + ((c ^ tile_swz<D>(r + 8)) << 4) + (i & 1) * 8;
+    return tr_pair(p, q);
+  }
+};
+
+// Scores of a block of 32 keys in base 2, in place: raw products in, x out (terms.hpp); with SLACK also 1 - tanh^2.
+// dist0 = pos - (first key of the block) - 4 (l / 32), slope2 = slope log2 e.  Register r is key 8 (r / 4) + r % 4 behind that.
+template <int MODE, bool SLACK>
+__device__ __forceinline__ void block_scores(float (&x)[16], float (&slack)[16], float in, float out, float dist0, float slope2) {
+  if constexpr (MODE & kModeCap) {
+    float big = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] *= in;
+      big = fmaxf(big, fabsf(x[r]));
+    }
+    if (__any(!(big <= kTanhSmall))) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = fabsf(x[r]) <= kTanhSmall ? tanh_small(x[r]) : tanh_large(x[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = tanh_small(x[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (SLACK) slack[r] = fmaf(-x[r], x[r], 1.f);
+      if constexpr (MODE & kModeBias)
+        x[r] = fmaf(-slope2, fabsf(dist0 - float(8 * (r >> 2) + (r & 3))), out * x[r]);
+      else
+        x[r] *= out;
+    }
+  } else if constexpr (MODE & kModeBias) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = fmaf(-slope2, fabsf(dist0 - float(8 * (r >> 2) + (r & 3))), x[r] * in);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= in;
+  }
+}
+
+}  // namespace fm
+
+namespace fm {
+
+// ---- where the rows of a tile lie ------------------------------------------------------------------------
+// contiguous [n][D]: rows behind the last repeat it (their scores are masked)
+template <int D>
+struct FlatSource {
+  const bf16_t *k, *v;
+  int n;
+  __device__ __forceinline__ void prefetch(int) {}
+  __device__ __forceinline__ void issue(int t, uint32_t lds_k, uint32_t lds_v, int w, int lane) const {
+    typedef TileLds<D> T;
+    const int kp0 = t * kTK;
+    const int64_t off = int64_t(kp0) * D;
+    const bf16_t* bk = ring_uniform_ptr(k + off);
+    const bf16_t* bv = ring_uniform_ptr(v + off);
+    const int last = n - 1 - kp0;
+#pragma unroll
+    for (int u = 0; u < T::kLoadsPerWave; ++u) {
+      const int row = T::load_row(w + 4 * u, lane);
+      const uint32_t voff = uint32_t(min(row, last)) * T::kRowBytes + T::load_chunk(row, lane);
+      tile_load(lds_k + uint32_t(w + 4 * u) * 1024u, voff, bk);
+    }
+#pragma unroll
+    for (int u = 0; u < T::kLoadsPerWave; ++u) {
+      const int row = T::load_row(w + 4 * u, lane);
+      const uint32_t voff = uint32_t(min(row, last)) * T::kRowBytes + T::load_chunk(row, lane);
+      tile_load(lds_v + uint32_t(w + 4 * u) * 1024u, voff, bv);
+    }
+  }
+};
+
+// What a lane's query sees, in the tile's terms.
+struct TileQuery {
+  int pos, lim, doc;   // doc: -1 sees nothing (only read where there are documents)
+  float slope2;
+};
+
+// The sweep of a workgroup: tiles [t_begin, t_end) of the keys, this lane's query `qy` (column l % 32 of wave w).
+//   lim_lo, lim_hi   fewest and most keys a query of this wave sees; wg_lo: fewest of the workgroup
+//   docs             null, or the documents of the keys (padded to whole tiles, negative: -2) and their {min, max} a tile
+//   q_doc            {min, max} document of the wave's queries, wg_doc of the workgroup's
+struct TileDocs {
+  const int32_t* dock;
+  const int2* kmeta;
+  int2 q_doc, wg_doc;
+};
+
+struct TileState {
+  float m, l;
+};
+
+template <bool F16, int D, int MODE, class Source>
+__device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16], const TileQuery& qy, int lim_lo, int lim_hi,
+                                           int wg_lo, int t_begin, int t_end, const TileDocs& docs, float in, float out_scale,
+                                           lds_char_t* lds, int* dirty_flag, typename Mma<F16>::f16v (&O)[D / 32], TileState& st) {
+  typedef TileLds<D> T;
+  using M = Mma<F16>;
+  constexpr int NKS = D / 16, NDT = D / 32;
+  constexpr float kLazyGrow = 8.f;  // growth of a running maximum (in powers of two) that is left unfollowed
+  const int tid = threadIdx.x, l = tid & 63, hb = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds)));
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
+  st.m = -INFINITY;
+  st.l = 0.f;
+  bool dirty = false;
+  const bool has_docs = docs.dock != nullptr;
+
+  // the next tile at or behind t that some query of the workgroup sees a document of
+  int mask_at = -64;
+  unsigned long long mask = 0;
+  auto next = [&](int t) {
+    if (!has_docs) return t;
+    while (t < t_end) {
+      if (t >= mask_at + 64 || mask_at < 0) {
+        mask_at = t;
+        const int tt = t + l;
+        bool hit = false;
+        if (tt < t_end) {
+          const int2 km = docs.kmeta[tt];
+          hit = km.y >= docs.wg_doc.x && km.x <= docs.wg_doc.y && km.y >= 0;
+        }
+        mask = __ballot(hit);
+      }
+      const unsigned long long m = mask >> (t - mask_at);
+      if (m) return t + __ffsll(m) - 1;
+      t = mask_at + 64;
+    }
+    return t_end;
+  };
+
+  auto compute = [&](int t, const lds_char_t* bK, const lds_char_t* bV) {
+    const int kp0 = t * kTK;
+    if (kp0 >= lim_hi) return;
+    bool masked = kp0 + kTK > lim_lo;
+    if (has_docs) {
+      const int2 km = docs.kmeta[t];
+      if (km.y < docs.q_doc.x || km.x > docs.q_doc.y) return;
+      masked |= km.x != km.y || docs.q_doc.x != docs.q_doc.y;
+    }
+    typename M::f16v s[2];
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[sb][r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb) s[sb] = M::m32(T::rows32(bK, 32 * sb, ks, l), qf[ks], s[sb]);
+    float x[2][16], none[16];
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[sb][r] = s[sb][r];
+      block_scores<MODE, false>(x[sb], none, in, out_scale, float(qy.pos - (kp0 + 32 * sb + 4 * hb)), qy.slope2);
+    }
+    if (masked) {
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int key0 = kp0 + 32 * sb + 8 * r4 + 4 * hb;
+          int4 dk = make_int4(0, 0, 0, 0);
+          if (has_docs) dk = *reinterpret_cast<const int4*>(docs.dock + key0);
+          const int dd[4] = {dk.x, dk.y, dk.z, dk.w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            bool ok = key0 + r < qy.lim;
+            if (has_docs) ok = ok && dd[r] == qy.doc;
+            if (!ok) x[sb][4 * r4 + r] = -INFINITY;
+          }
+        }
+    }
+    float mx = x[0][0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[0][r]);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[1][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    // The running maximum follows only when some query's grew by more than 2^kLazyGrow (or it sees its first key): until
+    // then p stays below 2^kLazyGrow against the older maximum, which neither the fp32 sums nor the relative rounding
+    // of p notice, and the accumulator's multiplications are spared in most tiles.
+    const float m_new = fmaxf(st.m, mx);
+    if (__any(m_new > st.m + kLazyGrow)) {
+      const float m_to = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(st.m - m_to);
+      st.l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
+      st.m = m_new;
+    }
+    const float m_sub = st.m == -INFINITY ? 0.f : st.m;
+    uint4 pf[2][2];
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        x[sb][r] = __builtin_amdgcn_exp2f(x[sb][r] - m_sub);
+        st.l += x[sb][r];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        pf[sb][h] = make_uint4(M::pack2(x[sb][8 * h + 0], x[sb][8 * h + 1]), M::pack2(x[sb][8 * h + 2], x[sb][8 * h + 3]),
+                               M::pack2(x[sb][8 * h + 4], x[sb][8 * h + 5]), M::pack2(x[sb][8 * h + 6], x[sb][8 * h + 7]));
+    }
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bV, 32 * sb + 16 * h, dt, l), pf[sb][h], O[dt]);
+  };
+
+  int t = next(t_begin);
+  if (t < t_end) {
+    src.prefetch(t);
+    src.issue(t, lds0, lds0 + T::kBytes, w, l);
+  }
+  int par = 0;
+  while (t < t_end) {
+    const int t_next = next(t + 1);
+    if (t_next < t_end) src.prefetch(t_next);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    ring_barrier();  // tile t is in place, and every wave has finished the tile before it, whose buffer is free
+    if (t_next < t_end) {
+      const uint32_t to = lds0 + uint32_t(par ^ 1) * 2u * T::kBytes;
+      src.issue(t_next, to, to + T::kBytes, w, l);
+    }
+    const lds_char_t* bK = lds + par * 2 * T::kBytes;
+    const lds_char_t* bV = bK + T::kBytes;
+    // masked places for some query of the workgroup: are there values that 0 x would not erase?
+    bool wg_masked = t * kTK + kTK > wg_lo;
+    if (has_docs) {
+      const int2 km = docs.kmeta[t];
+      wg_masked |= km.x != km.y || docs.wg_doc.x != docs.wg_doc.y;
+    }
+    if (wg_masked) {
+#pragma unroll
+      for (int u = 0; u < T::kBytes / 4096; ++u) dirty |= any_nonfinite<F16>(lds_read16(bV + (u * 256 + tid) * 16));
+    }
+    compute(t, bK, bV);
+    t = t_next;
+    par ^= 1;
+  }
+  if (dirty) *dirty_flag = 1;  // (every writer writes the same)
+  __syncthreads();
+  return *dirty_flag != 0;
+}
+
+// This lane's share of a finished query: dimensions 32 dt + 8 (r / 4) + 4 (l / 32) + r % 4.
+template <bool F16, int D>
+__device__ __forceinline__ void tile_write(const typename Mma<F16>::f16v (&O)[D / 32], const TileState& st, bf16_t* out,
+                                           float* lse) {
+  const int hb = (threadIdx.x >> 5) & 1;
+  const float l = st.l + __shfl_xor(st.l, 32);
+  const bool none = st.m == -INFINITY && !(l > 0.f) && l == 0.f;
+  const float inv = none ? 0.f : 1.f / l;
+  if (!out) return;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      uint2 o;
+      o.x = Mma<F16>::pack2(O[dt][4 * rq + 0] * inv, O[dt][4 * rq + 1] * inv);
+      o.y = Mma<F16>::pack2(O[dt][4 * rq + 2] * inv, O[dt][4 * rq + 3] * inv);
+      *reinterpret_cast<uint2*>(out + dt * 32 + 8 * rq + 4 * hb) = o;
+    }
+  if (hb == 0) *lse = none ? -FLT_MAX : (st.m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+}  // namespace fm

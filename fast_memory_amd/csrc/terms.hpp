@@ -208,6 +208,48 @@ __device__ __forceinline__ void row_dq(const T* __restrict__ q, const T* __restr
     if (lane + 64 * r < d) Elem<T>::store(dq + lane + 64 * r, acc[r] * sm_scale);
 }
 
+// The share of 64 queries i0 .. of head hq in one key's gradients (not yet times sm_scale): lane = query, then dimension.
+struct KeyGrads {
+  float k[4], v[4];
+};
+__device__ __forceinline__ void key_grads_zero(KeyGrads& g) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) g.k[r] = 0.f, g.v[r] = 0.f;
+}
+template <typename T, bool CAP>
+__device__ __forceinline__ void row_dkv_chunk(const T* __restrict__ k, const T* __restrict__ v, int j, int hq, int i0, int S, int L,
+                                              int d, const T* __restrict__ q, const T* __restrict__ dout,
+                                              const float* __restrict__ lse, const float* __restrict__ delta, const Terms& t,
+                                              const Score<CAP>& score, KeyGrads& a) {
+  const int lane = lane_id(), i = i0 + lane;
+  bool ok = false;
+  float p = 0.f, gr = 0.f;
+  if (i < S) {
+    const QueryView qv = query_view(t, i, S, L, hq);
+    ok = qv.sees(j, t.doc_k);
+    if (ok) {
+      const int64_t row = int64_t(hq) * S + i;
+      float slack;
+      const float x = fmaf(-qv.slope2, fabsf(float(qv.pos - j)), score(row_dot(q + row * d, k, d), slack));
+      p = __builtin_amdgcn_exp2f(x - lse[row] * kLog2e);
+      gr = p * (row_dot(dout + row * d, v, d) - delta[row]) * slack;
+    }
+  }
+  unsigned long long seen = __ballot(ok);
+  while (seen) {
+    const int u = __ffsll(seen) - 1;
+    seen &= seen - 1;
+    const float pu = __shfl(p, u), gu = __shfl(gr, u);
+    const int64_t row = (int64_t(hq) * S + i0 + u) * d;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (lane + 64 * r < d) {
+        a.k[r] = fmaf(gu, Elem<T>::load(q + row + lane + 64 * r), a.k[r]);
+        a.v[r] = fmaf(pu, Elem<T>::load(dout + row + lane + 64 * r), a.v[r]);
+      }
+  }
+}
+
 // dk and dv of one key: all queries of the G heads that read it, in order
 template <typename T, bool CAP>
 __device__ __forceinline__ void row_dkv(const T* __restrict__ k, const T* __restrict__ v, int j, int hk, int G, int S, int L,
@@ -215,44 +257,16 @@ __device__ __forceinline__ void row_dkv(const T* __restrict__ k, const T* __rest
                                         const float* __restrict__ lse, const float* __restrict__ delta, const Terms& t,
                                         float sm_scale, const Score<CAP>& score, T* __restrict__ dk, T* __restrict__ dv) {
   const int lane = lane_id();
-  float ak[4] = {0.f, 0.f, 0.f, 0.f}, av[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int g = 0; g < G; ++g) {
-    const int hq = hk * G + g;
-    for (int ib = 0; ib < S; ib += kWave) {
-      const int i = ib + lane;
-      bool ok = false;
-      float p = 0.f, gr = 0.f;
-      if (i < S) {
-        const QueryView qv = query_view(t, i, S, L, hq);
-        ok = qv.sees(j, t.doc_k);
-        if (ok) {
-          const int64_t row = int64_t(hq) * S + i;
-          float slack;
-          const float x = fmaf(-qv.slope2, fabsf(float(qv.pos - j)), score(row_dot(q + row * d, k, d), slack));
-          p = __builtin_amdgcn_exp2f(x - lse[row] * kLog2e);
-          gr = p * (row_dot(dout + row * d, v, d) - delta[row]) * slack;
-        }
-      }
-      unsigned long long seen = __ballot(ok);
-      while (seen) {
-        const int u = __ffsll(seen) - 1;
-        seen &= seen - 1;
-        const float pu = __shfl(p, u), gu = __shfl(gr, u);
-        const int64_t row = (int64_t(hq) * S + ib + u) * d;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (lane + 64 * r < d) {
-            ak[r] = fmaf(gu, Elem<T>::load(q + row + lane + 64 * r), ak[r]);
-            av[r] = fmaf(pu, Elem<T>::load(dout + row + lane + 64 * r), av[r]);
-          }
-      }
-    }
-  }
+  KeyGrads a;
+  key_grads_zero(a);
+  for (int g = 0; g < G; ++g)
+    for (int ib = 0; ib < S; ib += kWave)
+      row_dkv_chunk<T, CAP>(k, v, j, hk * G + g, ib, S, L, d, q, dout, lse, delta, t, score, a);
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (lane + 64 * r < d) {
-      Elem<T>::store(dk + lane + 64 * r, ak[r] * sm_scale);
-      Elem<T>::store(dv + lane + 64 * r, av[r]);
+      Elem<T>::store(dk + lane + 64 * r, a.k[r] * sm_scale);
+      Elem<T>::store(dv + lane + 64 * r, a.v[r]);
     }
 }
 

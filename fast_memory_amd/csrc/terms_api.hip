@@ -1,8 +1,10 @@
 // C entry points of the local attention with score terms and of the attention over a paged cache.
 #include <math.h>
 
+#include <algorithm>
 #include <initializer_list>
 
+#include "terms_bwd.hpp"
 #include "terms_fwd.hpp"
 
 namespace fm {
@@ -11,6 +13,10 @@ extern std::atomic<int> g_force_generic;
 extern template int terms_fwd_tiles<64>(const FwdTileArgs&, bool, hipStream_t);
 extern template int terms_fwd_tiles<128>(const FwdTileArgs&, bool, hipStream_t);
 extern template int terms_fwd_tiles<256>(const FwdTileArgs&, bool, hipStream_t);
+
+extern template int terms_bwd_tiles<64>(const BwdTileArgs&, bool, const void*, const float*, float*, float*, hipStream_t);
+extern template int terms_bwd_tiles<128>(const BwdTileArgs&, bool, const void*, const float*, float*, float*, hipStream_t);
+extern template int terms_bwd_tiles<256>(const BwdTileArgs&, bool, const void*, const float*, float*, float*, hipStream_t);
 
 static bool tiles_take(int d, int dtype) {
   return g_force_generic != 1 && dtype != FM_F32 && (d == 64 || d == 128 || d == 256);
@@ -83,6 +89,57 @@ static bool aligned16(std::initializer_list<const void*> ptrs) {
 
 static size_t delta_bytes(int H, int G, int S) { return align_up(size_t(H) * G * S * 4, 256); }
 
+// The workspace of a backward: D | masks | norms | partial sums.
+struct BwdLayout {
+  size_t masks, norms, part, total;
+  int n_q_norms, n_k_norms, splits;
+};
+
+// A workgroup of the dk / dv launch fills a compute unit, and under a causal mask the first keys' take up to twice the
+// average: the sweeps are cut until there are four workgroups a unit, or a piece would be less than four tiles.
+static int dkv_splits(int H, int G, int S, int L) {
+  const int64_t blocks = int64_t(H) * ceil_div(L, kDkvKeys), steps = int64_t(G) * ceil_div(S, kDkvQ);
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(1024, blocks), steps / 4), 16)));
+}
+
+static BwdLayout bwd_layout(int H, int G, int S, int L, int d, int dtype) {
+  BwdLayout b;
+  b.masks = delta_bytes(H, G, S);
+  b.norms = b.masks + masks_layout(nullptr, S, L).bytes;
+  b.n_q_norms = int(ceil_div(int64_t(H) * G * S, kNormRows));
+  b.n_k_norms = int(ceil_div(int64_t(H) * L, kNormRows));
+  b.part = b.norms + align_up(size_t(2 * b.n_q_norms + b.n_k_norms) * 4, 256);
+  b.splits = (dtype != FM_F32 && (d == 64 || d == 128 || d == 256)) ? dkv_splits(H, G, S, L) : 1;
+  b.total = b.part + (b.splits > 1 ? size_t(b.splits) * 2 * H * L * d * 4 : 0);
+  return b;
+}
+
+static int terms_bwd_run(const BwdArgs& b, void* ws, hipStream_t st) {
+  const FwdArgs& a = b.f;
+  const BwdLayout y = bwd_layout(a.H, a.G, a.S, a.L, a.d, a.dtype);
+  char* p = static_cast<char*>(ws);
+  float* delta = reinterpret_cast<float*>(p);
+  float* norms = reinterpret_cast<float*>(p + y.norms);
+  BwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (const bf16_t*)b.dout, a.lse, delta, norms, y.n_q_norms,
+                y.n_k_norms, (bf16_t*)b.dq, (bf16_t*)b.dk, (bf16_t*)b.dv, reinterpret_cast<float*>(p + y.part), a.t,
+                masks_layout(p + y.masks, a.S, a.L), a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, y.splits, 0.f, 0.f, a.sm_scale};
+  if (a.t.softcap > 0.f) {
+    const Score<true> s(a.sm_scale, a.t.softcap);
+    t.in = s.in, t.out_scale = s.out;
+  } else {
+    const Score<false> s(a.sm_scale, 0.f);
+    t.in = s.in, t.out_scale = s.out;
+  }
+  if (t.use_masks) {
+    const int rc = make_masks(t.m, a.t, a.S, a.L, st);
+    if (rc) return rc;
+  }
+  const bool f16 = a.dtype == FM_F16;
+  return a.d == 64    ? terms_bwd_tiles<64>(t, f16, a.out, b.dlse, delta, norms, st)
+         : a.d == 128 ? terms_bwd_tiles<128>(t, f16, a.out, b.dlse, delta, norms, st)
+                      : terms_bwd_tiles<256>(t, f16, a.out, b.dlse, delta, norms, st);
+}
+
 }  // namespace fm
 
 extern "C" size_t fm_local_attn_terms_fwd_workspace(int H, int G, int S, int L, int d, int dtype) {
@@ -108,8 +165,7 @@ extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void*
 
 extern "C" size_t fm_local_attn_terms_bwd_workspace(int H, int G, int S, int L, int d, int dtype) {
   if (H < 1 || G < 1 || S < 1 || L < 1 || d < 1) return 0;
-  (void)dtype;
-  return fm::delta_bytes(H, G, S);
+  return fm::bwd_layout(H, G, S, L, d, dtype).total;
 }
 
 extern "C" int fm_local_attn_terms_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
@@ -126,6 +182,7 @@ extern "C" int fm_local_attn_terms_bwd(const void* q, const void* k, const void*
   FM_REQUIRE(dout && dq && dk && dv && ws, FM_ERR_ARG, "fm_local_attn_terms_bwd: null pointer");
   const size_t need = fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dtype);
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_bwd: workspace %zu < %zu", ws_bytes, need);
+  if (tiles_take(d, dtype) && aligned16({q, k, v, out, dout, dq, dk, dv, ws})) return terms_bwd_run(a, ws, as_stream(stream));
   return by_type<BwdRows>(dtype, a, static_cast<float*>(ws), as_stream(stream));
 }
 

@@ -1,0 +1,8 @@
+// Attention of new tokens over a paged cache at head dimension 256 (paged_attn.hpp).
+#include <algorithm>
+
+#include "paged_attn.hpp"
+
+namespace fm {
+template int paged_tiles<256>(const PagedTileArgs&, const PagedPlan&, int, hipStream_t);
+}  // namespace fm

@@ -174,14 +174,12 @@ __device__ __forceinline__ void row_write(const RowState& st, int d, T* __restri
   if (lane == 0) *lse = none ? -FLT_MAX : (st.m + __builtin_amdgcn_logf(st.l)) * kLn2;
 }
 
-// dq of one query
+// dq of one query; rd = {lse log2 e, D}
 template <typename T, bool CAP>
-__device__ __forceinline__ void row_dq(const T* __restrict__ q, const T* __restrict__ dout, float lse, float delta,
-                                       const KeyRows<T>& K, const KeyRows<T>& V, const QueryView& qv,
+__device__ __forceinline__ void row_dq(const T* __restrict__ q, const T* __restrict__ dout, float2 rd, const KeyRows<T>& K, const KeyRows<T>& V, const QueryView& qv,
                                        const int32_t* __restrict__ doc_k, float sm_scale, const Score<CAP>& score,
                                        T* __restrict__ dq) {
   const int lane = lane_id(), d = K.d;
-  const float lse2 = lse * kLog2e;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   for (int jb = 0; jb < qv.lim; jb += kWave) {
     const int j = jb + lane;
@@ -190,7 +188,7 @@ __device__ __forceinline__ void row_dq(const T* __restrict__ q, const T* __restr
     if (ok) {
       float slack;
       const float x = fmaf(-qv.slope2, fabsf(float(qv.pos - j)), score(row_dot(q, K.row(j), d), slack));
-      g = __builtin_amdgcn_exp2f(x - lse2) * (row_dot(dout, V.row(j), d) - delta) * slack;
+      g = __builtin_amdgcn_exp2f(x - rd.x) * (row_dot(dout, V.row(j), d) - rd.y) * slack;
     }
     unsigned long long seen = __ballot(ok);
     while (seen) {
@@ -208,7 +206,7 @@ __device__ __forceinline__ void row_dq(const T* __restrict__ q, const T* __restr
     if (lane + 64 * r < d) Elem<T>::store(dq + lane + 64 * r, acc[r] * sm_scale);
 }
 
-// The share of 64 queries i0 .. of head hq in one key's gradients (not yet times sm_scale): lane = query, then dimension.
+// The share of the at most 64 queries [i0, i1) of head hq in one key's gradients (not yet times sm_scale): lane = query, then dimension.
 struct KeyGrads {
   float k[4], v[4];
 };
@@ -217,22 +215,22 @@ __device__ __forceinline__ void key_grads_zero(KeyGrads& g) {
   for (int r = 0; r < 4; ++r) g.k[r] = 0.f, g.v[r] = 0.f;
 }
 template <typename T, bool CAP>
-__device__ __forceinline__ void row_dkv_chunk(const T* __restrict__ k, const T* __restrict__ v, int j, int hq, int i0, int S, int L,
+__device__ __forceinline__ void row_dkv_chunk(const T* __restrict__ k, const T* __restrict__ v, int j, int hq, int i0, int i1, int S, int L,
                                               int d, const T* __restrict__ q, const T* __restrict__ dout,
-                                              const float* __restrict__ lse, const float* __restrict__ delta, const Terms& t,
-                                              const Score<CAP>& score, KeyGrads& a) {
+                                              const float2* __restrict__ rd, const Terms& t, const Score<CAP>& score,
+                                              KeyGrads& a) {
   const int lane = lane_id(), i = i0 + lane;
   bool ok = false;
   float p = 0.f, gr = 0.f;
-  if (i < S) {
+  if (i < i1) {
     const QueryView qv = query_view(t, i, S, L, hq);
     ok = qv.sees(j, t.doc_k);
     if (ok) {
       const int64_t row = int64_t(hq) * S + i;
       float slack;
       const float x = fmaf(-qv.slope2, fabsf(float(qv.pos - j)), score(row_dot(q + row * d, k, d), slack));
-      p = __builtin_amdgcn_exp2f(x - lse[row] * kLog2e);
-      gr = p * (row_dot(dout + row * d, v, d) - delta[row]) * slack;
+      p = __builtin_amdgcn_exp2f(x - rd[row].x);
+      gr = p * (row_dot(dout + row * d, v, d) - rd[row].y) * slack;
     }
   }
   unsigned long long seen = __ballot(ok);
@@ -254,14 +252,14 @@ __device__ __forceinline__ void row_dkv_chunk(const T* __restrict__ k, const T* 
 template <typename T, bool CAP>
 __device__ __forceinline__ void row_dkv(const T* __restrict__ k, const T* __restrict__ v, int j, int hk, int G, int S, int L,
                                         int d, const T* __restrict__ q, const T* __restrict__ dout,
-                                        const float* __restrict__ lse, const float* __restrict__ delta, const Terms& t,
-                                        float sm_scale, const Score<CAP>& score, T* __restrict__ dk, T* __restrict__ dv) {
+                                        const float2* __restrict__ rd, const Terms& t, float sm_scale,
+                                        const Score<CAP>& score, T* __restrict__ dk, T* __restrict__ dv) {
   const int lane = lane_id();
   KeyGrads a;
   key_grads_zero(a);
   for (int g = 0; g < G; ++g)
     for (int ib = 0; ib < S; ib += kWave)
-      row_dkv_chunk<T, CAP>(k, v, j, hk * G + g, ib, S, L, d, q, dout, lse, delta, t, score, a);
+      row_dkv_chunk<T, CAP>(k, v, j, hk * G + g, ib, min(S, ib + kWave), S, L, d, q, dout, rd, t, score, a);
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (lane + 64 * r < d) {

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <initializer_list>
 
+#include "paged_attn.hpp"
 #include "terms_bwd.hpp"
 #include "terms_fwd.hpp"
 
@@ -14,9 +15,13 @@ extern template int terms_fwd_tiles<64>(const FwdTileArgs&, bool, hipStream_t);
 extern template int terms_fwd_tiles<128>(const FwdTileArgs&, bool, hipStream_t);
 extern template int terms_fwd_tiles<256>(const FwdTileArgs&, bool, hipStream_t);
 
-extern template int terms_bwd_tiles<64>(const BwdTileArgs&, bool, const void*, const float*, float*, float*, hipStream_t);
-extern template int terms_bwd_tiles<128>(const BwdTileArgs&, bool, const void*, const float*, float*, float*, hipStream_t);
-extern template int terms_bwd_tiles<256>(const BwdTileArgs&, bool, const void*, const float*, float*, float*, hipStream_t);
+extern template int terms_bwd_tiles<64>(const BwdTileArgs&, bool, const void*, const float*, const float*, float2*, float*, hipStream_t);
+extern template int terms_bwd_tiles<128>(const BwdTileArgs&, bool, const void*, const float*, const float*, float2*, float*, hipStream_t);
+extern template int terms_bwd_tiles<256>(const BwdTileArgs&, bool, const void*, const float*, const float*, float2*, float*, hipStream_t);
+
+extern template int paged_tiles<64>(const PagedTileArgs&, const PagedPlan&, int, hipStream_t);
+extern template int paged_tiles<128>(const PagedTileArgs&, const PagedPlan&, int, hipStream_t);
+extern template int paged_tiles<256>(const PagedTileArgs&, const PagedPlan&, int, hipStream_t);
 
 static bool tiles_take(int d, int dtype) {
   return g_force_generic != 1 && dtype != FM_F32 && (d == 64 || d == 128 || d == 256);
@@ -24,14 +29,7 @@ static bool tiles_take(int d, int dtype) {
 
 static int terms_fwd_run(const FwdArgs& a, void* ws, hipStream_t st) {
   FwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (bf16_t*)a.out, a.lse, a.t, masks_layout(ws, a.S, a.L),
-                a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, 0.f, 0.f, a.sm_scale};
-  if (a.t.softcap > 0.f) {
-    const Score<true> s(a.sm_scale, a.t.softcap);
-    t.in = s.in, t.out_scale = s.out;
-  } else {
-    const Score<false> s(a.sm_scale, 0.f);
-    t.in = s.in, t.out_scale = s.out;
-  }
+                a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, a.sm_scale, tile_score(a.sm_scale, a.t.softcap)};
   if (t.use_masks) {
     const int rc = make_masks(t.m, a.t, a.S, a.L, st);
     if (rc) return rc;
@@ -70,9 +68,9 @@ struct FwdRows {
 };
 template <typename T>
 struct BwdRows {
-  static int run(const BwdArgs& a, float* delta, hipStream_t st) {
-    int rc = terms_delta<T>(a, delta, st);
-    return rc ? rc : terms_bwd_rows<T>(a, delta, st);
+  static int run(const BwdArgs& a, float2* rd, hipStream_t st) {
+    int rc = terms_delta<T>(a, rd, st);
+    return rc ? rc : terms_bwd_rows<T>(a, rd, st);
   }
 };
 template <typename T>
@@ -87,9 +85,9 @@ static bool aligned16(std::initializer_list<const void*> ptrs) {
   return true;
 }
 
-static size_t delta_bytes(int H, int G, int S) { return align_up(size_t(H) * G * S * 4, 256); }
+static size_t row_data_bytes(int H, int G, int S) { return align_up(size_t(H) * G * S * 8, 256); }
 
-// The workspace of a backward: D | masks | norms | partial sums.
+// The workspace of a backward: {lse log2 e, D} | masks | norms | partial sums.
 struct BwdLayout {
   size_t masks, norms, part, total;
   int n_q_norms, n_k_norms, splits;
@@ -104,7 +102,7 @@ static int dkv_splits(int H, int G, int S, int L) {
 
 static BwdLayout bwd_layout(int H, int G, int S, int L, int d, int dtype) {
   BwdLayout b;
-  b.masks = delta_bytes(H, G, S);
+  b.masks = row_data_bytes(H, G, S);
   b.norms = b.masks + masks_layout(nullptr, S, L).bytes;
   b.n_q_norms = int(ceil_div(int64_t(H) * G * S, kNormRows));
   b.n_k_norms = int(ceil_div(int64_t(H) * L, kNormRows));
@@ -118,26 +116,20 @@ static int terms_bwd_run(const BwdArgs& b, void* ws, hipStream_t st) {
   const FwdArgs& a = b.f;
   const BwdLayout y = bwd_layout(a.H, a.G, a.S, a.L, a.d, a.dtype);
   char* p = static_cast<char*>(ws);
-  float* delta = reinterpret_cast<float*>(p);
+  float2* rd = reinterpret_cast<float2*>(p);
   float* norms = reinterpret_cast<float*>(p + y.norms);
-  BwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (const bf16_t*)b.dout, a.lse, delta, norms, y.n_q_norms,
+  BwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (const bf16_t*)b.dout, rd, norms, y.n_q_norms,
                 y.n_k_norms, (bf16_t*)b.dq, (bf16_t*)b.dk, (bf16_t*)b.dv, reinterpret_cast<float*>(p + y.part), a.t,
-                masks_layout(p + y.masks, a.S, a.L), a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, y.splits, 0.f, 0.f, a.sm_scale};
-  if (a.t.softcap > 0.f) {
-    const Score<true> s(a.sm_scale, a.t.softcap);
-    t.in = s.in, t.out_scale = s.out;
-  } else {
-    const Score<false> s(a.sm_scale, 0.f);
-    t.in = s.in, t.out_scale = s.out;
-  }
+                masks_layout(p + y.masks, a.S, a.L), a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, y.splits, a.sm_scale,
+                tile_score(a.sm_scale, a.t.softcap)};
   if (t.use_masks) {
     const int rc = make_masks(t.m, a.t, a.S, a.L, st);
     if (rc) return rc;
   }
   const bool f16 = a.dtype == FM_F16;
-  return a.d == 64    ? terms_bwd_tiles<64>(t, f16, a.out, b.dlse, delta, norms, st)
-         : a.d == 128 ? terms_bwd_tiles<128>(t, f16, a.out, b.dlse, delta, norms, st)
-                      : terms_bwd_tiles<256>(t, f16, a.out, b.dlse, delta, norms, st);
+  return a.d == 64    ? terms_bwd_tiles<64>(t, f16, a.out, a.lse, b.dlse, rd, norms, st)
+         : a.d == 128 ? terms_bwd_tiles<128>(t, f16, a.out, a.lse, b.dlse, rd, norms, st)
+                      : terms_bwd_tiles<256>(t, f16, a.out, a.lse, b.dlse, rd, norms, st);
 }
 
 }  // namespace fm
@@ -183,14 +175,13 @@ extern "C" int fm_local_attn_terms_bwd(const void* q, const void* k, const void*
   const size_t need = fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dtype);
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_bwd: workspace %zu < %zu", ws_bytes, need);
   if (tiles_take(d, dtype) && aligned16({q, k, v, out, dout, dq, dk, dv, ws})) return terms_bwd_run(a, ws, as_stream(stream));
-  return by_type<BwdRows>(dtype, a, static_cast<float*>(ws), as_stream(stream));
+  return by_type<BwdRows>(dtype, a, static_cast<float2*>(ws), as_stream(stream));
 }
 
 extern "C" size_t fm_paged_attn_fwd_workspace(int rows, int T, int max_new, int H, int G, int d, int width, int page, int dtype) {
   if (rows < 1 || T < 1 || H < 1 || G < 1 || d < 1 || width < 1 || page < 1) return 0;
-  (void)max_new;
-  (void)dtype;
-  return 256;
+  if (dtype == FM_F32) return 256;
+  return std::max<size_t>(256, fm::paged_plan(rows, T, max_new, H, G, d, int64_t(width) * page).total);
 }
 
 extern "C" int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head, const void* k_pages, const void* v_pages,
@@ -217,5 +208,17 @@ extern "C" int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head,
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_paged_attn_fwd: workspace %zu < %zu", ws_bytes, need);
   const PagedArgs a{q, q_token, q_head, k_pages, v_pages, book, n_pages, rows, width, page, log2_exact(page), cu, out, out_token,
                     out_head, lse, lse_token, lse_head, T, H, G, d, sm_scale, softcap, slopes, prefix, dtype};
+  const int64_t e = dtype_bytes(dtype);
+  if (tiles_take(d, dtype) && page >= 16 && aligned16({q, k_pages, v_pages, out, ws}) && q_token * e % 16 == 0 &&
+      q_head * e % 16 == 0 && out_token * e % 8 == 0 && out_head * e % 8 == 0) {
+    const PagedPlan y = paged_plan(rows, T, max_new, H, G, d, int64_t(width) * page);
+    const int64_t groups = int64_t(H) * std::max(int64_t(rows) * y.few_pieces, int64_t(y.slots) * y.many_pieces) + 4;
+    FM_REQUIRE(groups <= 0x7fffffffLL, FM_ERR_UNSUPPORTED, "fm_paged_attn_fwd: %lld workgroups", (long long)groups);
+    char* w = static_cast<char*>(ws);
+    const PagedTileArgs t{a, tile_score(sm_scale, softcap), y.few_rows, y.few_pieces, y.many_pieces, reinterpret_cast<float*>(w),
+                          reinterpret_cast<float2*>(w + y.part_ml), y.pieces, y.slots};
+    hipStream_t st = as_stream(stream);
+    return d == 64 ? paged_tiles<64>(t, y, max_new, st) : d == 128 ? paged_tiles<128>(t, y, max_new, st) : paged_tiles<256>(t, y, max_new, st);
+  }
   return by_type<PagedRows>(dtype, a, as_stream(stream));
 }

@@ -52,8 +52,8 @@ __device__ __forceinline__ PagedRow paged_row(const PagedArgs& a, int row) {
   const int64_t cap = int64_t(a.M) << a.log2p;
   p.row = row;
   p.len = int(min(int64_t(max(len[row], 0)), cap));
-  p.q0 = a.cu[row];
-  p.q1 = a.cu[row + 1];
+  p.q0 = min(max(a.cu[row], 0), a.T);
+  p.q1 = min(max(a.cu[row + 1], p.q0), a.T);
   p.table = len + a.R + a.n_pages + int64_t(row) * a.M;
   return p;
 }
@@ -73,8 +73,8 @@ __device__ __forceinline__ PagedRow paged_row_of_token(const PagedArgs& a, int t
 
 // terms_generic.hip
 template <typename T> int terms_fwd_rows(const FwdArgs& a, hipStream_t st);
-template <typename T> int terms_delta(const BwdArgs& a, float* delta, hipStream_t st);
-template <typename T> int terms_bwd_rows(const BwdArgs& a, const float* delta, hipStream_t st);
+template <typename T> int terms_delta(const BwdArgs& a, float2* rd, hipStream_t st);
+template <typename T> int terms_bwd_rows(const BwdArgs& a, const float2* rd, hipStream_t st);
 template <typename T> int paged_attn_rows(const PagedArgs& a, hipStream_t st);
 
 }  // namespace fm

@@ -4,7 +4,7 @@
 //   dq     a workgroup of 128 queries sweeps the keys as the forward does:  S^T = K.Q^T, dP^T = V.dO^T (queries and
 //          their dout in registers), g^T in place, dQ^T += K^T.g^T.
 //   dk dv  a workgroup of 128 keys (32 per wave, keys and values in registers) sweeps the queries of all heads of its
-//          group, 64 at a time:  S = Q.K^T, dP = dO.V^T, dV^T += dO^T.P, dK^T += Q^T.g.  A lane column is a key; its
+//          group, 32 at a time:  S = Q.K^T, dP = dO.V^T, dV^T += dO^T.P, dK^T += Q^T.g.  A lane column is a key; its
 //          16 rows are queries, whose lse, D and limits come through LDS.
 // The score registers of a block are again the operand of the second product (terms_tile.hpp), and Q^T, dO^T and K^T are
 // read out of the row-major tiles by ds_read_b64_tr_b16.
@@ -23,12 +23,14 @@
 
 namespace fm {
 
+typedef int lds_int2 __attribute__((ext_vector_type(2)));
+
 constexpr float kPScaleF16 = 4096.f;
 constexpr int kNormRows = 256;  // rows whose norms a workgroup of the first launch takes the largest of
 
 struct BwdTileArgs {
   const bf16_t *q, *k, *v, *dout;
-  const float *lse, *delta;
+  const float2* rd;    // {lse log2 e, D} of every query row
   const float* norms;  // {largest |do|, largest |D|} per kNormRows query rows, then the largest |v| per kNormRows keys
   int n_q_norms, n_k_norms;
   bf16_t *dq, *dk, *dv;
@@ -36,7 +38,8 @@ struct BwdTileArgs {
   Terms t;
   Masks m;
   int use_masks, H, G, S, L, splits;
-  float in, out_scale, sm_scale;
+  float sm_scale;
+  TileScore score;
 };
 
 // 2^e for the fp16 gradients of the call, the same in every workgroup
@@ -62,10 +65,11 @@ __device__ __forceinline__ float grad_scale(const BwdTileArgs& a, float* smem) {
 // D_i and, for fp16, the norms.  16 lanes a row, 4 rows a wave at a time; blocks behind the queries' take the values.
 template <bool F16, int D>
 __global__ __launch_bounds__(256) void terms_delta_tile_kernel(const bf16_t* __restrict__ out, const bf16_t* __restrict__ dout,
-                                                               const float* __restrict__ dlse, const bf16_t* __restrict__ v,
-                                                               float* __restrict__ delta, float* __restrict__ norms,
+                                                               const float* __restrict__ lse, const float* __restrict__ dlse,
+                                                               const bf16_t* __restrict__ v, float2* __restrict__ rd,
+                                                               float* __restrict__ norms,
                                                                int64_t rows, int64_t keys, int q_blocks, int S, int L,
-                                                               const int32_t* __restrict__ lim, const int32_t* __restrict__ dock) {
+                                                               const int2* __restrict__ qinfo, const int32_t* __restrict__ dock) {
   using M = Mma<F16>;
   __shared__ float s_d[4], s_D[4];
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63, part = l & 15;
@@ -102,12 +106,12 @@ __global__ __launch_bounds__(256) void terms_delta_tile_kernel(const bf16_t* __r
     }
     if (!is_v && row < n) {
       s -= dlse ? dlse[row] : 0.f;
-      if (part == 0) delta[row] = s;
+      if (part == 0) rd[row] = make_float2(lse[row] * kLog2e, s);
     }
     // (a row that is not finite has no finite gradients, and padding has none at all; the others' precision does not
     // depend on either)
     if constexpr (F16) {
-      const bool counts = row < n && (is_v ? !dock || dock[row % L] >= 0 : !lim || lim[row % S] > 0);
+      const bool counts = row < n && (is_v ? !dock || dock[row % L] >= 0 : !qinfo || qinfo[row % S].x > 0);
       if (counts && nn < INFINITY && fabsf(s) < INFINITY) big = fmaxf(big, nn), bigD = fmaxf(bigD, fabsf(s));
     }
   }
@@ -125,23 +129,66 @@ __global__ __launch_bounds__(256) void terms_delta_tile_kernel(const bf16_t* __r
   }
 }
 
-// 16 scores x (base 2), their products dP and derivatives of the cap in, p and g out
-template <bool F16, int MODE>
-__device__ __forceinline__ void block_grads(float (&x)[16], float (&dp)[16], const float (&slack)[16], int r, float lse2,
-                                            float delta, float g_scale) {
-  const float p = __builtin_amdgcn_exp2f(x[r] - lse2);
-  float g = p * (dp[r] - delta);
-  if constexpr (MODE & kModeCap) g *= slack[r];
-  if constexpr (F16) g *= g_scale;
-  x[r] = p;
-  dp[r] = g;
+// Raw products of a block of 32 x 32 in, p and p (1 - tanh^2) out.  lse2 is read per register (a query is a lane column in
+// the dq launch, a row in the dk / dv one); dist0 as for block_scores.
+template <int MODE, class Rows>
+__device__ __forceinline__ void block_probs(float (&x)[16], float (&y)[16], const TileScore& k, float dist0, float slope2,
+                                            const Rows& rows) {
+  auto dist = [&](int r) { return fabsf(dist0 - float(8 * (r >> 2) + (r & 3))); };
+  auto finish = [&](int r, float z, float slack) {  // z: the score before the bias
+    const float e = (MODE & kModeBias) ? fmaf(-slope2, dist(r), z) : z;
+    x[r] = __builtin_amdgcn_exp2f(e - rows.lse2(r));
+    y[r] = (MODE & kModeCap) ? x[r] * slack : x[r];
+  };
+  if constexpr (MODE & kModeCap) {
+    if (__any(!(abs_max16(x) <= k.zmax))) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float z = x[r] * k.in, t = fabsf(z) <= kTanhSmall ? tanh_small(z) : tanh_large(z);
+        finish(r, k.out * t, fmaf(-t, t, 1.f));
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float u = x[r] * k.in, z = u * capped_small(k, u);
+        finish(r, z, fmaf(z * k.k2, -z, 1.f));
+      }
+    }
+  } else if constexpr (MODE & kModeBias) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) finish(r, x[r] * k.in, 1.f);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[r] = x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], k.in, -rows.lse2(r)));
+  }
+}
+struct ColumnQuery {
+  float l;
+  __device__ __forceinline__ float lse2(int) const { return l; }
+};
+struct RowQueries {  // this lane's rows are queries 4 hb + 8 (r / 4) + r % 4 of the tile, 8 bytes each from `at`
+  const lds_char_t* at;
+  __device__ __forceinline__ uint4 pair(int r) const { return lds_read16(at + (8 * (r >> 2) + (r & 2)) * 8); }
+  __device__ __forceinline__ float lse2(int r) const { return __uint_as_float(r & 1 ? pair(r).z : pair(r).x); }
+  __device__ __forceinline__ float delta(int r) const { return __uint_as_float(r & 1 ? pair(r).w : pair(r).y); }
+};
+
+// keys of a tile of the dq launch
+template <int D>
+constexpr int dq_tile_keys() {
+  return 64;
+}
+template <int D>
+constexpr size_t dq_lds_bytes() {
+  return 256 + 4 * size_t(TileLds<D, dq_tile_keys<D>()>::kBytes);
 }
 
 // ---- dq -------------------------------------------------------------------------------------------------
 template <bool F16, int D, int MODE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTileArgs a) {
   using M = Mma<F16>;
-  typedef TileLds<D> T;
+  constexpr int KT = dq_tile_keys<D>(), NB = KT / 32;
+  typedef TileLds<D, KT> T;
   typedef typename std::conditional<F16, f16_t, bf16_t>::type E;
   constexpr int NKS = D / 16, NDT = D / 32;
   extern __shared__ __attribute__((aligned(256))) bf16_t lds_all[];
@@ -164,8 +211,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
   int lim, doc = 0, lim_lo, lim_hi, wg_lo, wg_hi;
   int2 q_doc = make_int2(0, 0), wg_doc = make_int2(0, 0);
   if (a.use_masks) {
-    lim = a.m.lim[iq];
-    doc = a.m.docq[iq];
+    const int2 qi = a.m.qinfo[iq];
+    lim = qi.x, doc = qi.y;
     const int4 q0 = a.m.qmeta[i0 / 32], q1 = a.m.qmeta[i0 / 32 + 1], q2 = a.m.qmeta[i0 / 32 + 2], q3 = a.m.qmeta[i0 / 32 + 3];
     const int4 mine = a.m.qmeta[wq0 / 32];
     lim_lo = mine.x, lim_hi = mine.y;
@@ -196,7 +243,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
       df[ks] = q_ok ? pd[2 * ks] : make_uint4(0, 0, 0, 0);
     }
   }
-  const float lse2 = q_ok ? a.lse[row] * kLog2e : 0.f, delta = q_ok ? a.delta[row] : 0.f;
+  const float2 rd = q_ok ? a.rd[row] : make_float2(0.f, 0.f);
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
     asm volatile("" : "+v"(qf[ks].x), "+v"(qf[ks].y), "+v"(qf[ks].z), "+v"(qf[ks].w));
@@ -208,8 +255,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
 #pragma unroll
     for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
 
-  FlatSource<D> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
-  const int t_end = (wg_hi + kTK - 1) / kTK;
+  FlatSource<D, KT> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
+  const int t_end = (wg_hi + KT - 1) / KT;
   int mask_at = -64;
   unsigned long long mask = 0;
   auto next = [&](int t) {
@@ -219,7 +266,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
         mask_at = t;
         bool hit = false;
         if (t + l < t_end) {
-          const int2 km = a.m.kmeta[t + l];
+          const int2 km = tile_docs<KT>(a.m.kmeta, t + l);
           hit = km.y >= wg_doc.x && km.x <= wg_doc.y && km.y >= 0;
         }
         mask = __ballot(hit);
@@ -231,6 +278,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
     return t_end;
   };
   bool dirty = false;
+  const typename T::Bases bases(l);
   int t = next(0), par = 0;
   if (t < t_end) src.issue(t, lds0, lds0 + T::kBytes, w, l);
   while (t < t_end) {
@@ -242,11 +290,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
       src.issue(t_next, to, to + T::kBytes, w, l);
     }
     const lds_char_t* bK = lds + par * 2 * T::kBytes;
-    const lds_char_t* bV = bK + T::kBytes;
-    const int kp0 = t * kTK;
-    bool wg_masked = kp0 + kTK > wg_lo, masked = kp0 + kTK > lim_lo, any = kp0 < lim_hi;
+    const auto at = bases.fresh(par * 2 * T::kBytes);
+    const int kp0 = t * KT;
+    bool wg_masked = kp0 + KT > wg_lo, masked = kp0 + KT > lim_lo, any = kp0 < lim_hi;
     if (has_docs) {
-      const int2 km = a.m.kmeta[t];
+      const int2 km = tile_docs<KT>(a.m.kmeta, t);
       wg_masked |= km.x != km.y || wg_doc.x != wg_doc.y;
       masked |= km.x != km.y || q_doc.x != q_doc.y;
       any = any && km.y >= q_doc.x && km.x <= q_doc.y;
@@ -257,22 +305,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
     }
     if (any) {
 #pragma unroll
-      for (int sb = 0; sb < 2; ++sb) {
+      for (int sb = 0; sb < NB; ++sb) {
         typename M::f16v s, p;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f, p[r] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
-          s = M::m32(T::rows32(bK, 32 * sb, ks, l), qf[ks], s);
-          p = M::m32(T::rows32(bV, 32 * sb, ks, l), df[ks], p);
+          s = M::m32(T::rows32(lds, at.rows, 32 * sb, ks), qf[ks], s);
+          p = M::m32(T::rows32(lds + T::kBytes, at.rows, 32 * sb, ks), df[ks], p);
         }
-        float x[16], dp[16], slack[16];
+        if constexpr ((MODE & kModeCap) != 0) tile_settle(s);
+        float x[16], dp[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = s[r], dp[r] = p[r];
+        for (int r = 0; r < 16; ++r) x[r] = s[r];
         const int key0 = kp0 + 32 * sb + 4 * hb;
-        block_scores<MODE, true>(x, slack, a.in, a.out_scale, float(pos - key0), slope2);
+        block_probs<MODE>(x, dp, a.score, float(pos - key0), slope2, ColumnQuery{rd.x});
 #pragma unroll
-        for (int r = 0; r < 16; ++r) block_grads<F16, MODE>(x, dp, slack, r, lse2, delta, g_scale);
+        for (int r = 0; r < 16; ++r) {
+          dp[r] *= p[r] - rd.y;
+          if constexpr (F16) dp[r] *= g_scale;
+        }
         if (masked) {
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
@@ -292,7 +344,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
           const uint4 gf = make_uint4(M::pack2(dp[8 * h + 0], dp[8 * h + 1]), M::pack2(dp[8 * h + 2], dp[8 * h + 3]),
                                       M::pack2(dp[8 * h + 4], dp[8 * h + 5]), M::pack2(dp[8 * h + 6], dp[8 * h + 7]));
 #pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bK, 32 * sb + 16 * h, dt, l), gf, O[dt]);
+          for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(lds, at.cols, 32 * sb + 16 * h, dt), gf, O[dt]);
         }
       }
     }
@@ -322,31 +374,34 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
   const Score<(MODE & kModeCap) != 0> score(a.sm_scale, a.t.softcap);
   for (int i = wq0; i < min(wq0 + 32, a.S); ++i) {
     const int64_t r = int64_t(hq) * a.S + i;
-    row_dq<E, (MODE & kModeCap) != 0>((const E*)a.q + r * D, (const E*)a.dout + r * D, a.lse[r], a.delta[r], K, V,
-                                      query_view(a.t, i, a.S, a.L, hq), a.t.doc_k, a.sm_scale, score, (E*)a.dq + r * D);
+    row_dq<E, (MODE & kModeCap) != 0>((const E*)a.q + r * D, (const E*)a.dout + r * D, a.rd[r], K, V, query_view(a.t, i, a.S, a.L, hq), a.t.doc_k, a.sm_scale, score, (E*)a.dq + r * D);
   }
 }
 
 // ---- dk, dv ------------------------------------------------------------------------------------------------
 constexpr int kDkvKeys = 128;  // keys of a workgroup
-constexpr int kDkvQ = 64;      // queries of a tile
+constexpr int kDkvQ = 32;      // queries of a tile
 
+// the values of the workgroup's keys, two tiles of q and dout, two of {lse log2 e, D} and {limit, document} of the queries
 template <int D>
 constexpr size_t dkv_lds_bytes() {
-  return 512 + 4 * size_t(TileLds<D>::kBytes) + 2 * 4 * 256;  // two tiles of q and dout, two of lse, D, limits, documents
+  return 512 + size_t(TileLds<D, kDkvKeys>::kBytes) + 4 * size_t(TileLds<D, kDkvQ>::kBytes) + 2 * 2 * kDkvQ * 8;
 }
 
 template <bool F16, int D, int MODE>
-__global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTileArgs a) {
   using M = Mma<F16>;
-  typedef TileLds<D> T;
+  typedef TileLds<D, kDkvQ> T;
+  typedef TileLds<D, kDkvKeys> TV;
   typedef typename std::conditional<F16, f16_t, bf16_t>::type E;
   constexpr int NKS = D / 16, NDT = D / 32;
   constexpr float p_scale = F16 ? kPScaleF16 : 1.f;
   extern __shared__ __attribute__((aligned(256))) bf16_t lds_all[];
   int* flag = reinterpret_cast<int*>(lds_all);
-  lds_char_t* lds = (lds_char_t*)(lds_all + 256);
-  lds_char_t* lds_row = lds + 4 * T::kBytes;  // [2]{lse, D, lim, doc}[64]
+  lds_char_t* lds_v = (lds_char_t*)(lds_all + 256);
+  lds_char_t* lds = lds_v + TV::kBytes;
+  lds_char_t* lds_row = lds + 4 * T::kBytes;  // [2]{ {lse log2 e, D}[32], {limit, document}[32] }
+  const uint32_t lds_v0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds_v)));
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds)));
   const uint32_t lds_row0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds_row)));
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5;
@@ -361,28 +416,29 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
   const bool j_ok = j < a.L;
   const bool has_docs = a.use_masks && a.t.doc_q;
   int doc = 0;
-  int2 k_doc = make_int2(0, 0), wg_doc = make_int2(0, 0);  // of 64 keys (this wave's are half of them), of the workgroup's
+  int2 k_doc = make_int2(0, 0), wg_doc = make_int2(0, 0);  // of the wave's keys, of the workgroup's
   if (has_docs) {
     doc = a.m.dock[j];
-    const int2 m0 = a.m.kmeta[j0 / 64], m1 = a.m.kmeta[j0 / 64 + 1];
-    k_doc = w < 2 ? m0 : m1;
+    const int2 m0 = tile_docs<64>(a.m.kmeta, j0 / 64), m1 = tile_docs<64>(a.m.kmeta, j0 / 64 + 1);
+    k_doc = a.m.kmeta[j0 / 32 + w];
     wg_doc = make_int2(min(m0.x, m1.x), max(m0.y, m1.y));
   }
-  uint4 kf[NKS], vf[NKS];
+  // keys in registers, values in LDS: with both in registers a wave would need more than half of its SIMD's
+  uint4 kf[NKS];
   {
-    const int64_t r = (int64_t(hk) * a.L + (j_ok ? j : 0)) * D + hb * 8;
-    const uint4* pk = reinterpret_cast<const uint4*>(a.k + r);
-    const uint4* pv = reinterpret_cast<const uint4*>(a.v + r);
+    const uint4* pk = reinterpret_cast<const uint4*>(a.k + (int64_t(hk) * a.L + (j_ok ? j : 0)) * D + hb * 8);
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      kf[ks] = j_ok ? pk[2 * ks] : make_uint4(0, 0, 0, 0);
-      vf[ks] = j_ok ? pv[2 * ks] : make_uint4(0, 0, 0, 0);
-    }
+    for (int ks = 0; ks < NKS; ++ks) kf[ks] = j_ok ? pk[2 * ks] : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
-    asm volatile("" : "+v"(kf[ks].x), "+v"(kf[ks].y), "+v"(kf[ks].z), "+v"(kf[ks].w));
-    asm volatile("" : "+v"(vf[ks].x), "+v"(vf[ks].y), "+v"(vf[ks].z), "+v"(vf[ks].w));
+  for (int ks = 0; ks < NKS; ++ks) asm volatile("" : "+v"(kf[ks].x), "+v"(kf[ks].y), "+v"(kf[ks].z), "+v"(kf[ks].w));
+  {
+    const bf16_t* bv = ring_uniform_ptr(a.v + (int64_t(hk) * a.L + j0) * D);
+#pragma unroll
+    for (int u = 0; u < TV::kLoadsPerWave; ++u) {
+      const int r = TV::load_row(w + 4 * u, l);
+      tile_load(lds_v0 + uint32_t(w + 4 * u) * 1024u, uint32_t(min(r, a.L - 1 - j0)) * TV::kRowBytes + TV::load_chunk(r, l), bv);
+    }
   }
   typename M::f16v dK[NDT], dV[NDT];
 #pragma unroll
@@ -390,8 +446,9 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dK[dt][r] = 0.f, dV[dt][r] = 0.f;
 
-  // Steps: tile qt of 64 queries of head g, counted from the first tile that can see the workgroup's keys:
-  // step = g n + (qt - qt0), and this workgroup's are [s0, s1).
+  // Steps: tile qt of 32 queries of head g, from the last tile down to the first that can see the workgroup's keys (so
+  // that workgroups with other keys, which see other first queries, read the same tiles at the same time):
+  // step = g n + (last - qt), and this workgroup's are [s0, s1).
   const int nqt = (a.S + kDkvQ - 1) / kDkvQ;
   const int qt0 = (a.t.causal && !a.use_masks) ? min(max(0, j0 - (a.L - a.S)) / kDkvQ, nqt) : 0;
   const int n = nqt - qt0;
@@ -407,10 +464,10 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
         mask_at = s;
         bool hit = false;
         if (s + l < s1) {
-          const int qt = qt0 + (s + l) % n;
-          const int4 x = a.m.qmeta[2 * qt], y = a.m.qmeta[2 * qt + 1];
-          hit = max(x.y, y.y) > j0;
-          if (has_docs) hit = hit && wg_doc.y >= 0 && max(x.w, y.w) >= wg_doc.x && min(x.z, y.z) <= wg_doc.y;
+          const int qt = nqt - 1 - (s + l) % n;
+          const int4 x = a.m.qmeta[qt];
+          hit = x.y > j0;
+          if (has_docs) hit = hit && wg_doc.y >= 0 && x.w >= wg_doc.x && x.z <= wg_doc.y;
         }
         mask = __ballot(hit);
       }
@@ -421,7 +478,7 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
     return s1;
   };
   auto issue = [&](int s, int par) {
-    const int g = s / n, qt = qt0 + (s - g * n), hq = hk * a.G + g;
+    const int g = s / n, qt = nqt - 1 - (s - g * n), hq = hk * a.G + g;
     const int i0 = qt * kDkvQ, last = a.S - 1 - i0;
     const int64_t row = int64_t(hq) * a.S + i0;
     const bf16_t* bq = ring_uniform_ptr(a.q + row * D);
@@ -437,14 +494,13 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
       const int r = T::load_row(w + 4 * u, l);
       tile_load(to + T::kBytes + uint32_t(w + 4 * u) * 1024u, uint32_t(min(r, last)) * T::kRowBytes + T::load_chunk(r, l), bd);
     }
-    // wave 0: lse, 1: D, 2: limits, 3: documents (the last two without masks: nobody reads them)
-    const void* base = w == 0 ? (const void*)(a.lse + row) : w == 1 ? (const void*)(a.delta + row)
-                       : !a.use_masks ? (const void*)(a.lse + row)
-                       : w == 2       ? (const void*)(a.m.lim + i0)
-                                      : (const void*)(a.m.docq + i0);
-    ring_load4(lds_row0 + uint32_t(par) * 1024u + uint32_t(w) * 256u, uint32_t(min(l, last)) * 4u, ring_uniform_ptr((const char*)base));
+    // 8 bytes a query: wave 0 {lse log2 e, D}, wave 1 {limit, document} where there are masks
+    const uint32_t voff = uint32_t(min(l >> 1, last)) * 8u + uint32_t(l & 1) * 4u;
+    if (w == 0) ring_load4(lds_row0 + uint32_t(par) * 512u, voff, ring_uniform_ptr(a.rd + row));
+    if (w == 1 && a.use_masks) ring_load4(lds_row0 + uint32_t(par) * 512u + 256u, voff, ring_uniform_ptr(a.m.qinfo + i0));
   };
   bool dirty = false;
+  const typename T::Bases bases(l);
   int s = next(s0), par = 0;
   if (s < s1) issue(s, 0);
   while (s < s1) {
@@ -452,76 +508,61 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     ring_barrier();
     if (s_next < s1) issue(s_next, par ^ 1);
-    const int g = s / n, qt = qt0 + (s - g * n), hq = hk * a.G + g;
+    const int g = s / n, qt = nqt - 1 - (s - g * n), hq = hk * a.G + g;
     const int i0 = qt * kDkvQ;
     const float slope2 = (MODE & kModeBias) ? a.t.slopes[hq] * kLog2e : 0.f;
     const lds_char_t* bQ = lds + par * 2 * T::kBytes;
     const lds_char_t* bD = bQ + T::kBytes;
-    const lds_char_t* rows = lds_row + par * 1024;
-    // who sees what: fewest and most keys of the 64 queries, and of each 32
-    int lo[2], hi[2];
-    bool mixed[2] = {false, false};
+    const lds_char_t* rows = lds_row + par * 512;
+    // who sees what: fewest and most keys of the 32 queries
+    int lo, hi;
+    bool mixed = false;
     if (a.use_masks) {
-      const int4 x = a.m.qmeta[2 * qt], y = a.m.qmeta[2 * qt + 1];
-      lo[0] = x.x, hi[0] = x.y, lo[1] = y.x, hi[1] = y.y;
-      if (has_docs) {
-        mixed[0] = k_doc.x != k_doc.y || x.z != x.w || x.z != k_doc.x;
-        mixed[1] = k_doc.x != k_doc.y || y.z != y.w || y.z != k_doc.x;
-      }
+      const int4 x = a.m.qmeta[qt];
+      lo = x.x, hi = x.y;
+      if (has_docs) mixed = k_doc.x != k_doc.y || x.z != x.w || x.z != k_doc.x || wg_doc.x != wg_doc.y;
     } else {
-#pragma unroll
-      for (int sb = 0; sb < 2; ++sb) {
-        const int a0 = i0 + 32 * sb, a1 = min(a0 + 31, a.S - 1);
-        lo[sb] = seen_limit(a0 + (a.L - a.S), a.L, a.t.causal, 0);
-        hi[sb] = a0 < a.S ? seen_limit(a1 + (a.L - a.S), a.L, a.t.causal, 0) : 0;
-      }
+      lo = seen_limit(i0 + (a.L - a.S), a.L, a.t.causal, 0);
+      hi = seen_limit(min(i0 + 31, a.S - 1) + (a.L - a.S), a.L, a.t.causal, 0);
     }
     const bool ragged = i0 + kDkvQ > a.S;
-    if (ragged || min(lo[0], lo[1]) < min(j0 + kDkvKeys, a.L) || mixed[0] || mixed[1] ||
-        (has_docs && wg_doc.x != wg_doc.y)) {
+    if (ragged || mixed || lo < min(j0 + kDkvKeys, a.L)) {
 #pragma unroll
-      for (int u = 0; u < T::kBytes / 4096; ++u) {
-        dirty |= any_nonfinite<F16>(lds_read16(bQ + (u * 256 + tid) * 16));
-        dirty |= any_nonfinite<F16>(lds_read16(bD + (u * 256 + tid) * 16));
+      for (int u = 0; u < (T::kBytes + 4095) / 4096; ++u) {
+        const int at = (u * 256 + tid) * 16;
+        if (T::kBytes % 4096 && at >= T::kBytes) continue;
+        dirty |= any_nonfinite<F16>(lds_read16(bQ + at)) | any_nonfinite<F16>(lds_read16(bD + at));
       }
     }
+    if (hi > wj0) {
+      const auto at = bases.fresh(par * 2 * T::kBytes);
+      int vrows = bases.rows + 32 * w * TV::kRowBytes;
+      asm volatile("" : "+v"(vrows));
+      // scores, p, and dv first, then dP, g and dk: of the two products' operands one is held at a time
+      typename M::f16v sc;
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb) {
-      if (hi[sb] <= wj0) continue;
-      typename M::f16v sc, pr;
+      for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] = 0.f, pr[r] = 0.f;
+      for (int ks = 0; ks < NKS; ++ks) sc = M::m32(T::rows32(lds, at.rows, 0, ks), kf[ks], sc);
+      if constexpr ((MODE & kModeCap) != 0) tile_settle(sc);
+      float x[16], y[16];  // p; p slack
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
-        sc = M::m32(T::rows32(bQ, 32 * sb, ks, l), kf[ks], sc);
-        pr = M::m32(T::rows32(bD, 32 * sb, ks, l), vf[ks], pr);
-      }
-      float x[16], dp[16], slack[16];
+      for (int r = 0; r < 16; ++r) x[r] = sc[r];
+      const RowQueries rq{rows + 4 * hb * 8};
+      block_probs<MODE>(x, y, a.score, float(j - (i0 + 4 * hb + (a.L - a.S))), slope2, rq);
+      const bool masked = mixed || ragged || wj0 + 32 > lo;
+      if (masked) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = sc[r], dp[r] = pr[r];
-      const int q0 = 32 * sb + 4 * hb;  // of the tile: this lane's rows are q0 + 8 (r / 4) + r % 4
-      block_scores<MODE, true>(x, slack, a.in, a.out_scale, float(j - (i0 + q0 + (a.L - a.S))), slope2);
-      const bool masked = mixed[sb] || ragged || wj0 + 32 > lo[sb];
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const int at = (q0 + 8 * r4) * 4;
-        const uint4 ls = lds_read16(rows + at), de = lds_read16(rows + 256 + at);
-        const float lsv[4] = {__uint_as_float(ls.x), __uint_as_float(ls.y), __uint_as_float(ls.z), __uint_as_float(ls.w)};
-        const float dev[4] = {__uint_as_float(de.x), __uint_as_float(de.y), __uint_as_float(de.z), __uint_as_float(de.w)};
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          block_grads<F16, MODE>(x, dp, slack, 4 * r4 + r, lsv[r] * kLog2e, dev[r], g_scale);
-        if (masked) {
-          uint4 li = make_uint4(0, 0, 0, 0), dq4 = make_uint4(0, 0, 0, 0);
-          if (a.use_masks) li = lds_read16(rows + 512 + at), dq4 = lds_read16(rows + 768 + at);
-          const uint32_t liv[4] = {li.x, li.y, li.z, li.w}, dqv[4] = {dq4.x, dq4.y, dq4.z, dq4.w};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = i0 + q0 + 8 * r4 + r;
-            bool ok = i < a.S && j < (a.use_masks ? int(liv[r]) : seen_limit(i + (a.L - a.S), a.L, a.t.causal, 0));
-            if (has_docs) ok = ok && int(dqv[r]) == doc;
-            if (!ok) x[4 * r4 + r] = 0.f, dp[4 * r4 + r] = 0.f;
+        for (int r = 0; r < 16; ++r) {
+          const int iq = 4 * hb + 8 * (r >> 2) + (r & 3), i = i0 + iq;
+          bool ok = i < a.S;
+          if (a.use_masks) {
+            const lds_int2 qi = *reinterpret_cast<const __attribute__((address_space(3))) lds_int2*>(rows + 256 + iq * 8);
+            ok = ok && j < qi.x && (!has_docs || qi.y == doc);
+          } else {
+            ok = ok && j < seen_limit(i + (a.L - a.S), a.L, a.t.causal, 0);
           }
+          if (!ok) x[r] = 0.f, y[r] = 0.f;
         }
       }
 #pragma unroll
@@ -532,13 +573,31 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
         }
         const uint4 pf = make_uint4(M::pack2(x[8 * h + 0], x[8 * h + 1]), M::pack2(x[8 * h + 2], x[8 * h + 3]),
                                     M::pack2(x[8 * h + 4], x[8 * h + 5]), M::pack2(x[8 * h + 6], x[8 * h + 7]));
-        const uint4 gf = make_uint4(M::pack2(dp[8 * h + 0], dp[8 * h + 1]), M::pack2(dp[8 * h + 2], dp[8 * h + 3]),
-                                    M::pack2(dp[8 * h + 4], dp[8 * h + 5]), M::pack2(dp[8 * h + 6], dp[8 * h + 7]));
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) {
-          dV[dt] = M::m32(T::cols32(bD, 32 * sb + 16 * h, dt, l), pf, dV[dt]);
-          dK[dt] = M::m32(T::cols32(bQ, 32 * sb + 16 * h, dt, l), gf, dK[dt]);
-        }
+        for (int dt = 0; dt < NDT; ++dt) dV[dt] = M::m32(T::cols32(lds + T::kBytes, at.cols, 16 * h, dt), pf, dV[dt]);
+      }
+      typename M::f16v pr;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) pr[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks)
+        pr = M::m32(T::rows32(lds + T::kBytes, at.rows, 0, ks), TV::rows32(lds_v, vrows, 0, ks), pr);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        pr[r] = (pr[r] - rq.delta(r)) * y[r];
+        if constexpr (F16) pr[r] *= g_scale;
+      }
+      if (masked) {  // (what is not seen may have made a NaN)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (y[r] == 0.f) pr[r] = 0.f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 gf = make_uint4(M::pack2(pr[8 * h + 0], pr[8 * h + 1]), M::pack2(pr[8 * h + 2], pr[8 * h + 3]),
+                                    M::pack2(pr[8 * h + 4], pr[8 * h + 5]), M::pack2(pr[8 * h + 6], pr[8 * h + 7]));
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) dK[dt] = M::m32(T::cols32(lds, at.cols, 16 * h, dt), gf, dK[dt]);
       }
     }
     s = s_next;
@@ -576,9 +635,10 @@ __global__ __launch_bounds__(256, 1) void terms_dkv_kernel(BwdTileArgs a) {
     KeyGrads kg;
     key_grads_zero(kg);
     for (int ss = s0; ss < s1; ++ss) {
-      const int g = ss / n, qt = qt0 + (ss - g * n);
-      row_dkv_chunk<E, (MODE & kModeCap) != 0>((const E*)a.k + at, (const E*)a.v + at, jj, hk * a.G + g, qt * kDkvQ, a.S, a.L, D,
-                                               (const E*)a.q, (const E*)a.dout, a.lse, a.delta, a.t, score, kg);
+      const int g = ss / n, qt = nqt - 1 - (ss - g * n);
+      row_dkv_chunk<E, (MODE & kModeCap) != 0>((const E*)a.k + at, (const E*)a.v + at, jj, hk * a.G + g, qt * kDkvQ,
+                                               min(a.S, (qt + 1) * kDkvQ), a.S, a.L, D,
+                                               (const E*)a.q, (const E*)a.dout, a.rd, a.t, score, kg);
     }
     for (int r = 0; r < (D + 63) / 64; ++r) {
       const int c = l + 64 * r;
@@ -611,10 +671,10 @@ __global__ __launch_bounds__(256) void terms_dkv_join_kernel(const float* __rest
 
 template <bool F16, int D, int MODE>
 static int launch_terms_bwd(const BwdTileArgs& a, hipStream_t st) {
-  FM_ALLOW_LDS((terms_dq_kernel<F16, D, MODE>), 256 + 4 * size_t(TileLds<D>::kBytes), "fm_local_attn_terms_bwd(lds)");
+  FM_ALLOW_LDS((terms_dq_kernel<F16, D, MODE>), dq_lds_bytes<D>(), "fm_local_attn_terms_bwd(lds)");
   FM_ALLOW_LDS((terms_dkv_kernel<F16, D, MODE>), dkv_lds_bytes<D>(), "fm_local_attn_terms_bwd(lds)");
   hipLaunchKernelGGL((terms_dq_kernel<F16, D, MODE>), dim3(unsigned(a.H * a.G * ceil_div(a.S, kTQ))), dim3(256),
-                     256 + 4 * size_t(TileLds<D>::kBytes), st, a);
+                     dq_lds_bytes<D>(), st, a);
   hipLaunchKernelGGL((terms_dkv_kernel<F16, D, MODE>), dim3(unsigned(a.H * a.splits * ceil_div(a.L, kDkvKeys))), dim3(256),
                      dkv_lds_bytes<D>(), st, a);
   if (a.splits > 1) {
@@ -626,11 +686,11 @@ static int launch_terms_bwd(const BwdTileArgs& a, hipStream_t st) {
 }
 
 template <bool F16, int D>
-static int launch_terms_bwd_type(const BwdTileArgs& a, const void* out, const float* dlse, float* delta, float* norms, hipStream_t st) {
+static int launch_terms_bwd_type(const BwdTileArgs& a, const void* out, const float* lse, const float* dlse, float2* rd, float* norms, hipStream_t st) {
   const int64_t rows = int64_t(a.H) * a.G * a.S, keys = int64_t(a.H) * a.L;
   const int qb = int(ceil_div(rows, kNormRows)), kb = F16 ? int(ceil_div(keys, kNormRows)) : 0;
-  hipLaunchKernelGGL((terms_delta_tile_kernel<F16, D>), dim3(unsigned(qb + kb)), dim3(256), 0, st, (const bf16_t*)out, a.dout, dlse,
-                     a.v, delta, norms, rows, keys, qb, a.S, a.L, a.use_masks ? a.m.lim : nullptr, a.use_masks ? a.m.dock : nullptr);
+  hipLaunchKernelGGL((terms_delta_tile_kernel<F16, D>), dim3(unsigned(qb + kb)), dim3(256), 0, st, (const bf16_t*)out, a.dout, lse,
+                     dlse, a.v, rd, norms, rows, keys, qb, a.S, a.L, a.use_masks ? a.m.qinfo : nullptr, a.use_masks ? a.m.dock : nullptr);
   switch ((a.t.softcap > 0.f ? kModeCap : 0) | (a.t.slopes ? kModeBias : 0)) {
     case 0: return launch_terms_bwd<F16, D, 0>(a, st);
     case kModeCap: return launch_terms_bwd<F16, D, kModeCap>(a, st);
@@ -640,9 +700,9 @@ static int launch_terms_bwd_type(const BwdTileArgs& a, const void* out, const fl
 }
 
 template <int D>
-int terms_bwd_tiles(const BwdTileArgs& a, bool f16, const void* out, const float* dlse, float* delta, float* norms, hipStream_t st) {
-  return f16 ? launch_terms_bwd_type<true, D>(a, out, dlse, delta, norms, st)
-             : launch_terms_bwd_type<false, D>(a, out, dlse, delta, norms, st);
+int terms_bwd_tiles(const BwdTileArgs& a, bool f16, const void* out, const float* lse, const float* dlse, float2* rd, float* norms, hipStream_t st) {
+  return f16 ? launch_terms_bwd_type<true, D>(a, out, lse, dlse, rd, norms, st)
+             : launch_terms_bwd_type<false, D>(a, out, lse, dlse, rd, norms, st);
 }
 
 }  // namespace fm

@@ -2,5 +2,5 @@
 #include "terms_bwd.hpp"
 
 namespace fm {
-template int terms_bwd_tiles<64>(const BwdTileArgs&, bool, const void*, const float*, float*, float*, hipStream_t);
+template int terms_bwd_tiles<64>(const BwdTileArgs&, bool, const void*, const float*, const float*, float2*, float*, hipStream_t);
 }  // namespace fm

@@ -15,7 +15,7 @@ namespace fm {
 
 template <int D>
 constexpr size_t tile_lds_bytes() {
-  return 256 + 4 * size_t(TileLds<D>::kBytes);
+  return 256 + 4 * size_t(TileLds<D, fwd_tile_keys<D>()>::kBytes);
 }
 
 struct FwdTileArgs {
@@ -25,7 +25,8 @@ struct FwdTileArgs {
   Terms t;
   Masks m;
   int use_masks, H, G, S, L;
-  float in, out_scale, sm_scale;
+  float sm_scale;
+  TileScore score;
 };
 
 template <bool F16, int D, int MODE>
@@ -48,8 +49,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
   TileDocs docs{nullptr, nullptr, make_int2(0, 0), make_int2(0, 0)};
   int lim_lo, lim_hi, wg_lo, wg_hi;
   if (a.use_masks) {
-    qy.lim = a.m.lim[iq];
-    qy.doc = a.m.docq[iq];
+    const int2 qi = a.m.qinfo[iq];
+    qy.lim = qi.x, qy.doc = qi.y;
     const int4 q0 = a.m.qmeta[i0 / 32], q1 = a.m.qmeta[i0 / 32 + 1], q2 = a.m.qmeta[i0 / 32 + 2], q3 = a.m.qmeta[i0 / 32 + 3];
     const int4 mine = a.m.qmeta[wq0 / 32];
     lim_lo = mine.x, lim_hi = mine.y;
@@ -85,11 +86,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(qf[ks].x), "+v"(qf[ks].y), "+v"(qf[ks].z), "+v"(qf[ks].w));
 
-  const FlatSource<D> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
+  constexpr int KT = fwd_tile_keys<D>();
+  const FlatSource<D, KT> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
   typename M::f16v O[D / 32];
   TileState st;
-  const bool again = tile_sweep<F16, D, MODE>(src, qf, qy, lim_lo, lim_hi, wg_lo, 0, (wg_hi + kTK - 1) / kTK, docs, a.in,
-                                              a.out_scale, lds, flag, O, st);
+  const bool again = tile_sweep<F16, D, MODE>(src, qf, qy, lim_lo, lim_hi, wg_lo, 0, (wg_hi + KT - 1) / KT, docs, a.score,
+                                              lds, flag, O, st);
   if (!again) {
     tile_write<F16, D>(O, st, q_ok ? a.out + row * D : nullptr, a.lse + row);
     return;

@@ -33,73 +33,71 @@ int terms_fwd_rows(const FwdArgs& a, hipStream_t st) {
   return launch_status("fm_local_attn_terms_fwd(rows)");
 }
 
-// D_i = do_i.o_i - dlse_i, a wave per row
+// {lse_i log2 e, D_i = do_i.o_i - dlse_i}, a wave per row
 template <typename T>
 __global__ __launch_bounds__(256) void terms_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout,
-                                                          const float* __restrict__ dlse, float* __restrict__ delta, int d,
-                                                          int64_t rows) {
+                                                          const float* __restrict__ lse, const float* __restrict__ dlse,
+                                                          float2* __restrict__ rd, int d, int64_t rows) {
   const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   float s = 0.f;
   for (int k = lane_id(); k < d; k += 64) s = fmaf(Elem<T>::load(dout + row * d + k), Elem<T>::load(out + row * d + k), s);
   s = wave_sum(s);
-  if (lane_id() == 0) delta[row] = s - (dlse ? dlse[row] : 0.f);
+  if (lane_id() == 0) rd[row] = make_float2(lse[row] * kLog2e, s - (dlse ? dlse[row] : 0.f));
 }
 
 template <typename T, bool CAP>
 __global__ __launch_bounds__(256) void terms_dq_row_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                            const T* __restrict__ v, const T* __restrict__ dout,
-                                                           const float* __restrict__ lse, const float* __restrict__ delta,
-                                                           T* __restrict__ dq, Terms t, int G, int S, int L, int d,
+                                                           const float2* __restrict__ rd, T* __restrict__ dq, Terms t, int G, int S, int L, int d,
                                                            int64_t rows, float sm_scale, Score<CAP> score) {
   const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int hq = int(row / S), i = int(row - int64_t(hq) * S);
   const int64_t head = int64_t(hq / G) * L * d;
   const KeyRows<T> K{k + head, nullptr, 0, 0, 0, d}, V{v + head, nullptr, 0, 0, 0, d};
-  row_dq<T, CAP>(q + row * d, dout + row * d, lse[row], delta[row], K, V, query_view(t, i, S, L, hq), t.doc_k, sm_scale, score,
+  row_dq<T, CAP>(q + row * d, dout + row * d, rd[row], K, V, query_view(t, i, S, L, hq), t.doc_k, sm_scale, score,
                  dq + row * d);
 }
 
 template <typename T, bool CAP>
 __global__ __launch_bounds__(256) void terms_dkv_row_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                             const T* __restrict__ v, const T* __restrict__ dout,
-                                                            const float* __restrict__ lse, const float* __restrict__ delta,
-                                                            T* __restrict__ dk, T* __restrict__ dv, Terms t, int G, int S,
+                                                            const float2* __restrict__ rd, T* __restrict__ dk, T* __restrict__ dv, Terms t, int G, int S,
                                                             int L, int d, int64_t rows, float sm_scale, Score<CAP> score) {
   const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int hk = int(row / L), j = int(row - int64_t(hk) * L);
-  row_dkv<T, CAP>(k + row * d, v + row * d, j, hk, G, S, L, d, q, dout, lse, delta, t, sm_scale, score, dk + row * d,
+  row_dkv<T, CAP>(k + row * d, v + row * d, j, hk, G, S, L, d, q, dout, rd, t, sm_scale, score, dk + row * d,
                   dv + row * d);
 }
 
 template <typename T>
-int terms_delta(const BwdArgs& a, float* delta, hipStream_t st) {
+int terms_delta(const BwdArgs& a, float2* rd, hipStream_t st) {
   const int64_t rows = int64_t(a.f.H) * a.f.G * a.f.S;
   hipLaunchKernelGGL(terms_delta_kernel<T>, dim3(unsigned(ceil_div(rows, 4))), dim3(256), 0, st, (const T*)a.f.out,
-                     (const T*)a.dout, a.dlse, delta, a.f.d, rows);
+                     (const T*)a.dout, a.f.lse, a.dlse, rd, a.f.d, rows);
   return launch_status("fm_local_attn_terms_bwd(delta)");
 }
 
 template <typename T, bool CAP>
-static void launch_bwd_rows(const BwdArgs& a, const float* delta, Score<CAP> score, hipStream_t st) {
+static void launch_bwd_rows(const BwdArgs& a, const float2* rd, Score<CAP> score, hipStream_t st) {
   const FwdArgs& f = a.f;
   const int64_t rows = int64_t(f.H) * f.G * f.S, keys = int64_t(f.H) * f.L;
   hipLaunchKernelGGL((terms_dq_row_kernel<T, CAP>), dim3(unsigned(ceil_div(rows, 4))), dim3(256), 0, st, (const T*)f.q,
-                     (const T*)f.k, (const T*)f.v, (const T*)a.dout, f.lse, delta, (T*)a.dq, f.t, f.G, f.S, f.L, f.d, rows,
+                     (const T*)f.k, (const T*)f.v, (const T*)a.dout, rd, (T*)a.dq, f.t, f.G, f.S, f.L, f.d, rows,
                      f.sm_scale, score);
   hipLaunchKernelGGL((terms_dkv_row_kernel<T, CAP>), dim3(unsigned(ceil_div(keys, 4))), dim3(256), 0, st, (const T*)f.q,
-                     (const T*)f.k, (const T*)f.v, (const T*)a.dout, f.lse, delta, (T*)a.dk, (T*)a.dv, f.t, f.G, f.S, f.L, f.d,
+                     (const T*)f.k, (const T*)f.v, (const T*)a.dout, rd, (T*)a.dk, (T*)a.dv, f.t, f.G, f.S, f.L, f.d,
                      keys, f.sm_scale, score);
 }
 
 template <typename T>
-int terms_bwd_rows(const BwdArgs& a, const float* delta, hipStream_t st) {
+int terms_bwd_rows(const BwdArgs& a, const float2* rd, hipStream_t st) {
   if (a.f.t.softcap > 0.f)
-    launch_bwd_rows<T, true>(a, delta, Score<true>(a.f.sm_scale, a.f.t.softcap), st);
+    launch_bwd_rows<T, true>(a, rd, Score<true>(a.f.sm_scale, a.f.t.softcap), st);
   else
-    launch_bwd_rows<T, false>(a, delta, Score<false>(a.f.sm_scale, 0.f), st);
+    launch_bwd_rows<T, false>(a, rd, Score<false>(a.f.sm_scale, 0.f), st);
   return launch_status("fm_local_attn_terms_bwd(rows)");
 }
 
@@ -138,8 +136,8 @@ int paged_attn_rows(const PagedArgs& a, hipStream_t st) {
 
 #define FM_INST(T)                                                       \
   template int terms_fwd_rows<T>(const FwdArgs&, hipStream_t);           \
-  template int terms_delta<T>(const BwdArgs&, float*, hipStream_t);      \
-  template int terms_bwd_rows<T>(const BwdArgs&, const float*, hipStream_t); \
+  template int terms_delta<T>(const BwdArgs&, float2*, hipStream_t);      \
+  template int terms_bwd_rows<T>(const BwdArgs&, const float2*, hipStream_t); \
   template int paged_attn_rows<T>(const PagedArgs&, hipStream_t);
 FM_INST(float)
 FM_INST(bf16_t)

@@ -23,8 +23,7 @@ __global__ __launch_bounds__(256) void terms_masks_kernel(Masks m, Terms t, int 
       doc = t.doc_q ? t.doc_q[i] : 0;
       if (doc < 0) doc = -1, lim = 0;
     }
-    m.lim[i] = lim;
-    m.docq[i] = doc;
+    m.qinfo[i] = make_int2(lim, doc);
     const int a = wave_min_i(is ? lim : 0x7fffffff, 32), b = wave_max_i(lim, 32);
     const int c = wave_min_i(is ? doc : 0x7fffffff, 32), e = wave_max_i(is ? doc : -1, 32);
     if ((threadIdx.x & 31) == 0) m.qmeta[i / 32] = make_int4(a, b, c, e);
@@ -38,8 +37,8 @@ __global__ __launch_bounds__(256) void terms_masks_kernel(Masks m, Terms t, int 
     if (doc < 0) doc = -2;
   }
   m.dock[j] = doc;
-  const int a = wave_min_i(doc, 64), b = wave_max_i(doc, 64);
-  if ((threadIdx.x & 63) == 0) m.kmeta[j / 64] = make_int2(a, b);
+  const int a = wave_min_i(doc, 32), b = wave_max_i(doc, 32);
+  if ((threadIdx.x & 31) == 0) m.kmeta[j / 32] = make_int2(a, b);
 }
 
 int make_masks(const Masks& m, const Terms& t, int S, int L, hipStream_t st) {

@@ -1,10 +1,9 @@
 // What the queries of a call see, laid out for the tiled kernels by one small launch (terms_masks.hip); only made where
 // there are documents or prefixes -- a causal or full attention needs none of it.
-//   lim [S8]     keys query i sees as far as order goes (the rows behind the last query: 0)
-//   docq [S8]    its document, -1 where it has none
+//   qinfo [S8]   {keys query i sees as far as order goes (the rows behind the last query: 0), its document or -1}
 //   dock [L8]    a key's document, -2 where it has none or lies behind the last key
 //   qmeta [S8 / 32]   {fewest, most keys, smallest, largest document} of 32 queries (of those there are)
-//   kmeta [L8 / 64]   {smallest, largest document} of 64 keys
+//   kmeta [L8 / 32]   {smallest, largest document} of 32 keys
 // S8, L8: S and L rounded up to 128.
 #pragma once
 #include "terms_api.hpp"
@@ -12,7 +11,8 @@
 namespace fm {
 
 struct Masks {
-  int32_t *lim, *docq, *dock;
+  int2* qinfo;
+  int32_t* dock;
   int4* qmeta;
   int2* kmeta;
   size_t bytes;
@@ -28,11 +28,10 @@ inline Masks masks_layout(void* ws, int S, int L) {
     at += align_up(n, 256);
     return r;
   };
-  m.lim = reinterpret_cast<int32_t*>(take(S8 * 4));
-  m.docq = reinterpret_cast<int32_t*>(take(S8 * 4));
+  m.qinfo = reinterpret_cast<int2*>(take(S8 * 8));
   m.dock = reinterpret_cast<int32_t*>(take(L8 * 4));
   m.qmeta = reinterpret_cast<int4*>(take(S8 / 32 * 16));
-  m.kmeta = reinterpret_cast<int2*>(take(L8 / 64 * 8));
+  m.kmeta = reinterpret_cast<int2*>(take(L8 / 32 * 8));
   m.bytes = at;
   return m;
 }

@@ -1,5 +1,5 @@
 // The tiled forward of the attention with score terms (bf16 / fp16, head dimension 64, 128 or 256): 128 query rows per
-// workgroup, 32 per wave, over tiles of 64 keys.  The training forward (terms_fwd.hip) and the chunks over a paged cache
+// workgroup, 32 per wave, over tiles of keys.  The training forward (terms_fwd.hip) and the chunks over a paged cache
 // (paged_attn.hip) run it; they differ in where a key's row lies and in what a query row is.
 //
 //   S^T = K.Q^T   v_mfma_f32_32x32x16: A = 32 keys of the tile from LDS, B = this wave's queries, in registers for the
@@ -26,7 +26,9 @@
 namespace fm {
 
 constexpr int kTQ = 128;  // query rows of a workgroup
-constexpr int kTK = 64;   // keys of a tile
+// keys of a tile of the forward
+template <int D>
+constexpr int fwd_tile_keys() { return 32; }
 
 // what the scores have, beside the product: bit 0 the cap, bit 1 the distance bias
 constexpr int kModeCap = 1, kModeBias = 2;
@@ -68,7 +70,7 @@ __device__ __forceinline__ uint4 tr_pair(const lds_char_t* p, const lds_char_t* 
 }
 
 // LDS of one tile of ROWS rows: where a wave's lanes load, and where the operands are read
-template <int D, int ROWS = kTK>
+template <int D, int ROWS>
 struct TileLds {
   static constexpr int kRowBytes = 2 * D;
   static constexpr int kBytes = ROWS * kRowBytes;
@@ -80,53 +82,112 @@ struct TileLds {
   __device__ static __forceinline__ uint32_t load_chunk(int row, int lane) {
     return uint32_t((lane % (D / 8)) ^ tile_swz<D>(row)) << 4;
   }
-  // operand of 32 consecutive rows (row = l % 32), contraction step ks: 8 elements from 16 ks + 8 (l / 32)
-  __device__ static __forceinline__ uint4 rows32(const lds_char_t* tile, int row0, int ks, int lane) {
-    const int row = row0 + (lane & 31);
-    return lds_read16(tile + row * kRowBytes + (((2 * ks + (lane >> 5)) ^ tile_swz<D>(row)) << 4));
+  // Operand addresses.  A chunk's position is c ^ f(r) and f looks at r % 16 only, so that the bytes of step ks (or of
+  // dimensions 32 dt ..) are the lane's first address with some of its low bits flipped: one XOR each from a base that
+  // is formed once -- and re-formed by `fresh` in every tile, or the compiler would keep all of them in registers.
+  struct Bases {
+    int rows, cols;
+    __device__ __forceinline__ Bases(int lane) {
+      const int row = lane & 31, hb = lane >> 5, i = lane & 15, r = 4 * hb + (i >> 2);
+      rows = row * kRowBytes + ((hb ^ tile_swz<D>(row)) << 4);
+      cols = r * kRowBytes + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ tile_swz<D>(r)) << 4) + (i & 1) * 8;
+    }
+    __device__ __forceinline__ Bases fresh(int offset) const {
+      Bases b = *this;
+      b.rows += offset;
+      b.cols += offset;
+      asm volatile("" : "+v"(b.rows), "+v"(b.cols));
+      return b;
+    }
+  };
+  // 32 rows from row0 (row = l % 32), contraction step ks: 8 elements from 16 ks + 8 (l / 32)
+  __device__ static __forceinline__ uint4 rows32(const lds_char_t* tile, int base, int row0, int ks) {
+    return lds_read16(tile + (base ^ (ks << 5)) + row0 * kRowBytes);
   }
-  // transposed operand: dimensions 32 dt + l % 32, contraction over the 16 rows from row0 in the order 0-3, 8-11 | 4-7, 12-15
-  __device__ static __forceinline__ uint4 cols32(const lds_char_t* tile, int row0, int dt, int lane) {
-    const int i = lane & 15, c = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-    const int r = row0 + 4 * (lane >> 5) + (i >> 2);
-    const lds_char_t* p = tile + r * kRowBytes + ((c ^ tile_swz<D>(r)) << 4) + (i & 1) * 8;
-    const lds_char_t* q = tile + (r + 8) * kRowBytes + ((c ^ tile_swz<D>(r + 8)) << 4) + (i & 1) * 8;
-    return tr_pair(p, q);
+  // transposed: dimensions 32 dt + l % 32, contraction over the 16 rows from row0 in the order 0-3, 8-11 | 4-7, 12-15
+  // (f(r + 8) = f(r) ^ 2)
+  __device__ static __forceinline__ uint4 cols32(const lds_char_t* tile, int base, int row0, int dt) {
+    return tr_pair(tile + (base ^ (dt << 6)) + row0 * kRowBytes, tile + (base ^ (dt << 6) ^ 32) + (row0 + 8) * kRowBytes);
   }
 };
 
-// Scores of a block of 32 keys in base 2, in place: raw products in, x out (terms.hpp); with SLACK also 1 - tanh^2.
-// dist0 = pos - (first key of the block) - 4 (l / 32), slope2 = slope log2 e.  Register r is key 8 (r / 4) + r % 4 behind that.
-template <int MODE, bool SLACK>
-__device__ __forceinline__ void block_scores(float (&x)[16], float (&slack)[16], float in, float out, float dist0, float slope2) {
+// Score arithmetic of a launch (base 2, see Score in terms.hpp): with y = raw in and w = y^2 the small-argument cap is
+// y (c0 + w (c1 + w (..))), the polynomial's coefficients times `out`; it serves |raw| <= zmax (|y| <= 1/2).
+// 1 - tanh^2 = 1 - k2 x^2 from the capped score x.
+struct TileScore {
+  float in, out, c1, c2, c3, c4, c5, zmax, k2;
+};
+
+inline TileScore tile_score(float sm_scale, float softcap) {
+  TileScore t{};
+  if (!(softcap > 0.f)) {
+    t.in = sm_scale * kLog2e;
+    t.out = 1.f;
+    return t;
+  }
+  t.in = sm_scale / softcap;
+  t.out = softcap * kLog2e;
+  t.k2 = 1.f / t.out / t.out;
+  t.c1 = -0.333333328f * t.out;
+  t.c2 = 0.133332274f * t.out;
+  t.c3 = -0.0539337893f * t.out;
+  t.c4 = 0.021472721f * t.out;
+  t.c5 = -0.00694700312f * t.out;
+  t.zmax = kTanhSmall / t.in;
+  return t;
+}
+
+__device__ __forceinline__ float capped_small(const TileScore& k, float y) {
+  const float w = y * y;
+  float p = fmaf(w, k.c5, k.c4);
+  p = fmaf(w, p, k.c3);
+  p = fmaf(w, p, k.c2);
+  p = fmaf(w, p, k.c1);
+  return fmaf(w, p, k.out);  // times y
+}
+
+typedef float tile_f16v __attribute__((__vector_size__(16 * sizeof(float))));
+// What an MFMA of 8 passes wrote may be read by inline assembly (the maxima below) 11 slots after it at the earliest, and
+// the compiler does not look into assembly: these spend the slots (see mma16.hpp) and take the registers through.
+__device__ __forceinline__ void tile_settle(tile_f16v& a) { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(a)); }
+
+// maximum of 16 registers in 8 instructions (attn_staged.hpp: the assembly spares the quieting of each operand)
+__device__ __forceinline__ float max16(const float (&x)[16], float m) {
+#pragma unroll
+  for (int r = 0; r < 16; r += 2) m = st_max3(m, x[r], x[r + 1]);
+  return m;
+}
+__device__ __forceinline__ float abs_max16(const float (&x)[16]) {
+  float m = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; r += 2) asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[r]), "v"(x[r + 1]));
+  return m;
+}
+
+// Scores of a block of 32 x 32 in place: raw products in; out come the scores in base 2, or, where there is neither cap
+// nor bias, the products as they are (x in = the score).  dist0 = pos - (first key of the block) - 4 (l / 32), slope2 =
+// slope log2 e.  Register r is key (or query) 8 (r / 4) + r % 4 behind that.
+template <int MODE>
+__device__ __forceinline__ void block_scores(float (&x)[16], const TileScore& k, float dist0, float slope2) {
+  auto dist = [&](int r) { return fabsf(dist0 - float(8 * (r >> 2) + (r & 3))); };
   if constexpr (MODE & kModeCap) {
-    float big = 0.f;
+    if (__any(!(abs_max16(x) <= k.zmax))) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] *= in;
-      big = fmaxf(big, fabsf(x[r]));
-    }
-    if (__any(!(big <= kTanhSmall))) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = fabsf(x[r]) <= kTanhSmall ? tanh_small(x[r]) : tanh_large(x[r]);
+      for (int r = 0; r < 16; ++r) {
+        const float y = x[r] * k.in;
+        const float t = fabsf(y) <= kTanhSmall ? tanh_small(y) : tanh_large(y);
+        x[r] = (MODE & kModeBias) ? fmaf(-slope2, dist(r), k.out * t) : k.out * t;
+      }
     } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = tanh_small(x[r]);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      if constexpr (SLACK) slack[r] = fmaf(-x[r], x[r], 1.f);
-      if constexpr (MODE & kModeBias)
-        x[r] = fmaf(-slope2, fabsf(dist0 - float(8 * (r >> 2) + (r & 3))), out * x[r]);
-      else
-        x[r] *= out;
+      for (int r = 0; r < 16; ++r) {
+        const float y = x[r] * k.in, p = capped_small(k, y);
+        x[r] = (MODE & kModeBias) ? fmaf(y, p, -slope2 * dist(r)) : y * p;
+      }
     }
   } else if constexpr (MODE & kModeBias) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = fmaf(-slope2, fabsf(dist0 - float(8 * (r >> 2) + (r & 3))), x[r] * in);
-  } else {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] *= in;
+    for (int r = 0; r < 16; ++r) x[r] = fmaf(-slope2, dist(r), x[r] * k.in);
   }
 }
 
@@ -136,14 +197,14 @@ namespace fm {
 
 // ---- where the rows of a tile lie ------------------------------------------------------------------------
 // contiguous [n][D]: rows behind the last repeat it (their scores are masked)
-template <int D>
+template <int D, int KT>
 struct FlatSource {
   const bf16_t *k, *v;
   int n;
   __device__ __forceinline__ void prefetch(int) {}
   __device__ __forceinline__ void issue(int t, uint32_t lds_k, uint32_t lds_v, int w, int lane) const {
-    typedef TileLds<D> T;
-    const int kp0 = t * kTK;
+    typedef TileLds<D, KT> T;
+    const int kp0 = t * KT;
     const int64_t off = int64_t(kp0) * D;
     const bf16_t* bk = ring_uniform_ptr(k + off);
     const bf16_t* bv = ring_uniform_ptr(v + off);
@@ -179,15 +240,24 @@ struct TileDocs {
   int2 q_doc, wg_doc;
 };
 
+// {min, max} document of a tile of KT keys out of those of 32
+template <int KT>
+__device__ __forceinline__ int2 tile_docs(const int2* kmeta, int t) {
+  if constexpr (KT == 32) return kmeta[t];
+  const int2 a = kmeta[2 * t], b = kmeta[2 * t + 1];
+  return make_int2(min(a.x, b.x), max(a.y, b.y));
+}
+
 struct TileState {
   float m, l;
 };
 
 template <bool F16, int D, int MODE, class Source>
 __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16], const TileQuery& qy, int lim_lo, int lim_hi,
-                                           int wg_lo, int t_begin, int t_end, const TileDocs& docs, float in, float out_scale,
+                                           int wg_lo, int t_begin, int t_end, const TileDocs& docs, const TileScore& score,
                                            lds_char_t* lds, int* dirty_flag, typename Mma<F16>::f16v (&O)[D / 32], TileState& st) {
-  typedef TileLds<D> T;
+  constexpr int KT = fwd_tile_keys<D>(), NB = KT / 32;
+  typedef TileLds<D, KT> T;
   using M = Mma<F16>;
   constexpr int NKS = D / 16, NDT = D / 32;
   constexpr float kLazyGrow = 8.f;  // growth of a running maximum (in powers of two) that is left unfollowed
@@ -214,7 +284,7 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
         const int tt = t + l;
         bool hit = false;
         if (tt < t_end) {
-          const int2 km = docs.kmeta[tt];
+          const int2 km = tile_docs<KT>(docs.kmeta, tt);
           hit = km.y >= docs.wg_doc.x && km.x <= docs.wg_doc.y && km.y >= 0;
         }
         mask = __ballot(hit);
@@ -226,34 +296,34 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
     return t_end;
   };
 
-  auto compute = [&](int t, const lds_char_t* bK, const lds_char_t* bV) {
-    const int kp0 = t * kTK;
+  const typename T::Bases bases(l);
+  auto compute = [&](int t, int offset) {
+    const lds_char_t* bV = lds + T::kBytes;
+    const auto at = bases.fresh(offset);
+    const int kp0 = t * KT;
     if (kp0 >= lim_hi) return;
-    bool masked = kp0 + kTK > lim_lo;
+    bool masked = kp0 + KT > lim_lo;
     if (has_docs) {
-      const int2 km = docs.kmeta[t];
+      const int2 km = tile_docs<KT>(docs.kmeta, t);
       if (km.y < docs.q_doc.x || km.x > docs.q_doc.y) return;
       masked |= km.x != km.y || docs.q_doc.x != docs.q_doc.y;
     }
-    typename M::f16v s[2];
+    float x[NB][16];
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb)
+    for (int sb = 0; sb < NB; ++sb) {
+      typename M::f16v s;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[sb][r] = 0.f;
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks)
+      for (int ks = 0; ks < NKS; ++ks) s = M::m32(T::rows32(lds, at.rows, 32 * sb, ks), qf[ks], s);
+      tile_settle(s);
 #pragma unroll
-      for (int sb = 0; sb < 2; ++sb) s[sb] = M::m32(T::rows32(bK, 32 * sb, ks, l), qf[ks], s[sb]);
-    float x[2][16], none[16];
-#pragma unroll
-    for (int sb = 0; sb < 2; ++sb) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[sb][r] = s[sb][r];
-      block_scores<MODE, false>(x[sb], none, in, out_scale, float(qy.pos - (kp0 + 32 * sb + 4 * hb)), qy.slope2);
+      for (int r = 0; r < 16; ++r) x[sb][r] = s[r];
+      block_scores<MODE>(x[sb], score, float(qy.pos - (kp0 + 32 * sb + 4 * hb)), qy.slope2);
     }
     if (masked) {
 #pragma unroll
-      for (int sb = 0; sb < 2; ++sb)
+      for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int key0 = kp0 + 32 * sb + 8 * r4 + 4 * hb;
@@ -268,12 +338,11 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
           }
         }
     }
-    float mx = x[0][0];
+    float mx = -INFINITY;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[0][r]);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[1][r]);
+    for (int sb = 0; sb < NB; ++sb) mx = max16(x[sb], mx);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if constexpr (MODE == 0) mx *= score.in;  // (in > 0: scaling commutes with the maximum)
     // The running maximum follows only when some query's grew by more than 2^kLazyGrow (or it sees its first key): until
     // then p stays below 2^kLazyGrow against the older maximum, which neither the fp32 sums nor the relative rounding
     // of p notice, and the accumulator's multiplications are spared in most tiles.
@@ -289,12 +358,12 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
       st.m = m_new;
     }
     const float m_sub = st.m == -INFINITY ? 0.f : st.m;
-    uint4 pf[2][2];
+    uint4 pf[NB][2];
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb) {
+    for (int sb = 0; sb < NB; ++sb) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        x[sb][r] = __builtin_amdgcn_exp2f(x[sb][r] - m_sub);
+        x[sb][r] = __builtin_amdgcn_exp2f(MODE == 0 ? fmaf(x[sb][r], score.in, -m_sub) : x[sb][r] - m_sub);
         st.l += x[sb][r];
       }
 #pragma unroll
@@ -303,11 +372,11 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
                                M::pack2(x[sb][8 * h + 4], x[sb][8 * h + 5]), M::pack2(x[sb][8 * h + 6], x[sb][8 * h + 7]));
     }
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb)
+    for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bV, 32 * sb + 16 * h, dt, l), pf[sb][h], O[dt]);
+        for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bV, at.cols, 32 * sb + 16 * h, dt), pf[sb][h], O[dt]);
   };
 
   int t = next(t_begin);
@@ -325,19 +394,18 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
       const uint32_t to = lds0 + uint32_t(par ^ 1) * 2u * T::kBytes;
       src.issue(t_next, to, to + T::kBytes, w, l);
     }
-    const lds_char_t* bK = lds + par * 2 * T::kBytes;
-    const lds_char_t* bV = bK + T::kBytes;
+    const lds_char_t* bV = lds + (par * 2 + 1) * T::kBytes;
     // masked places for some query of the workgroup: are there values that 0 x would not erase?
-    bool wg_masked = t * kTK + kTK > wg_lo;
+    bool wg_masked = t * KT + KT > wg_lo;
     if (has_docs) {
-      const int2 km = docs.kmeta[t];
+      const int2 km = tile_docs<KT>(docs.kmeta, t);
       wg_masked |= km.x != km.y || docs.wg_doc.x != docs.wg_doc.y;
     }
     if (wg_masked) {
 #pragma unroll
       for (int u = 0; u < T::kBytes / 4096; ++u) dirty |= any_nonfinite<F16>(lds_read16(bV + (u * 256 + tid) * 16));
     }
-    compute(t, bK, bV);
+    compute(t, par * 2 * T::kBytes);
     t = t_next;
     par ^= 1;
   }

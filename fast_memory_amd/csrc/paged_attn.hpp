@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_many_kernel(Paged
   const TileDocs docs{nullptr, nullptr, make_int2(0, 0), make_int2(0, 0)};
   typename M::f16v O[D / 32];
   TileState st;
-  const bool again = tile_sweep<F16, D, MODE>(src, qf, qy, lim_lo, lim_hi, wg_lo, j0 / KT, (j1 + KT - 1) / KT, docs, a.score, lds,
+  const bool again = tile_sweep<F16, D, MODE, false>(src, qf, qy, lim_lo, lim_hi, wg_lo, j0 / KT, (j1 + KT - 1) / KT, docs, a.score, lds,
                                               flag, O, st);
   if (again) {
     for (int rr = wr0; rr < min(wr0 + 32, n_rows); ++rr)

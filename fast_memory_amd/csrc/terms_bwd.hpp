@@ -77,6 +77,7 @@ __global__ __launch_bounds__(256) void terms_delta_tile_kernel(const bf16_t* __r
   const int64_t n = is_v ? keys : rows, first = int64_t(is_v ? int(blockIdx.x) - q_blocks : int(blockIdx.x)) * kNormRows;
   const bf16_t* x = is_v ? v : dout;
   float big = 0.f, bigD = 0.f;
+#pragma unroll 4
   for (int i = 4 * w + (l >> 4); i < kNormRows; i += 16) {
     const int64_t row = first + i;
     float s = 0.f, nn = 0.f;
@@ -180,7 +181,7 @@ constexpr int dq_tile_keys() {
 }
 template <int D>
 constexpr size_t dq_lds_bytes() {
-  return 256 + 4 * size_t(TileLds<D, dq_tile_keys<D>()>::kBytes);
+  return 256 + 4 * size_t(TileLds<D, dq_tile_keys<D>()>::kBytes) + 512;
 }
 
 // ---- dq -------------------------------------------------------------------------------------------------
@@ -280,7 +281,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
   bool dirty = false;
   const typename T::Bases bases(l);
   int t = next(0), par = 0;
-  if (t < t_end) src.issue(t, lds0, lds0 + T::kBytes, w, l);
+  const uint32_t lds_docs = lds0 + 4u * T::kBytes;
+  if (t < t_end) {
+    src.issue(t, lds0, lds0 + T::kBytes, w, l);
+    if (has_docs) issue_docs<KT>(a.m.dock, t, lds_docs, w, l);
+  }
   while (t < t_end) {
     const int t_next = next(t + 1);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -288,13 +293,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
     if (t_next < t_end) {
       const uint32_t to = lds0 + uint32_t(par ^ 1) * 2u * T::kBytes;
       src.issue(t_next, to, to + T::kBytes, w, l);
+      if (has_docs) issue_docs<KT>(a.m.dock, t_next, lds_docs + uint32_t(par ^ 1) * 256u, w, l);
     }
     const lds_char_t* bK = lds + par * 2 * T::kBytes;
     const auto at = bases.fresh(par * 2 * T::kBytes);
     const int kp0 = t * KT;
     bool wg_masked = kp0 + KT > wg_lo, masked = kp0 + KT > lim_lo, any = kp0 < lim_hi;
     if (has_docs) {
-      const int2 km = tile_docs<KT>(a.m.kmeta, t);
+      const int2 km = tile_docs_scalar<KT>(a.m.kmeta, t);
       wg_masked |= km.x != km.y || wg_doc.x != wg_doc.y;
       masked |= km.x != km.y || q_doc.x != q_doc.y;
       any = any && km.y >= q_doc.x && km.x <= q_doc.y;
@@ -328,9 +334,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
         if (masked) {
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
-            int4 dk = make_int4(0, 0, 0, 0);
-            if (has_docs) dk = *reinterpret_cast<const int4*>(a.m.dock + key0 + 8 * r4);
-            const int dd[4] = {dk.x, dk.y, dk.z, dk.w};
+            uint4 dk = make_uint4(0, 0, 0, 0);
+            if (has_docs) dk = lds_read16(lds + 4 * T::kBytes + par * 256 + (key0 - kp0 + 8 * r4) * 4);
+            const int dd[4] = {int(dk.x), int(dk.y), int(dk.z), int(dk.w)};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               bool ok = key0 + 8 * r4 + r < lim;
@@ -510,7 +516,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
     if (s_next < s1) issue(s_next, par ^ 1);
     const int g = s / n, qt = nqt - 1 - (s - g * n), hq = hk * a.G + g;
     const int i0 = qt * kDkvQ;
-    const float slope2 = (MODE & kModeBias) ? a.t.slopes[hq] * kLog2e : 0.f;
+    const float slope2 = (MODE & kModeBias) ? scalar_load(a.t.slopes, hq) * kLog2e : 0.f;
     const lds_char_t* bQ = lds + par * 2 * T::kBytes;
     const lds_char_t* bD = bQ + T::kBytes;
     const lds_char_t* rows = lds_row + par * 512;
@@ -518,7 +524,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
     int lo, hi;
     bool mixed = false;
     if (a.use_masks) {
-      const int4 x = a.m.qmeta[qt];
+      const int4 x = scalar_load(a.m.qmeta, qt);
       lo = x.x, hi = x.y;
       if (has_docs) mixed = k_doc.x != k_doc.y || x.z != x.w || x.z != k_doc.x || wg_doc.x != wg_doc.y;
     } else {

@@ -15,7 +15,7 @@ namespace fm {
 
 template <int D>
 constexpr size_t tile_lds_bytes() {
-  return 256 + 4 * size_t(TileLds<D, fwd_tile_keys<D>()>::kBytes);
+  return 256 + 4 * size_t(TileLds<D, fwd_tile_keys<D>()>::kBytes) + 512;  // flag, two tiles, their documents
 }
 
 struct FwdTileArgs {
@@ -29,7 +29,7 @@ struct FwdTileArgs {
   TileScore score;
 };
 
-template <bool F16, int D, int MODE>
+template <bool F16, int D, int MODE, bool DOCS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTileArgs a) {
   using M = Mma<F16>;
   extern __shared__ __attribute__((aligned(256))) bf16_t lds_all[];
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
     lim_lo = mine.x, lim_hi = mine.y;
     wg_lo = min(min(q0.x, q1.x), min(q2.x, q3.x));
     wg_hi = max(max(q0.y, q1.y), max(q2.y, q3.y));
-    if (a.t.doc_q) {
+    if constexpr (DOCS) {
       docs.dock = a.m.dock;
       docs.kmeta = a.m.kmeta;
       docs.q_doc = make_int2(mine.z, mine.w);
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
   const FlatSource<D, KT> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
   typename M::f16v O[D / 32];
   TileState st;
-  const bool again = tile_sweep<F16, D, MODE>(src, qf, qy, lim_lo, lim_hi, wg_lo, 0, (wg_hi + KT - 1) / KT, docs, a.score,
+  const bool again = tile_sweep<F16, D, MODE, DOCS>(src, qf, qy, lim_lo, lim_hi, wg_lo, 0, (wg_hi + KT - 1) / KT, docs, a.score,
                                               lds, flag, O, st);
   if (!again) {
     tile_write<F16, D>(O, st, q_ok ? a.out + row * D : nullptr, a.lse + row);
@@ -109,12 +109,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
   }
 }
 
-template <bool F16, int D, int MODE>
-static int launch_terms_fwd(const FwdTileArgs& a, hipStream_t st) {
-  FM_ALLOW_LDS((terms_fwd_kernel<F16, D, MODE>), tile_lds_bytes<D>(), "fm_local_attn_terms_fwd(lds)");
-  hipLaunchKernelGGL((terms_fwd_kernel<F16, D, MODE>), dim3(unsigned(a.H * a.G * ceil_div(a.S, kTQ))), dim3(256),
+template <bool F16, int D, int MODE, bool DOCS>
+static int launch_terms_fwd_docs(const FwdTileArgs& a, hipStream_t st) {
+  FM_ALLOW_LDS((terms_fwd_kernel<F16, D, MODE, DOCS>), tile_lds_bytes<D>(), "fm_local_attn_terms_fwd(lds)");
+  hipLaunchKernelGGL((terms_fwd_kernel<F16, D, MODE, DOCS>), dim3(unsigned(a.H * a.G * ceil_div(a.S, kTQ))), dim3(256),
                      tile_lds_bytes<D>(), st, a);
   return launch_status("fm_local_attn_terms_fwd(tiles)");
+}
+template <bool F16, int D, int MODE>
+static int launch_terms_fwd(const FwdTileArgs& a, hipStream_t st) {
+  return a.t.doc_q ? launch_terms_fwd_docs<F16, D, MODE, true>(a, st) : launch_terms_fwd_docs<F16, D, MODE, false>(a, st);
 }
 
 template <bool F16, int D>

@@ -28,7 +28,7 @@ namespace fm {
 constexpr int kTQ = 128;  // query rows of a workgroup
 // keys of a tile of the forward
 template <int D>
-constexpr int fwd_tile_keys() { return 32; }
+constexpr int fwd_tile_keys() { return D == 256 ? 32 : 64; }
 
 // what the scores have, beside the product: bit 0 the cap, bit 1 the distance bias
 constexpr int kModeCap = 1, kModeBias = 2;
@@ -67,6 +67,25 @@ __device__ __forceinline__ uint4 tr_pair(const lds_char_t* p, const lds_char_t* 
   a.s[0] = lds_read_tr(p);
   a.s[1] = lds_read_tr(q);
   return a.u;
+}
+
+// Loads through the scalar cache, from a place that is the same in the whole wave and that nothing writes meanwhile.  A
+// vector load in a tile's loop would be waited for with all direct loads in flight (they share a counter, in order).
+typedef int tile_int2 __attribute__((ext_vector_type(2)));
+typedef int tile_int4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ int2 scalar_load(const int2* p, int i) {
+  const tile_int2 v = reinterpret_cast<const __attribute__((address_space(4))) tile_int2*>(reinterpret_cast<uintptr_t>(p))[__builtin_amdgcn_readfirstlane(i)];
+  return make_int2(v[0], v[1]);
+}
+__device__ __forceinline__ int4 scalar_load(const int4* p, int i) {
+  const tile_int4 v = reinterpret_cast<const __attribute__((address_space(4))) tile_int4*>(reinterpret_cast<uintptr_t>(p))[__builtin_amdgcn_readfirstlane(i)];
+  return make_int4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ float scalar_load(const float* p, int i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) float*>(reinterpret_cast<uintptr_t>(p))[__builtin_amdgcn_readfirstlane(i)];
+}
+__device__ __forceinline__ int scalar_load(const int32_t* p, int i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p))[__builtin_amdgcn_readfirstlane(i)];
 }
 
 // LDS of one tile of ROWS rows: where a wave's lanes load, and where the operands are read
@@ -164,6 +183,13 @@ __device__ __forceinline__ float abs_max16(const float (&x)[16]) {
   return m;
 }
 
+// maximum over the two halves of the wave, without a round trip through LDS (attn_staged.hpp)
+__device__ __forceinline__ float max_halves(float x) {
+  const unsigned u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return st_max(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 // Scores of a block of 32 x 32 in place: raw products in; out come the scores in base 2, or, where there is neither cap
 // nor bias, the products as they are (x in = the score).  dist0 = pos - (first key of the block) - 4 (l / 32), slope2 =
 // slope log2 e.  Register r is key (or query) 8 (r / 4) + r % 4 behind that.
@@ -247,12 +273,23 @@ __device__ __forceinline__ int2 tile_docs(const int2* kmeta, int t) {
   const int2 a = kmeta[2 * t], b = kmeta[2 * t + 1];
   return make_int2(min(a.x, b.x), max(a.y, b.y));
 }
+template <int KT>
+__device__ __forceinline__ int2 tile_docs_scalar(const int2* kmeta, int t) {
+  if constexpr (KT == 32) return scalar_load(kmeta, t);
+  const int2 a = scalar_load(kmeta, 2 * t), b = scalar_load(kmeta, 2 * t + 1);
+  return make_int2(min(a.x, b.x), max(a.y, b.y));
+}
+// the documents of a tile's keys on their way to LDS beside its rows (wave 3's share)
+template <int KT>
+__device__ __forceinline__ void issue_docs(const int32_t* dock, int t, uint32_t lds_addr, int w, int lane) {
+  if (w == 3) ring_load4(lds_addr, uint32_t(min(lane, KT - 1)) * 4u, ring_uniform_ptr(dock + int64_t(t) * KT));
+}
 
 struct TileState {
   float m, l;
 };
 
-template <bool F16, int D, int MODE, class Source>
+template <bool F16, int D, int MODE, bool DOCS, class Source>
 __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16], const TileQuery& qy, int lim_lo, int lim_hi,
                                            int wg_lo, int t_begin, int t_end, const TileDocs& docs, const TileScore& score,
                                            lds_char_t* lds, int* dirty_flag, typename Mma<F16>::f16v (&O)[D / 32], TileState& st) {
@@ -264,6 +301,12 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
   const int tid = threadIdx.x, l = tid & 63, hb = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds)));
+  lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+  lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
+  wg_lo = __builtin_amdgcn_readfirstlane(wg_lo);
+  t_end = __builtin_amdgcn_readfirstlane(t_end);
+  const int qd_lo = __builtin_amdgcn_readfirstlane(docs.q_doc.x), qd_hi = __builtin_amdgcn_readfirstlane(docs.q_doc.y);
+  const int wd_lo = __builtin_amdgcn_readfirstlane(docs.wg_doc.x), wd_hi = __builtin_amdgcn_readfirstlane(docs.wg_doc.y);
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -271,23 +314,18 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
   st.m = -INFINITY;
   st.l = 0.f;
   bool dirty = false;
-  const bool has_docs = docs.dock != nullptr;
 
   // the next tile at or behind t that some query of the workgroup sees a document of
   int mask_at = -64;
   unsigned long long mask = 0;
   auto next = [&](int t) {
-    if (!has_docs) return t;
+    if constexpr (!DOCS) return t;
     while (t < t_end) {
       if (t >= mask_at + 64 || mask_at < 0) {
         mask_at = t;
-        const int tt = t + l;
-        bool hit = false;
-        if (tt < t_end) {
-          const int2 km = tile_docs<KT>(docs.kmeta, tt);
-          hit = km.y >= docs.wg_doc.x && km.x <= docs.wg_doc.y && km.y >= 0;
-        }
-        mask = __ballot(hit);
+        const int tt = min(t + l, t_end - 1);
+        const int2 km = tile_docs<KT>(docs.kmeta, tt);
+        mask = __ballot(t + l < t_end && km.y >= wd_lo && km.x <= wd_hi && km.y >= 0);
       }
       const unsigned long long m = mask >> (t - mask_at);
       if (m) return t + __ffsll(m) - 1;
@@ -297,17 +335,17 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
   };
 
   const typename T::Bases bases(l);
-  auto compute = [&](int t, int offset) {
-    const lds_char_t* bV = lds + T::kBytes;
-    const auto at = bases.fresh(offset);
+  auto compute = [&](int t, int buf, int2 km) {
+    const lds_char_t* bK = lds + buf * 2 * T::kBytes;
+    const lds_char_t* bV = bK + T::kBytes;
     const int kp0 = t * KT;
     if (kp0 >= lim_hi) return;
     bool masked = kp0 + KT > lim_lo;
-    if (has_docs) {
-      const int2 km = tile_docs<KT>(docs.kmeta, t);
-      if (km.y < docs.q_doc.x || km.x > docs.q_doc.y) return;
-      masked |= km.x != km.y || docs.q_doc.x != docs.q_doc.y;
+    if constexpr (DOCS) {
+      if (km.y < qd_lo || km.x > qd_hi) return;
+      masked |= km.x != km.y || qd_lo != qd_hi;
     }
+    const auto at = bases.fresh(0);
     float x[NB][16];
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
@@ -315,7 +353,7 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) s = M::m32(T::rows32(lds, at.rows, 32 * sb, ks), qf[ks], s);
+      for (int ks = 0; ks < NKS; ++ks) s = M::m32(T::rows32(bK, at.rows, 32 * sb, ks), qf[ks], s);
       tile_settle(s);
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[sb][r] = s[r];
@@ -327,13 +365,13 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int key0 = kp0 + 32 * sb + 8 * r4 + 4 * hb;
-          int4 dk = make_int4(0, 0, 0, 0);
-          if (has_docs) dk = *reinterpret_cast<const int4*>(docs.dock + key0);
-          const int dd[4] = {dk.x, dk.y, dk.z, dk.w};
+          uint4 dk = make_uint4(0, 0, 0, 0);
+          if constexpr (DOCS) dk = lds_read16(lds + 4 * T::kBytes + buf * 256 + (key0 - kp0) * 4);
+          const int dd[4] = {int(dk.x), int(dk.y), int(dk.z), int(dk.w)};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             bool ok = key0 + r < qy.lim;
-            if (has_docs) ok = ok && dd[r] == qy.doc;
+            if constexpr (DOCS) ok = ok && dd[r] == qy.doc;
             if (!ok) x[sb][4 * r4 + r] = -INFINITY;
           }
         }
@@ -341,7 +379,7 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
     float mx = -INFINITY;
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) mx = max16(x[sb], mx);
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = max_halves(mx);
     if constexpr (MODE == 0) mx *= score.in;  // (in > 0: scaling commutes with the maximum)
     // The running maximum follows only when some query's grew by more than 2^kLazyGrow (or it sees its first key): until
     // then p stays below 2^kLazyGrow against the older maximum, which neither the fp32 sums nor the relative rounding
@@ -358,9 +396,9 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
       st.m = m_new;
     }
     const float m_sub = st.m == -INFINITY ? 0.f : st.m;
-    uint4 pf[NB][2];
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
+      uint4 pf[2];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         x[sb][r] = __builtin_amdgcn_exp2f(MODE == 0 ? fmaf(x[sb][r], score.in, -m_sub) : x[sb][r] - m_sub);
@@ -368,46 +406,54 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        pf[sb][h] = make_uint4(M::pack2(x[sb][8 * h + 0], x[sb][8 * h + 1]), M::pack2(x[sb][8 * h + 2], x[sb][8 * h + 3]),
-                               M::pack2(x[sb][8 * h + 4], x[sb][8 * h + 5]), M::pack2(x[sb][8 * h + 6], x[sb][8 * h + 7]));
-    }
-#pragma unroll
-    for (int sb = 0; sb < NB; ++sb)
+        pf[h] = make_uint4(M::pack2(x[sb][8 * h + 0], x[sb][8 * h + 1]), M::pack2(x[sb][8 * h + 2], x[sb][8 * h + 3]),
+                           M::pack2(x[sb][8 * h + 4], x[sb][8 * h + 5]), M::pack2(x[sb][8 * h + 6], x[sb][8 * h + 7]));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bV, at.cols, 32 * sb + 16 * h, dt), pf[sb][h], O[dt]);
+        for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bV, at.cols, 32 * sb + 16 * h, dt), pf[h], O[dt]);
+    }
   };
 
+  const uint32_t lds_docs = lds0 + 4u * T::kBytes;
   int t = next(t_begin);
   if (t < t_end) {
     src.prefetch(t);
     src.issue(t, lds0, lds0 + T::kBytes, w, l);
+    if constexpr (DOCS) issue_docs<KT>(docs.dock, t, lds_docs, w, l);
+    src.prefetch(t + 1);
   }
-  int par = 0;
-  while (t < t_end) {
+  auto step = [&](int buf) {
     const int t_next = next(t + 1);
-    if (t_next < t_end) src.prefetch(t_next);
+    int2 km = make_int2(0, 0);
+    if constexpr (DOCS) km = tile_docs_scalar<KT>(docs.kmeta, t);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     ring_barrier();  // tile t is in place, and every wave has finished the tile before it, whose buffer is free
     if (t_next < t_end) {
-      const uint32_t to = lds0 + uint32_t(par ^ 1) * 2u * T::kBytes;
+      const uint32_t to = lds0 + uint32_t(buf ^ 1) * 2u * T::kBytes;
       src.issue(t_next, to, to + T::kBytes, w, l);
+      if constexpr (DOCS) issue_docs<KT>(docs.dock, t_next, lds_docs + uint32_t(buf ^ 1) * 256u, w, l);
+      src.prefetch(t_next + 1);  // (what a source looks up for its rows: a tile ahead of them)
     }
-    const lds_char_t* bV = lds + (par * 2 + 1) * T::kBytes;
     // masked places for some query of the workgroup: are there values that 0 x would not erase?
     bool wg_masked = t * KT + KT > wg_lo;
-    if (has_docs) {
-      const int2 km = tile_docs<KT>(docs.kmeta, t);
-      wg_masked |= km.x != km.y || docs.wg_doc.x != docs.wg_doc.y;
-    }
+    if constexpr (DOCS) wg_masked |= km.x != km.y || wd_lo != wd_hi;
     if (wg_masked) {
+      const lds_char_t* bV = lds + (buf * 2 + 1) * T::kBytes;
 #pragma unroll
       for (int u = 0; u < T::kBytes / 4096; ++u) dirty |= any_nonfinite<F16>(lds_read16(bV + (u * 256 + tid) * 16));
     }
-    compute(t, par * 2 * T::kBytes);
+    compute(t, buf, km);
     t = t_next;
-    par ^= 1;
+  };
+  if constexpr (D == 256) {  // (one copy of the step: two would not fit the instruction cache)
+    for (int buf = 0; t < t_end; buf ^= 1) step(buf);
+  } else {  // two tiles a round, so that the buffers are constants
+    while (t < t_end) {
+      step(0);
+      if (t >= t_end) break;
+      step(1);
+    }
   }
   if (dirty) *dirty_flag = 1;  // (every writer writes the same)
   __syncthreads();

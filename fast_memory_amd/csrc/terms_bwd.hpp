@@ -16,6 +16,7 @@
 // fp16: p and g of a long row lie below fp16's normal numbers.  p is held times 2^12; g times 2^e, e from the largest
 // |do_i|_2 max_j |v_j|_2 + |D_i| of the call (a bound of |g|), such that |g| 2^e <= 2^13.  bf16 has fp32's range: e = 0.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "terms_masks.hpp"
@@ -26,7 +27,7 @@ namespace fm {
 typedef int lds_int2 __attribute__((ext_vector_type(2)));
 
 constexpr float kPScaleF16 = 4096.f;
-constexpr int kNormRows = 256;  // rows whose norms a workgroup of the first launch takes the largest of
+constexpr int kNormRows = 64;   // rows whose norms a workgroup of the first launch takes the largest of
 
 struct BwdTileArgs {
   const bf16_t *q, *k, *v, *dout;
@@ -77,7 +78,6 @@ __global__ __launch_bounds__(256) void terms_delta_tile_kernel(const bf16_t* __r
   const int64_t n = is_v ? keys : rows, first = int64_t(is_v ? int(blockIdx.x) - q_blocks : int(blockIdx.x)) * kNormRows;
   const bf16_t* x = is_v ? v : dout;
   float big = 0.f, bigD = 0.f;
-#pragma unroll 4
   for (int i = 4 * w + (l >> 4); i < kNormRows; i += 16) {
     const int64_t row = first + i;
     float s = 0.f, nn = 0.f;
@@ -181,34 +181,39 @@ constexpr int dq_tile_keys() {
 }
 template <int D>
 constexpr size_t dq_lds_bytes() {
-  return 256 + 4 * size_t(TileLds<D, dq_tile_keys<D>()>::kBytes) + 512;
+  return 512 + 4 * size_t(TileLds<D, dq_tile_keys<D>()>::kBytes) + 512;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const float (&x)[16], int h) {
+  using M = Mma<F16>;
+  return make_uint4(M::pack2(x[8 * h + 0], x[8 * h + 1]), M::pack2(x[8 * h + 2], x[8 * h + 3]),
+                    M::pack2(x[8 * h + 4], x[8 * h + 5]), M::pack2(x[8 * h + 6], x[8 * h + 7]));
 }
 
 // ---- dq -------------------------------------------------------------------------------------------------
-template <bool F16, int D, int MODE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTileArgs a) {
+template <bool F16, int D, int MODE, bool DOCS>
+__device__ __forceinline__ void dq_block(const BwdTileArgs& a, int block, bf16_t* lds_all) {
   using M = Mma<F16>;
   constexpr int KT = dq_tile_keys<D>(), NB = KT / 32;
   typedef TileLds<D, KT> T;
   typedef typename std::conditional<F16, f16_t, bf16_t>::type E;
   constexpr int NKS = D / 16, NDT = D / 32;
-  extern __shared__ __attribute__((aligned(256))) bf16_t lds_all[];
   int* flag = reinterpret_cast<int*>(lds_all);
-  lds_char_t* lds = (lds_char_t*)(lds_all + 128);
+  lds_char_t* lds = (lds_char_t*)(lds_all + 256);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds)));
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5;
   if (tid == 0) *flag = 0;
   float g_scale = 1.f;
   if constexpr (F16) g_scale = grad_scale(a, reinterpret_cast<float*>(lds_all) + 16);
   __syncthreads();
-  const int heads = a.H * a.G, bx = int(blockIdx.x) % heads;
+  const int heads = a.H * a.G, bx = block % heads;
   const int hk = bx % a.H, hq = hk * a.G + bx / a.H;
-  const int qb = (a.S + kTQ - 1) / kTQ - 1 - int(blockIdx.x) / heads;
+  const int qb = (a.S + kTQ - 1) / kTQ - 1 - block / heads;
   const int i0 = qb * kTQ, wq0 = i0 + 32 * w, iq = wq0 + col;
   const bool q_ok = iq < a.S;
   const int pos = iq + (a.L - a.S);
-  const float slope2 = (MODE & kModeBias) ? a.t.slopes[hq] * kLog2e : 0.f;
-  const bool has_docs = a.use_masks && a.t.doc_q;
+  const float slope2 = (MODE & kModeBias) ? scalar_load(a.t.slopes, hq) * kLog2e : 0.f;
   int lim, doc = 0, lim_lo, lim_hi, wg_lo, wg_hi;
   int2 q_doc = make_int2(0, 0), wg_doc = make_int2(0, 0);
   if (a.use_masks) {
@@ -231,6 +236,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
   }
   lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
   lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
+  wg_lo = __builtin_amdgcn_readfirstlane(wg_lo);
+  const int qd_lo = __builtin_amdgcn_readfirstlane(q_doc.x), qd_hi = __builtin_amdgcn_readfirstlane(q_doc.y);
+  const int wd_lo = __builtin_amdgcn_readfirstlane(wg_doc.x), wd_hi = __builtin_amdgcn_readfirstlane(wg_doc.y);
 
   const int64_t row = int64_t(hq) * a.S + iq;
   uint4 qf[NKS], df[NKS];
@@ -257,20 +265,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
     for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
 
   FlatSource<D, KT> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
-  const int t_end = (wg_hi + KT - 1) / KT;
+  const int t_end = __builtin_amdgcn_readfirstlane((wg_hi + KT - 1) / KT);
   int mask_at = -64;
   unsigned long long mask = 0;
   auto next = [&](int t) {
-    if (!has_docs) return t;
+    if constexpr (!DOCS) return t;
     while (t < t_end) {
       if (t >= mask_at + 64 || mask_at < 0) {
         mask_at = t;
-        bool hit = false;
-        if (t + l < t_end) {
-          const int2 km = tile_docs<KT>(a.m.kmeta, t + l);
-          hit = km.y >= wg_doc.x && km.x <= wg_doc.y && km.y >= 0;
-        }
-        mask = __ballot(hit);
+        const int2 km = tile_docs<KT>(a.m.kmeta, min(t + l, t_end - 1));
+        mask = __ballot(t + l < t_end && km.y >= wd_lo && km.x <= wd_hi && km.y >= 0);
       }
       const unsigned long long m = mask >> (t - mask_at);
       if (m) return t + __ffsll(m) - 1;
@@ -280,82 +284,93 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dq_kernel(BwdTile
   };
   bool dirty = false;
   const typename T::Bases bases(l);
-  int t = next(0), par = 0;
   const uint32_t lds_docs = lds0 + 4u * T::kBytes;
+  auto compute = [&](int t, int buf, int2 km) {
+    const int kp0 = t * KT;
+    if (kp0 >= lim_hi) return;
+    bool masked = kp0 + KT > lim_lo;
+    if constexpr (DOCS) {
+      if (km.y < qd_lo || km.x > qd_hi) return;
+      masked |= km.x != km.y || qd_lo != qd_hi;
+    }
+    const auto at = bases.fresh(buf * 2 * T::kBytes);
+#pragma unroll
+    for (int sb = 0; sb < NB; ++sb) {
+      typename M::f16v s, p;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f, p[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        s = M::m32(T::rows32(lds, at.rows, 32 * sb, ks), qf[ks], s);
+        p = M::m32(T::rows32(lds + T::kBytes, at.rows, 32 * sb, ks), df[ks], p);
+      }
+      if constexpr ((MODE & kModeCap) != 0) tile_settle(s);
+      float x[16], g[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = s[r];
+      const int key0 = kp0 + 32 * sb + 4 * hb;
+      block_probs<MODE>(x, g, a.score, float(pos - key0), slope2, ColumnQuery{rd.x});
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        g[r] *= p[r] - rd.y;
+        if constexpr (F16) g[r] *= g_scale;
+      }
+      if (masked) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          uint4 dk = make_uint4(0, 0, 0, 0);
+          if constexpr (DOCS) dk = lds_read16(lds + 4 * T::kBytes + buf * 256 + (key0 - kp0 + 8 * r4) * 4);
+          const int dd[4] = {int(dk.x), int(dk.y), int(dk.z), int(dk.w)};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            bool ok = key0 + 8 * r4 + r < lim;
+            if constexpr (DOCS) ok = ok && dd[r] == doc;
+            if (!ok) g[4 * r4 + r] = 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 gf = pack8<F16>(g, h);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(lds, at.cols, 32 * sb + 16 * h, dt), gf, O[dt]);
+      }
+    }
+  };
+  int t = next(0);
   if (t < t_end) {
     src.issue(t, lds0, lds0 + T::kBytes, w, l);
-    if (has_docs) issue_docs<KT>(a.m.dock, t, lds_docs, w, l);
+    if constexpr (DOCS) issue_docs<KT>(a.m.dock, t, lds_docs, w, l);
   }
-  while (t < t_end) {
+  auto step = [&](int buf) {
     const int t_next = next(t + 1);
+    int2 km = make_int2(0, 0);
+    if constexpr (DOCS) km = tile_docs_scalar<KT>(a.m.kmeta, t);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     ring_barrier();
     if (t_next < t_end) {
-      const uint32_t to = lds0 + uint32_t(par ^ 1) * 2u * T::kBytes;
+      const uint32_t to = lds0 + uint32_t(buf ^ 1) * 2u * T::kBytes;
       src.issue(t_next, to, to + T::kBytes, w, l);
-      if (has_docs) issue_docs<KT>(a.m.dock, t_next, lds_docs + uint32_t(par ^ 1) * 256u, w, l);
+      if constexpr (DOCS) issue_docs<KT>(a.m.dock, t_next, lds_docs + uint32_t(buf ^ 1) * 256u, w, l);
     }
-    const lds_char_t* bK = lds + par * 2 * T::kBytes;
-    const auto at = bases.fresh(par * 2 * T::kBytes);
-    const int kp0 = t * KT;
-    bool wg_masked = kp0 + KT > wg_lo, masked = kp0 + KT > lim_lo, any = kp0 < lim_hi;
-    if (has_docs) {
-      const int2 km = tile_docs_scalar<KT>(a.m.kmeta, t);
-      wg_masked |= km.x != km.y || wg_doc.x != wg_doc.y;
-      masked |= km.x != km.y || q_doc.x != q_doc.y;
-      any = any && km.y >= q_doc.x && km.x <= q_doc.y;
-    }
+    bool wg_masked = t * KT + KT > wg_lo;
+    if constexpr (DOCS) wg_masked |= km.x != km.y || wd_lo != wd_hi;
     if (wg_masked) {
+      const lds_char_t* bK = lds + buf * 2 * T::kBytes;
 #pragma unroll
       for (int u = 0; u < T::kBytes / 4096; ++u) dirty |= any_nonfinite<F16>(lds_read16(bK + (u * 256 + tid) * 16));
     }
-    if (any) {
-#pragma unroll
-      for (int sb = 0; sb < NB; ++sb) {
-        typename M::f16v s, p;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f, p[r] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-          s = M::m32(T::rows32(lds, at.rows, 32 * sb, ks), qf[ks], s);
-          p = M::m32(T::rows32(lds + T::kBytes, at.rows, 32 * sb, ks), df[ks], p);
-        }
-        if constexpr ((MODE & kModeCap) != 0) tile_settle(s);
-        float x[16], dp[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = s[r];
-        const int key0 = kp0 + 32 * sb + 4 * hb;
-        block_probs<MODE>(x, dp, a.score, float(pos - key0), slope2, ColumnQuery{rd.x});
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          dp[r] *= p[r] - rd.y;
-          if constexpr (F16) dp[r] *= g_scale;
-        }
-        if (masked) {
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            uint4 dk = make_uint4(0, 0, 0, 0);
-            if (has_docs) dk = lds_read16(lds + 4 * T::kBytes + par * 256 + (key0 - kp0 + 8 * r4) * 4);
-            const int dd[4] = {int(dk.x), int(dk.y), int(dk.z), int(dk.w)};
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              bool ok = key0 + 8 * r4 + r < lim;
-              if (has_docs) ok = ok && dd[r] == doc;
-              if (!ok) dp[4 * r4 + r] = 0.f;
-            }
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 gf = make_uint4(M::pack2(dp[8 * h + 0], dp[8 * h + 1]), M::pack2(dp[8 * h + 2], dp[8 * h + 3]),
-                                      M::pack2(dp[8 * h + 4], dp[8 * h + 5]), M::pack2(dp[8 * h + 6], dp[8 * h + 7]));
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(lds, at.cols, 32 * sb + 16 * h, dt), gf, O[dt]);
-        }
-      }
-    }
+    compute(t, buf, km);
     t = t_next;
-    par ^= 1;
+  };
+  if constexpr (D >= 128) {
+    for (int buf = 0; t < t_end; buf ^= 1) step(buf);
+  } else {
+    while (t < t_end) {
+      step(0);
+      if (t >= t_end) break;
+      step(1);
+    }
   }
   if (dirty) *flag = 1;
   __syncthreads();
@@ -394,15 +409,18 @@ constexpr size_t dkv_lds_bytes() {
   return 512 + size_t(TileLds<D, kDkvKeys>::kBytes) + 4 * size_t(TileLds<D, kDkvQ>::kBytes) + 2 * 2 * kDkvQ * 8;
 }
 
-template <bool F16, int D, int MODE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTileArgs a) {
+// What a block of keys forms.  At head dimension 256 the accumulators of both gradients, 256 registers a lane, leave too
+// few for the rest: dv and dk have workgroups of their own there, and the scores are formed twice.
+constexpr int kDkAndDv = 0, kDvOnly = 1, kDkOnly = 2;
+
+template <bool F16, int D, int MODE, bool DOCS, int PART>
+__device__ __forceinline__ void dkv_block(const BwdTileArgs& a, int block, bf16_t* lds_all) {
   using M = Mma<F16>;
   typedef TileLds<D, kDkvQ> T;
   typedef TileLds<D, kDkvKeys> TV;
   typedef typename std::conditional<F16, f16_t, bf16_t>::type E;
   constexpr int NKS = D / 16, NDT = D / 32;
   constexpr float p_scale = F16 ? kPScaleF16 : 1.f;
-  extern __shared__ __attribute__((aligned(256))) bf16_t lds_all[];
   int* flag = reinterpret_cast<int*>(lds_all);
   lds_char_t* lds_v = (lds_char_t*)(lds_all + 256);
   lds_char_t* lds = lds_v + TV::kBytes;
@@ -416,17 +434,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
   if constexpr (F16) g_scale = grad_scale(a, reinterpret_cast<float*>(lds_all) + 16);
   __syncthreads();
   // the first keys, which a causal mask shows to the most queries, go first
-  const int hk = int(blockIdx.x) % a.H, rest = int(blockIdx.x) / a.H;
+  const int hk = block % a.H, rest = block / a.H;
   const int split = rest % a.splits, j0 = (rest / a.splits) * kDkvKeys;
   const int wj0 = j0 + 32 * w, j = wj0 + col;
   const bool j_ok = j < a.L;
-  const bool has_docs = a.use_masks && a.t.doc_q;
   int doc = 0;
   int2 k_doc = make_int2(0, 0), wg_doc = make_int2(0, 0);  // of the wave's keys, of the workgroup's
-  if (has_docs) {
+  if constexpr (DOCS) {
     doc = a.m.dock[j];
-    const int2 m0 = tile_docs<64>(a.m.kmeta, j0 / 64), m1 = tile_docs<64>(a.m.kmeta, j0 / 64 + 1);
-    k_doc = a.m.kmeta[j0 / 32 + w];
+    const int2 m0 = tile_docs_scalar<64>(a.m.kmeta, j0 / 64), m1 = tile_docs_scalar<64>(a.m.kmeta, j0 / 64 + 1);
+    k_doc = scalar_load(a.m.kmeta, j0 / 32 + w);
     wg_doc = make_int2(min(m0.x, m1.x), max(m0.y, m1.y));
   }
   // keys in registers, values in LDS: with both in registers a wave would need more than half of its SIMD's
@@ -438,7 +455,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
   }
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) asm volatile("" : "+v"(kf[ks].x), "+v"(kf[ks].y), "+v"(kf[ks].z), "+v"(kf[ks].w));
-  {
+  if constexpr (PART != kDvOnly) {
     const bf16_t* bv = ring_uniform_ptr(a.v + (int64_t(hk) * a.L + j0) * D);
 #pragma unroll
     for (int u = 0; u < TV::kLoadsPerWave; ++u) {
@@ -468,13 +485,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
     while (s < s1) {
       if (s >= mask_at + 64 || mask_at < 0) {
         mask_at = s;
-        bool hit = false;
-        if (s + l < s1) {
-          const int qt = nqt - 1 - (s + l) % n;
-          const int4 x = a.m.qmeta[qt];
-          hit = x.y > j0;
-          if (has_docs) hit = hit && wg_doc.y >= 0 && x.w >= wg_doc.x && x.z <= wg_doc.y;
-        }
+        const int4 x = a.m.qmeta[nqt - 1 - min(s + l, s1 - 1) % n];
+        bool hit = s + l < s1 && x.y > j0;
+        if constexpr (DOCS) hit = hit && wg_doc.y >= 0 && x.w >= wg_doc.x && x.z <= wg_doc.y;
         mask = __ballot(hit);
       }
       const unsigned long long m = mask >> (s - mask_at);
@@ -483,56 +496,59 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
     }
     return s1;
   };
-  auto issue = [&](int s, int par) {
-    const int g = s / n, qt = nqt - 1 - (s - g * n), hq = hk * a.G + g;
-    const int i0 = qt * kDkvQ, last = a.S - 1 - i0;
-    const int64_t row = int64_t(hq) * a.S + i0;
+  // a step's head and tile, kept by counting on
+  struct Place {
+    int s, g, qt;
+  };
+  auto place_at = [&](int s) {
+    const int g = n > 0 ? s / n : 0;
+    return Place{s, g, nqt - 1 - (s - g * n)};
+  };
+  auto move_to = [&](Place p, int s) {
+    p.qt -= s - p.s;
+    p.s = s;
+    while (p.qt < qt0) p.qt += n, ++p.g;
+    return p;
+  };
+  const int64_t head0 = int64_t(hk) * a.G * a.S;
+  auto issue = [&](const Place& p, int buf) {
+    const int i0 = p.qt * kDkvQ, last = a.S - 1 - i0;
+    const int64_t row = head0 + (p.g * a.S + i0);
     const bf16_t* bq = ring_uniform_ptr(a.q + row * D);
     const bf16_t* bd = ring_uniform_ptr(a.dout + row * D);
-    const uint32_t to = lds0 + uint32_t(par) * 2u * T::kBytes;
+    const uint32_t to = lds0 + uint32_t(buf) * 2u * T::kBytes;
 #pragma unroll
     for (int u = 0; u < T::kLoadsPerWave; ++u) {
       const int r = T::load_row(w + 4 * u, l);
-      tile_load(to + uint32_t(w + 4 * u) * 1024u, uint32_t(min(r, last)) * T::kRowBytes + T::load_chunk(r, l), bq);
-    }
-#pragma unroll
-    for (int u = 0; u < T::kLoadsPerWave; ++u) {
-      const int r = T::load_row(w + 4 * u, l);
-      tile_load(to + T::kBytes + uint32_t(w + 4 * u) * 1024u, uint32_t(min(r, last)) * T::kRowBytes + T::load_chunk(r, l), bd);
+      const uint32_t voff = uint32_t(min(r, last)) * T::kRowBytes + T::load_chunk(r, l);
+      tile_load(to + uint32_t(w + 4 * u) * 1024u, voff, bq);
+      tile_load(to + T::kBytes + uint32_t(w + 4 * u) * 1024u, voff, bd);
     }
     // 8 bytes a query: wave 0 {lse log2 e, D}, wave 1 {limit, document} where there are masks
     const uint32_t voff = uint32_t(min(l >> 1, last)) * 8u + uint32_t(l & 1) * 4u;
-    if (w == 0) ring_load4(lds_row0 + uint32_t(par) * 512u, voff, ring_uniform_ptr(a.rd + row));
-    if (w == 1 && a.use_masks) ring_load4(lds_row0 + uint32_t(par) * 512u + 256u, voff, ring_uniform_ptr(a.m.qinfo + i0));
+    if (w == 0) ring_load4(lds_row0 + uint32_t(buf) * 512u, voff, ring_uniform_ptr(a.rd + row));
+    if (w == 1 && a.use_masks) ring_load4(lds_row0 + uint32_t(buf) * 512u + 256u, voff, ring_uniform_ptr(a.m.qinfo + i0));
   };
   bool dirty = false;
   const typename T::Bases bases(l);
-  int s = next(s0), par = 0;
-  if (s < s1) issue(s, 0);
-  while (s < s1) {
-    const int s_next = next(s + 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    ring_barrier();
-    if (s_next < s1) issue(s_next, par ^ 1);
-    const int g = s / n, qt = nqt - 1 - (s - g * n), hq = hk * a.G + g;
-    const int i0 = qt * kDkvQ;
-    const float slope2 = (MODE & kModeBias) ? scalar_load(a.t.slopes, hq) * kLog2e : 0.f;
-    const lds_char_t* bQ = lds + par * 2 * T::kBytes;
+  const int L_end = min(j0 + kDkvKeys, a.L);
+  auto compute = [&](const Place& p, int buf, const int4& qm) {
+    const int i0 = p.qt * kDkvQ;
+    const lds_char_t* bQ = lds + buf * 2 * T::kBytes;
     const lds_char_t* bD = bQ + T::kBytes;
-    const lds_char_t* rows = lds_row + par * 512;
+    const lds_char_t* rows = lds_row + buf * 512;
     // who sees what: fewest and most keys of the 32 queries
     int lo, hi;
     bool mixed = false;
     if (a.use_masks) {
-      const int4 x = scalar_load(a.m.qmeta, qt);
-      lo = x.x, hi = x.y;
-      if (has_docs) mixed = k_doc.x != k_doc.y || x.z != x.w || x.z != k_doc.x || wg_doc.x != wg_doc.y;
+      lo = qm.x, hi = qm.y;
+      if constexpr (DOCS) mixed = k_doc.x != k_doc.y || qm.z != qm.w || qm.z != k_doc.x || wg_doc.x != wg_doc.y;
     } else {
       lo = seen_limit(i0 + (a.L - a.S), a.L, a.t.causal, 0);
       hi = seen_limit(min(i0 + 31, a.S - 1) + (a.L - a.S), a.L, a.t.causal, 0);
     }
     const bool ragged = i0 + kDkvQ > a.S;
-    if (ragged || mixed || lo < min(j0 + kDkvKeys, a.L)) {
+    if (ragged || mixed || lo < L_end) {
 #pragma unroll
       for (int u = 0; u < (T::kBytes + 4095) / 4096; ++u) {
         const int at = (u * 256 + tid) * 16;
@@ -540,74 +556,101 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
         dirty |= any_nonfinite<F16>(lds_read16(bQ + at)) | any_nonfinite<F16>(lds_read16(bD + at));
       }
     }
-    if (hi > wj0) {
-      const auto at = bases.fresh(par * 2 * T::kBytes);
-      int vrows = bases.rows + 32 * w * TV::kRowBytes;
-      asm volatile("" : "+v"(vrows));
-      // scores, p, and dv first, then dP, g and dk: of the two products' operands one is held at a time
-      typename M::f16v sc;
+    if (hi <= wj0) return;
+    const float slope2 = (MODE & kModeBias) ? scalar_load(a.t.slopes, hk * a.G + p.g) * kLog2e : 0.f;
+    const auto at = bases.fresh(buf * 2 * T::kBytes);
+    int vrows = bases.rows + 32 * w * TV::kRowBytes;
+    asm volatile("" : "+v"(vrows));
+    // scores, p, and dv first, then dP, g and dk: of the two products' operands one is held at a time
+    typename M::f16v sc;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) sc = M::m32(T::rows32(lds, at.rows, 0, ks), kf[ks], sc);
-      if constexpr ((MODE & kModeCap) != 0) tile_settle(sc);
-      float x[16], y[16];  // p; p slack
+    for (int ks = 0; ks < NKS; ++ks) sc = M::m32(T::rows32(lds, at.rows, 0, ks), kf[ks], sc);
+    if constexpr ((MODE & kModeCap) != 0) tile_settle(sc);
+    float x[16], y[16];  // p; p slack
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = sc[r];
-      const RowQueries rq{rows + 4 * hb * 8};
-      block_probs<MODE>(x, y, a.score, float(j - (i0 + 4 * hb + (a.L - a.S))), slope2, rq);
-      const bool masked = mixed || ragged || wj0 + 32 > lo;
-      if (masked) {
+    for (int r = 0; r < 16; ++r) x[r] = sc[r];
+    const RowQueries rq{rows + 4 * hb * 8};
+    block_probs<MODE>(x, y, a.score, float(j - (i0 + 4 * hb + (a.L - a.S))), slope2, rq);
+    const bool masked = mixed || ragged || wj0 + 32 > lo;
+    if (masked) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int iq = 4 * hb + 8 * (r >> 2) + (r & 3), i = i0 + iq;
-          bool ok = i < a.S;
-          if (a.use_masks) {
-            const lds_int2 qi = *reinterpret_cast<const __attribute__((address_space(3))) lds_int2*>(rows + 256 + iq * 8);
-            ok = ok && j < qi.x && (!has_docs || qi.y == doc);
-          } else {
-            ok = ok && j < seen_limit(i + (a.L - a.S), a.L, a.t.causal, 0);
-          }
-          if (!ok) x[r] = 0.f, y[r] = 0.f;
+      for (int r = 0; r < 16; ++r) {
+        const int iq = 4 * hb + 8 * (r >> 2) + (r & 3), i = i0 + iq;
+        bool ok = i < a.S;
+        if (a.use_masks) {
+          const lds_int2 qi = *reinterpret_cast<const __attribute__((address_space(3))) lds_int2*>(rows + 256 + iq * 8);
+          ok = ok && j < qi.x;
+          if constexpr (DOCS) ok = ok && qi.y == doc;
+        } else {
+          ok = ok && j < seen_limit(i + (a.L - a.S), a.L, a.t.causal, 0);
         }
+        if (!ok) x[r] = 0.f, y[r] = 0.f;
       }
+    }
+    if constexpr (PART != kDkOnly) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if constexpr (F16) {
 #pragma unroll
           for (int r = 0; r < 8; ++r) x[8 * h + r] *= p_scale;
         }
-        const uint4 pf = make_uint4(M::pack2(x[8 * h + 0], x[8 * h + 1]), M::pack2(x[8 * h + 2], x[8 * h + 3]),
-                                    M::pack2(x[8 * h + 4], x[8 * h + 5]), M::pack2(x[8 * h + 6], x[8 * h + 7]));
+        const uint4 pf = pack8<F16>(x, h);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) dV[dt] = M::m32(T::cols32(lds + T::kBytes, at.cols, 16 * h, dt), pf, dV[dt]);
       }
-      typename M::f16v pr;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) pr[r] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks)
-        pr = M::m32(T::rows32(lds + T::kBytes, at.rows, 0, ks), TV::rows32(lds_v, vrows, 0, ks), pr);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        pr[r] = (pr[r] - rq.delta(r)) * y[r];
-        if constexpr (F16) pr[r] *= g_scale;
-      }
-      if (masked) {  // (what is not seen may have made a NaN)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (y[r] == 0.f) pr[r] = 0.f;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 gf = make_uint4(M::pack2(pr[8 * h + 0], pr[8 * h + 1]), M::pack2(pr[8 * h + 2], pr[8 * h + 3]),
-                                    M::pack2(pr[8 * h + 4], pr[8 * h + 5]), M::pack2(pr[8 * h + 6], pr[8 * h + 7]));
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) dK[dt] = M::m32(T::cols32(lds, at.cols, 16 * h, dt), gf, dK[dt]);
-      }
     }
+    if constexpr (PART == kDvOnly) return;
+    typename M::f16v pr;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) pr[r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) pr = M::m32(T::rows32(lds + T::kBytes, at.rows, 0, ks), TV::rows32(lds_v, vrows, 0, ks), pr);
+    float gr[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      gr[r] = (pr[r] - rq.delta(r)) * y[r];
+      if constexpr (F16) gr[r] *= g_scale;
+    }
+    if (masked) {  // (what is not seen may have made a NaN)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (y[r] == 0.f) gr[r] = 0.f;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 gf = pack8<F16>(gr, h);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) dK[dt] = M::m32(T::cols32(lds, at.cols, 16 * h, dt), gf, dK[dt]);
+    }
+  };
+  int s = next(s0);
+  Place here = place_at(min(s, s1 - 1 < s0 ? s0 : s1 - 1));
+  if (s < s1) issue(here, 0);
+  auto step = [&](int buf) {
+    const int s_next = next(s + 1);
+    int4 qm = make_int4(0, 0, 0, 0);
+    if (a.use_masks) qm = scalar_load(a.m.qmeta, here.qt);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    ring_barrier();
+    Place there = here;
+    if (s_next < s1) {
+      there = move_to(here, s_next);
+      issue(there, buf ^ 1);
+    }
+    compute(here, buf, qm);
+    here = there;
     s = s_next;
-    par ^= 1;
+  };
+  if constexpr (D >= 128) {  // (two copies of the step: the accumulators would not fit the registers)
+    for (int buf = 0; s < s1; buf ^= 1) step(buf);
+  } else {
+    while (s < s1) {
+      step(0);
+      if (s >= s1) break;
+      step(1);
+    }
   }
   if (dirty) *flag = 1;
   __syncthreads();
@@ -625,11 +668,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
         const float4 x = make_float4(dK[dt][4 * rq] * fk, dK[dt][4 * rq + 1] * fk, dK[dt][4 * rq + 2] * fk, dK[dt][4 * rq + 3] * fk);
         const float4 y = make_float4(dV[dt][4 * rq] * fv, dV[dt][4 * rq + 1] * fv, dV[dt][4 * rq + 2] * fv, dV[dt][4 * rq + 3] * fv);
         if (a.splits > 1) {
-          *reinterpret_cast<float4*>(a.part + 2 * split * plane + at) = x;
-          *reinterpret_cast<float4*>(a.part + (2 * split + 1) * plane + at) = y;
+          if constexpr (PART != kDvOnly) *reinterpret_cast<float4*>(a.part + 2 * split * plane + at) = x;
+          if constexpr (PART != kDkOnly) *reinterpret_cast<float4*>(a.part + (2 * split + 1) * plane + at) = y;
         } else {
-          *reinterpret_cast<uint2*>(a.dk + at) = make_uint2(M::pack2(x.x, x.y), M::pack2(x.z, x.w));
-          *reinterpret_cast<uint2*>(a.dv + at) = make_uint2(M::pack2(y.x, y.y), M::pack2(y.z, y.w));
+          if constexpr (PART != kDvOnly) *reinterpret_cast<uint2*>(a.dk + at) = make_uint2(M::pack2(x.x, x.y), M::pack2(x.z, x.w));
+          if constexpr (PART != kDkOnly) *reinterpret_cast<uint2*>(a.dv + at) = make_uint2(M::pack2(y.x, y.y), M::pack2(y.z, y.w));
         }
       }
     return;
@@ -650,13 +693,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_dkv_kernel(BwdTil
       const int c = l + 64 * r;
       if (c >= D) continue;
       if (a.splits > 1) {
-        a.part[2 * split * plane + at + c] = kg.k[r] * a.sm_scale;
-        a.part[(2 * split + 1) * plane + at + c] = kg.v[r];
+        if constexpr (PART != kDvOnly) a.part[2 * split * plane + at + c] = kg.k[r] * a.sm_scale;
+        if constexpr (PART != kDkOnly) a.part[(2 * split + 1) * plane + at + c] = kg.v[r];
       } else {
-        Elem<E>::store((E*)a.dk + at + c, kg.k[r] * a.sm_scale);
-        Elem<E>::store((E*)a.dv + at + c, kg.v[r]);
+        if constexpr (PART != kDvOnly) Elem<E>::store((E*)a.dk + at + c, kg.k[r] * a.sm_scale);
+        if constexpr (PART != kDkOnly) Elem<E>::store((E*)a.dv + at + c, kg.v[r]);
       }
     }
+  }
+}
+
+// One launch: the blocks of keys first, heaviest first, then those of queries, which fill the card as the others end.
+template <bool F16, int D, int MODE, bool DOCS>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_bwd_kernel(BwdTileArgs a, int dkv_blocks) {
+  extern __shared__ __attribute__((aligned(256))) bf16_t lds_all[];
+  const int block = blockIdx.x;
+  if constexpr (D == 256) {
+    if (block < dkv_blocks) return dkv_block<F16, D, MODE, DOCS, kDkOnly>(a, block, lds_all);
+    if (block < 2 * dkv_blocks) return dkv_block<F16, D, MODE, DOCS, kDvOnly>(a, block - dkv_blocks, lds_all);
+    dq_block<F16, D, MODE, DOCS>(a, block - 2 * dkv_blocks, lds_all);
+  } else {
+    if (block < dkv_blocks) return dkv_block<F16, D, MODE, DOCS, kDkAndDv>(a, block, lds_all);
+    dq_block<F16, D, MODE, DOCS>(a, block - dkv_blocks, lds_all);
   }
 }
 
@@ -675,20 +733,25 @@ __global__ __launch_bounds__(256) void terms_dkv_join_kernel(const float* __rest
   *reinterpret_cast<uint2*>(to) = make_uint2(Mma<F16>::pack2(s.x, s.y), Mma<F16>::pack2(s.z, s.w));
 }
 
+template <bool F16, int D, int MODE, bool DOCS>
+static int launch_terms_bwd_docs(const BwdTileArgs& a, hipStream_t st) {
+  constexpr size_t lds = std::max(dq_lds_bytes<D>(), dkv_lds_bytes<D>());
+  FM_ALLOW_LDS((terms_bwd_kernel<F16, D, MODE, DOCS>), lds, "fm_local_attn_terms_bwd(lds)");
+  const int dkv = int(a.H * a.splits * ceil_div(a.L, kDkvKeys)), dq = int(a.H * a.G * ceil_div(a.S, kTQ));
+  hipLaunchKernelGGL((terms_bwd_kernel<F16, D, MODE, DOCS>), dim3(unsigned((D == 256 ? 2 : 1) * dkv + dq)), dim3(256), lds, st, a, dkv);
+  return launch_status("fm_local_attn_terms_bwd(tiles)");
+}
+
 template <bool F16, int D, int MODE>
 static int launch_terms_bwd(const BwdTileArgs& a, hipStream_t st) {
-  FM_ALLOW_LDS((terms_dq_kernel<F16, D, MODE>), dq_lds_bytes<D>(), "fm_local_attn_terms_bwd(lds)");
-  FM_ALLOW_LDS((terms_dkv_kernel<F16, D, MODE>), dkv_lds_bytes<D>(), "fm_local_attn_terms_bwd(lds)");
-  hipLaunchKernelGGL((terms_dq_kernel<F16, D, MODE>), dim3(unsigned(a.H * a.G * ceil_div(a.S, kTQ))), dim3(256),
-                     dq_lds_bytes<D>(), st, a);
-  hipLaunchKernelGGL((terms_dkv_kernel<F16, D, MODE>), dim3(unsigned(a.H * a.splits * ceil_div(a.L, kDkvKeys))), dim3(256),
-                     dkv_lds_bytes<D>(), st, a);
+  const int rc = a.t.doc_q ? launch_terms_bwd_docs<F16, D, MODE, true>(a, st) : launch_terms_bwd_docs<F16, D, MODE, false>(a, st);
+  if (rc) return rc;
   if (a.splits > 1) {
     const int64_t plane = int64_t(a.H) * a.L * D;
     hipLaunchKernelGGL((terms_dkv_join_kernel<F16>), dim3(unsigned(ceil_div(2 * plane, 1024))), dim3(256), 0, st, a.part, a.dk,
                        a.dv, plane, a.splits);
   }
-  return launch_status("fm_local_attn_terms_bwd(tiles)");
+  return launch_status("fm_local_attn_terms_bwd(join)");
 }
 
 template <bool F16, int D>

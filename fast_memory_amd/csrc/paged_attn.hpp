@@ -90,11 +90,28 @@ __device__ __forceinline__ void paged_row_again(const PagedTileArgs& a, const Pa
   paged_row_result<E>(a, st, t, hq, piece, pieces);
 }
 
-// the keys of piece i of n, in whole tiles of `tile`
+// the keys of piece i of n, in whole tiles of `tile`; a piece behind the last tile has j0 >= j1 and no tile j0 / tile .. either
 __device__ __forceinline__ void piece_keys(int keys, int tile, int i, int n, int& j0, int& j1) {
   const int tiles = (keys + tile - 1) / tile, each = (tiles + n - 1) / n;
-  j0 = min(i * each * tile, keys);
+  j0 = min(i * each, tiles) * tile;
   j1 = min(j0 + each * tile, keys);
+}
+
+// The row and its first query row that slot s of ROWS query rows stands for: row i owns slots first(i) .. first(i + 1) - 1,
+// first(i) = cu[i] G / ROWS + i: at least as many as it has blocks.
+template <int ROWS>
+__device__ __forceinline__ void paged_slot(const PagedArgs& p, int s, int& row, int& r0) {
+  auto first = [&](int i) { return int(int64_t(max(p.cu[i], 0)) * p.G / ROWS) + i; };
+  int lo = 0, hi = p.R - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first(mid) <= s)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  row = __builtin_amdgcn_readfirstlane(lo);
+  r0 = (s - first(row)) * ROWS;
 }
 
 // ---- few query rows ----------------------------------------------------------------------------------------------
@@ -401,19 +418,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_many_kernel(Paged
   // KV head first: the query blocks of a head run on one XCD and share its pages there
   const int hk = int(blockIdx.x) % a.p.H, rest = int(blockIdx.x) / a.p.H;
   const int piece = rest % a.many_pieces, slot = a.many_slots - 1 - rest / a.many_pieces;  // (a row's last tokens, which see most, first)
-  // Row i owns slots first(i) .. first(i + 1) - 1, first(i) = cu[i] G / 128 + i: at least as many as it has blocks.
-  auto first = [&](int i) { return int(int64_t(max(a.p.cu[i], 0)) * a.p.G / kTQ) + i; };
-  int lo = 0, hi = a.p.R - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first(mid) <= slot)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int row = __builtin_amdgcn_readfirstlane(lo);
+  int row, r0;
+  paged_slot<kTQ>(a.p, slot, row, r0);
   const PagedRow pr = paged_row(a.p, row);
-  const int n = pr.q1 - pr.q0, n_rows = n * a.p.G, r0 = (slot - first(row)) * kTQ;
+  const int n = pr.q1 - pr.q0, n_rows = n * a.p.G;
   if (n <= 0 || n_rows <= a.few_rows || r0 < 0 || r0 >= n_rows) return;
   if (tid == 0) *flag = 0;
   __syncthreads();
@@ -531,6 +539,21 @@ inline PagedPlan paged_plan(int rows, int T, int max_new, int H, int G, int d, i
   y.few_pieces = y.few ? pieces(int64_t(rows) * H) : 1;
   y.many_pieces = y.many ? pieces(std::max<int64_t>(1, int64_t(T) * G / kTQ) * H) : 1;
   y.pieces = std::max(y.few_pieces, y.many_pieces);
+  const size_t units = y.pieces > 1 ? size_t(T) * H * G * y.pieces : 0;
+  y.part_ml = align_up(units * d * 4, 256);
+  y.total = y.part_ml + align_up(units * 8, 256);
+  return y;
+}
+
+// of the fp32 products' kernel: 32 query rows a slot.  What a split costs is a write and a read of d values for each query row and
+// piece, against 512 keys read: little.
+inline PagedPlan paged_f32_plan(int rows, int T, int H, int G, int d, int64_t keys) {
+  PagedPlan y{};
+  y.many = true;
+  y.slots = int(int64_t(T) * G / 32) + rows;
+  const int64_t groups = std::max<int64_t>(std::min<int64_t>(rows, T), int64_t(T) * G / 32) * H;
+  y.few_pieces = 1;
+  y.pieces = y.many_pieces = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(keys, 512), 64), ceil_div(1024, groups))));
   const size_t units = y.pieces > 1 ? size_t(T) * H * G * y.pieces : 0;
   y.part_ml = align_up(units * d * 4, 256);
   y.total = y.part_ml + align_up(units * 8, 256);

@@ -248,24 +248,4 @@ __device__ __forceinline__ void row_dkv_chunk(const T* __restrict__ k, const T* 
   }
 }
 
-// dk and dv of one key: all queries of the G heads that read it, in order
-template <typename T, bool CAP>
-__device__ __forceinline__ void row_dkv(const T* __restrict__ k, const T* __restrict__ v, int j, int hk, int G, int S, int L,
-                                        int d, const T* __restrict__ q, const T* __restrict__ dout,
-                                        const float2* __restrict__ rd, const Terms& t, float sm_scale,
-                                        const Score<CAP>& score, T* __restrict__ dk, T* __restrict__ dv) {
-  const int lane = lane_id();
-  KeyGrads a;
-  key_grads_zero(a);
-  for (int g = 0; g < G; ++g)
-    for (int ib = 0; ib < S; ib += kWave)
-      row_dkv_chunk<T, CAP>(k, v, j, hk * G + g, ib, min(S, ib + kWave), S, L, d, q, dout, rd, t, score, a);
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (lane + 64 * r < d) {
-      Elem<T>::store(dk + lane + 64 * r, a.k[r] * sm_scale);
-      Elem<T>::store(dv + lane + 64 * r, a.v[r]);
-    }
-}
-
 }  // namespace fm

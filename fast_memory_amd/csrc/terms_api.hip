@@ -6,6 +6,8 @@
 
 #include "paged_attn.hpp"
 #include "terms_bwd.hpp"
+#include "paged_f32.hpp"
+#include "terms_f32.hpp"
 #include "terms_fwd.hpp"
 
 namespace fm {
@@ -22,6 +24,15 @@ extern template int terms_bwd_tiles<256>(const BwdTileArgs&, bool, const void*, 
 extern template int paged_tiles<64>(const PagedTileArgs&, const PagedPlan&, int, hipStream_t);
 extern template int paged_tiles<128>(const PagedTileArgs&, const PagedPlan&, int, hipStream_t);
 extern template int paged_tiles<256>(const PagedTileArgs&, const PagedPlan&, int, hipStream_t);
+
+#define FM_EXTERN(T)                                                                            \
+  extern template int terms_f32_fwd<T>(const F32Args&, hipStream_t);                             \
+  extern template int terms_f32_bwd<T>(const F32Args&, const BwdArgs&, float2*, hipStream_t);    \
+  extern template int paged_f32<T>(const PagedTileArgs&, const PagedPlan&, hipStream_t);
+FM_EXTERN(float)
+FM_EXTERN(bf16_t)
+FM_EXTERN(f16_t)
+#undef FM_EXTERN
 
 static bool tiles_take(int d, int dtype) {
   return g_force_generic != 1 && dtype != FM_F32 && (d == 64 || d == 128 || d == 256);
@@ -56,27 +67,28 @@ static int terms_check(const char* name, const FwdArgs& a) {
   return FM_OK;
 }
 
-template <template <typename> class F, typename... A>
-static int by_type(int dtype, A&&... a) {
-  if (dtype == FM_F32) return F<float>::run(a...);
-  if (dtype == FM_BF16) return F<bf16_t>::run(a...);
-  return F<f16_t>::run(a...);
-}
-template <typename T>
-struct FwdRows {
-  static int run(const FwdArgs& a, hipStream_t st) { return terms_fwd_rows<T>(a, st); }
-};
-template <typename T>
-struct BwdRows {
-  static int run(const BwdArgs& a, float2* rd, hipStream_t st) {
-    int rc = terms_delta<T>(a, rd, st);
-    return rc ? rc : terms_bwd_rows<T>(a, rd, st);
+static int terms_fwd_f32(const FwdArgs& f, void* ws, hipStream_t st) {
+  F32Args a{f, nullptr, nullptr, nullptr, nullptr, nullptr, masks_layout(ws, f.S, f.L), f.t.doc_q || f.t.prefix,
+            f32_score(f.sm_scale, f.t.softcap)};
+  if (a.use_masks) {
+    const int rc = make_masks(a.m, f.t, f.S, f.L, st);
+    if (rc) return rc;
   }
-};
-template <typename T>
-struct PagedRows {
-  static int run(const PagedArgs& a, hipStream_t st) { return paged_attn_rows<T>(a, st); }
-};
+  return f.dtype == FM_F32 ? terms_f32_fwd<float>(a, st) : f.dtype == FM_BF16 ? terms_f32_fwd<bf16_t>(a, st) : terms_f32_fwd<f16_t>(a, st);
+}
+static int terms_bwd_f32(const BwdArgs& b, char* ws, size_t masks_at, hipStream_t st) {
+  const FwdArgs& f = b.f;
+  float2* rd = reinterpret_cast<float2*>(ws);
+  F32Args a{f, b.dout, rd, b.dq, b.dk, b.dv, masks_layout(ws + masks_at, f.S, f.L), f.t.doc_q || f.t.prefix,
+            f32_score(f.sm_scale, f.t.softcap)};
+  if (a.use_masks) {
+    const int rc = make_masks(a.m, f.t, f.S, f.L, st);
+    if (rc) return rc;
+  }
+  return f.dtype == FM_F32    ? terms_f32_bwd<float>(a, b, rd, st)
+         : f.dtype == FM_BF16 ? terms_f32_bwd<bf16_t>(a, b, rd, st)
+                              : terms_f32_bwd<f16_t>(a, b, rd, st);
+}
 
 // (the tiled kernels read rows of q, k, v in 16-byte pieces, 8 bytes at a time written)
 static bool aligned16(std::initializer_list<const void*> ptrs) {
@@ -155,7 +167,7 @@ extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void*
   FM_REQUIRE(ws, FM_ERR_ARG, "fm_local_attn_terms_fwd: null pointer");
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_fwd: workspace %zu < %zu", ws_bytes, need);
   if (tiles_take(d, dtype) && aligned16({q, k, v, out})) return terms_fwd_run(a, ws, as_stream(stream));
-  return by_type<FwdRows>(dtype, a, as_stream(stream));
+  return terms_fwd_f32(a, ws, as_stream(stream));
 }
 
 extern "C" size_t fm_local_attn_terms_bwd_workspace(int H, int G, int S, int L, int d, int dtype) {
@@ -178,13 +190,14 @@ extern "C" int fm_local_attn_terms_bwd(const void* q, const void* k, const void*
   const size_t need = fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dtype);
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_bwd: workspace %zu < %zu", ws_bytes, need);
   if (tiles_take(d, dtype) && aligned16({q, k, v, out, dout, dq, dk, dv, ws})) return terms_bwd_run(a, ws, as_stream(stream));
-  return by_type<BwdRows>(dtype, a, static_cast<float2*>(ws), as_stream(stream));
+  return terms_bwd_f32(a, static_cast<char*>(ws), bwd_layout(H, G, S, L, d, dtype).masks, as_stream(stream));
 }
 
 extern "C" size_t fm_paged_attn_fwd_workspace(int rows, int T, int max_new, int H, int G, int d, int width, int page, int dtype) {
   if (rows < 1 || T < 1 || H < 1 || G < 1 || d < 1 || width < 1 || page < 1) return 0;
-  if (dtype == FM_F32) return 256;
-  return std::max<size_t>(256, fm::paged_plan(rows, T, max_new, H, G, d, int64_t(width) * page).total);
+  const int64_t keys = int64_t(width) * page;
+  const size_t tiles = fm::tiles_take(d, dtype) ? fm::paged_plan(rows, T, max_new, H, G, d, keys).total : 0;
+  return std::max<size_t>(256, std::max(tiles, fm::paged_f32_plan(rows, T, H, G, d, keys).total));
 }
 
 extern "C" int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head, const void* k_pages, const void* v_pages,
@@ -211,17 +224,16 @@ extern "C" int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head,
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_paged_attn_fwd: workspace %zu < %zu", ws_bytes, need);
   const PagedArgs a{q, q_token, q_head, k_pages, v_pages, book, n_pages, rows, width, page, log2_exact(page), cu, out, out_token,
                     out_head, lse, lse_token, lse_head, T, H, G, d, sm_scale, softcap, slopes, prefix, dtype};
-  const int64_t e = dtype_bytes(dtype);
-  if (tiles_take(d, dtype) && page >= 16 && aligned16({q, k_pages, v_pages, out, ws}) && q_token * e % 16 == 0 &&
-      q_head * e % 16 == 0 && out_token * e % 8 == 0 && out_head * e % 8 == 0) {
-    const PagedPlan y = paged_plan(rows, T, max_new, H, G, d, int64_t(width) * page);
-    const int64_t groups = int64_t(H) * std::max(int64_t(rows) * y.few_pieces, int64_t(y.slots) * y.many_pieces) + 4;
-    FM_REQUIRE(groups <= 0x7fffffffLL, FM_ERR_UNSUPPORTED, "fm_paged_attn_fwd: %lld workgroups", (long long)groups);
-    char* w = static_cast<char*>(ws);
-    const PagedTileArgs t{a, tile_score(sm_scale, softcap), y.few_rows, y.few_pieces, y.many_pieces, reinterpret_cast<float*>(w),
-                          reinterpret_cast<float2*>(w + y.part_ml), y.pieces, y.slots};
-    hipStream_t st = as_stream(stream);
-    return d == 64 ? paged_tiles<64>(t, y, max_new, st) : d == 128 ? paged_tiles<128>(t, y, max_new, st) : paged_tiles<256>(t, y, max_new, st);
-  }
-  return by_type<PagedRows>(dtype, a, as_stream(stream));
+  const int64_t e = dtype_bytes(dtype), keys = int64_t(width) * page;
+  const bool tiles = tiles_take(d, dtype) && page >= 16 && aligned16({q, k_pages, v_pages, out, ws}) && q_token * e % 16 == 0 &&
+                     q_head * e % 16 == 0 && out_token * e % 8 == 0 && out_head * e % 8 == 0;
+  const PagedPlan y = tiles ? paged_plan(rows, T, max_new, H, G, d, keys) : paged_f32_plan(rows, T, H, G, d, keys);
+  const int64_t groups = int64_t(H) * std::max(int64_t(rows) * y.few_pieces, int64_t(y.slots) * y.many_pieces) + 4;
+  FM_REQUIRE(groups <= 0x7fffffffLL, FM_ERR_UNSUPPORTED, "fm_paged_attn_fwd: %lld workgroups", (long long)groups);
+  char* w = static_cast<char*>(ws);
+  const PagedTileArgs t{a, tile_score(sm_scale, softcap), y.few_rows, y.few_pieces, y.many_pieces, reinterpret_cast<float*>(w),
+                        reinterpret_cast<float2*>(w + y.part_ml), y.pieces, y.slots};
+  hipStream_t st = as_stream(stream);
+  if (!tiles) return dtype == FM_F32 ? paged_f32<float>(t, y, st) : dtype == FM_BF16 ? paged_f32<bf16_t>(t, y, st) : paged_f32<f16_t>(t, y, st);
+  return d == 64 ? paged_tiles<64>(t, y, max_new, st) : d == 128 ? paged_tiles<128>(t, y, max_new, st) : paged_tiles<256>(t, y, max_new, st);
 }

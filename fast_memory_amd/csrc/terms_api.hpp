@@ -71,10 +71,4 @@ __device__ __forceinline__ PagedRow paged_row_of_token(const PagedArgs& a, int t
   return p;
 }
 
-// terms_generic.hip
-template <typename T> int terms_fwd_rows(const FwdArgs& a, hipStream_t st);
-template <typename T> int terms_delta(const BwdArgs& a, float2* rd, hipStream_t st);
-template <typename T> int terms_bwd_rows(const BwdArgs& a, const float2* rd, hipStream_t st);
-template <typename T> int paged_attn_rows(const PagedArgs& a, hipStream_t st);
-
 }  // namespace fm

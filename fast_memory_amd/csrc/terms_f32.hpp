@@ -1,0 +1,634 @@
+// Attention with score terms in fp32 products: fp32 inputs at any head dimension up to 256, and the 16-bit types at the
+// dimensions and page sizes that the 16-bit matrix instructions are not laid out for.  v_mfma_f32_32x32x2_f32.
+//
+// These instructions take 16 times as long as the 16-bit ones for the same product, so that the operands can come straight
+// from global memory (L1 and L2 serve the repeats): no LDS in the sweep, no barriers, every wave on its own.  A workgroup
+// owns 32 queries (or 32 keys) and its four waves take the tiles of 32 on the other side in turn; their sums meet in LDS
+// at the end, in wave order.  Short rows are spread over four waves this way, which is what bounds them.
+//
+//   operand of 32 rows   lane (row l % 32, half l / 32) holds half of the row's dimensions, [0, Dp / 2) or [Dp / 2, Dp): the
+//                        order of a contraction is free, and a lane then reads 16 consecutive bytes for four products
+//   scores               as in terms_tile.hpp: lane column = query (key), register r = row 8 (r / 4) + 4 (l / 32) + r % 4
+//   second product       register r of both halves is the operand of one instruction: rows k and k + 4; its partner is
+//                        one element per lane of those two rows, 32 neighbouring dimensions
+// Head dimensions are padded with zeros to Dp = 32 NDT in registers only.
+#pragma once
+#include <type_traits>
+
+#include "terms_masks.hpp"
+#include "terms_tile.hpp"
+
+namespace fm {
+
+typedef float f32_acc __attribute__((__vector_size__(16 * sizeof(float))));
+__device__ __forceinline__ f32_acc mfma_f32(float a, float b, f32_acc c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32_acc f32_zero() {
+  f32_acc a;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) a[r] = 0.f;
+  return a;
+}
+// the row of register r of a block, without the half's 4 hb
+__device__ __forceinline__ constexpr int f32_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+// four elements of a row from dimension c, zero behind the row's d
+template <typename T, bool VEC>
+__device__ __forceinline__ float4 f32_load4(const T* __restrict__ row, int c, int d) {
+  if constexpr (VEC) {  // d a multiple of 4, rows aligned to four elements
+    if (c >= d) return make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (std::is_same<T, float>::value) {
+      return *reinterpret_cast<const float4*>(row + c);
+    } else {
+      typedef Mma<std::is_same<T, f16_t>::value> M;
+      const uint2 u = *reinterpret_cast<const uint2*>(row + c);
+      return make_float4(M::lo(u.x), M::hi(u.x), M::lo(u.y), M::hi(u.y));
+    }
+  } else {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = c + i < d ? Elem<T>::load(row + c + i) : 0.f;
+    return make_float4(x[0], x[1], x[2], x[3]);
+  }
+}
+
+// this lane's half of a row, to stay in registers
+template <typename T, bool VEC, int NDT>
+__device__ __forceinline__ void f32_resident(float (&x)[16 * NDT], const T* row, bool ok, int d, int hb) {
+#pragma unroll
+  for (int j = 0; j < 4 * NDT; ++j) {
+    const float4 v = ok ? f32_load4<T, VEC>(row, 16 * NDT * hb + 4 * j, d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+  }
+}
+
+// products of 32 streamed rows (this lane's is `row`) with the resident ones.  Sixteen elements are in flight while the
+// products of the sixteen before them run (1024 cycles); the barriers keep the compiler from loading everything at once.
+template <typename T, bool VEC, int NDT>
+__device__ __forceinline__ f32_acc f32_products(const T* row, const float (&x)[16 * NDT], int d, int hb) {
+  f32_acc s = f32_zero();
+  float4 v[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[0][i] = f32_load4<T, VEC>(row, 16 * NDT * hb + 4 * i, d);
+#pragma unroll
+  for (int g = 0; g < NDT; ++g) {
+    if (g + 1 < NDT)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[(g + 1) & 1][i] = f32_load4<T, VEC>(row, 16 * NDT * hb + 16 * (g + 1) + 4 * i, d);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 u = v[g & 1][i];
+      const int j = 16 * g + 4 * i;
+      s = mfma_f32(u.x, x[j], s);
+      s = mfma_f32(u.y, x[j + 1], s);
+      s = mfma_f32(u.z, x[j + 2], s);
+      s = mfma_f32(u.w, x[j + 3], s);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return s;
+}
+
+// acc += sum over the 32 rows of a block of row^T w, w = 16 registers.  offset_of(k): of row k from base, in elements
+template <typename T, int NDT, class OffsetOf>
+__device__ __forceinline__ void f32_accumulate(f32_acc (&acc)[NDT], const float (&w)[16], const T* __restrict__ base,
+                                               const OffsetOf& offset_of, int d, int hb, int col, bool watch, bool& dirty) {
+  constexpr int kRows = 16 / NDT;  // a group: 16 elements
+  float v[2][16];
+  auto load = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const auto at = offset_of(f32_row(kRows * g + i) + 4 * hb);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) v[g & 1][NDT * i + dt] = 32 * dt + col < d ? Elem<T>::load(base + at + (32 * dt + col)) : 0.f;
+    }
+  };
+  load(0);
+#pragma unroll
+  for (int g = 0; g < NDT; ++g) {
+    if (g + 1 < NDT) load(g + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) acc[dt] = mfma_f32(v[g & 1][NDT * i + dt], w[kRows * g + i], acc[dt]);
+    if (watch)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dirty |= !(fabsf(v[g & 1][i]) < INFINITY);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// score arithmetic, chosen at run time (the products hide it)
+struct F32Score {
+  float in, out;  // terms.hpp; out = 0: no cap
+};
+// x = the block's scores in base 2; slack = 1 - tanh^2 where asked for.  dist: query's place - key's, of register 0, whose
+// sign in r is `along` (-1: registers are keys, 1: queries).
+template <bool SLACK>
+__device__ __forceinline__ void f32_scores(float (&x)[16], float (&slack)[16], const f32_acc& s, const F32Score& score, float slope2,
+                                           int dist, int along) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = s[r] * score.in, slack[r] = 1.f;
+  if (score.out != 0.f) {
+    float big = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(x[r]));
+    const bool small = !__any(!(big <= kTanhSmall));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float large = small ? 0.f : tanh_large(x[r]);
+      const float t = fabsf(x[r]) <= kTanhSmall ? tanh_small(x[r]) : large;
+      if (SLACK) slack[r] = fmaf(-t, t, 1.f);
+      x[r] = score.out * t;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = fmaf(-slope2, fabsf(float(dist + along * f32_row(r))), x[r]);
+}
+__device__ __forceinline__ bool wave_any(bool b) { return __any(b); }
+inline F32Score f32_score(float sm_scale, float softcap) {
+  if (softcap > 0.f) return F32Score{sm_scale / softcap, softcap * kLog2e};
+  return F32Score{sm_scale * kLog2e, 0.f};
+}
+
+struct F32Args {
+  FwdArgs f;
+  const void* dout;
+  const float2* rd;
+  void *dq, *dk, *dv;
+  Masks m;
+  int use_masks;
+  F32Score score;
+};
+
+// {fewest, most keys} and {smallest, largest document} of 32 queries
+__device__ __forceinline__ int4 f32_query_meta(const F32Args& a, int i0) {
+  if (a.use_masks) return a.m.qmeta[i0 / 32];
+  const FwdArgs& f = a.f;
+  return make_int4(seen_limit(i0 + (f.L - f.S), f.L, f.t.causal, 0),
+                   seen_limit(min(i0 + 31, f.S - 1) + (f.L - f.S), f.L, f.t.causal, 0), 0, 0);
+}
+__device__ __forceinline__ int2 f32_query_info(const F32Args& a, int i) {  // {limit, document}
+  if (a.use_masks) return a.m.qinfo[i];
+  return make_int2(i < a.f.S ? seen_limit(i + (a.f.L - a.f.S), a.f.L, a.f.t.causal, 0) : 0, 0);
+}
+
+template <int NDT>
+constexpr size_t f32_lds_bytes(int sums) {
+  return 256 + size_t(sums) * 4 * 32 * (32 * NDT + 4) * 4 + 4 * 32 * 8;
+}
+
+// A wave's sums into LDS ([wave][32][Dp + 4]), then `dims` of a row summed over the waves with weights f
+template <int NDT>
+__device__ __forceinline__ void f32_put(float* lds, const f32_acc (&acc)[NDT], int w, int col, int hb) {
+  float* mine = lds + (w * 32 + col) * (32 * NDT + 4) + 4 * hb;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<float4*>(mine + 32 * dt + 8 * q) = make_float4(acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]);
+}
+template <int NDT>
+__device__ __forceinline__ float f32_get(const float* lds, int row, int c, const float (&f)[4]) {
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) s = fmaf(lds[(w * 32 + row) * (32 * NDT + 4) + c], f[w], s);
+  return s;
+}
+
+// what wave k's sums of a query weigh under the maximum m, and the query's {maximum, sum} over the waves
+__device__ __forceinline__ float f32_weight(const float2* ml, int i, int k, float m) {
+  return __builtin_amdgcn_exp2f(ml[k * 32 + i].x - (m == -INFINITY ? 0.f : m));
+}
+__device__ __forceinline__ float2 f32_meet(const float2* ml, int i) {
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) m = fmaxf(m, ml[k * 32 + i].x);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) l = fmaf(ml[k * 32 + i].y, f32_weight(ml, i, k, m), l);
+  return make_float2(m, l);
+}
+
+// The sweep of a wave over tiles of 32 keys t = first, first + step, .. < t_end of one head.  row_of(j): where key j's row
+// begins, the same function for keys and values.  FLAT: rows follow one another.
+template <typename T, bool VEC, int NDT, bool FLAT, class RowOf, class Docs>
+__device__ __forceinline__ void f32_forward(const float (&qf)[16 * NDT], int pos, int lim, float slope2, int lim_lo, const T* K,
+                                            const T* V, const RowOf& row_of, int n, int first, int step, int t_end, int d,
+                                            const F32Score& score, const Docs& docs, f32_acc (&O)[NDT], float& m, float& sum,
+                                            bool& dirty) {
+  const int l = lane_id(), col = l & 31, hb = l >> 5;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) O[dt] = f32_zero();
+  m = -INFINITY;
+  sum = 0.f;
+  int64_t next = row_of(min(32 * first + col, n - 1));
+  for (int t = first; t < t_end; t += step) {
+    const int kp0 = 32 * t;
+    const int64_t at = next;
+    next = row_of(min(kp0 + 32 * step + col, n - 1));
+    bool masked = kp0 + 32 > lim_lo;
+    if (!docs.meets(t, masked)) continue;
+    masked = wave_any(masked);
+    const f32_acc s = f32_products<T, VEC, NDT>(K + at, qf, d, hb);
+    float x[16], slack[16], mx = -INFINITY;
+    f32_scores<false>(x, slack, s, score, slope2, pos - kp0 - 4 * hb, -1);
+    if (masked) {
+      const unsigned seen = docs.seen(kp0 + 4 * hb, lim);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = seen >> r & 1 ? x[r] : -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.f : m_new;
+    if (__any(m_new > m)) {
+      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      sum *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
+    }
+    m = m_new;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = __builtin_amdgcn_exp2f(x[r] - base);
+      sum += x[r];
+    }
+    if constexpr (FLAT) {
+      const int last = n - 1 - kp0;
+      f32_accumulate<T, NDT>(O, x, V + int64_t(kp0) * d, [&](int k) { return unsigned(min(k, last) * d); }, d, hb, col, masked, dirty);
+    } else {
+      f32_accumulate<T, NDT>(O, x, V, [&](int k) { return __shfl(at, k); }, d, hb, col, masked, dirty);
+    }
+  }
+}
+
+struct F32Docs {
+  const int2* kmeta;
+  const int32_t* dock;
+  int lo, hi, mine;  // of the 32 queries; of this lane's
+  bool has;
+  __device__ __forceinline__ bool meets(int t, bool& masked) const {
+    if (!has) return true;
+    const int2 km = kmeta[t];
+    masked |= km.x != km.y || lo != hi;
+    return wave_any(km.y >= 0 && km.y >= lo && km.x <= hi);
+  }
+  // bit r: the query sees key + f32_row(r); dock is padded to whole tiles
+  __device__ __forceinline__ unsigned seen(int key, int lim) const {
+    unsigned bits = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      int4 dk = make_int4(mine, mine, mine, mine);
+      if (has) dk = *reinterpret_cast<const int4*>(dock + key + 8 * q);
+      const int x[4] = {dk.x, dk.y, dk.z, dk.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bits |= unsigned(int(key + 8 * q + e < lim) & int(x[e] == mine)) << (4 * q + e);
+    }
+    return bits;
+  }
+};
+
+template <typename T, bool VEC, int NDT>
+__global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
+  extern __shared__ __attribute__((aligned(256))) float f32_lds[];
+  int* flag = reinterpret_cast<int*>(f32_lds);
+  float* lds = f32_lds + 64;
+  float2* ml = reinterpret_cast<float2*>(lds + 4 * 32 * (32 * NDT + 4));
+  const FwdArgs& f = a.f;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
+  const int heads = f.H * f.G, bx = int(blockIdx.x) % heads;
+  const int hk = bx % f.H, hq = hk * f.G + bx / f.H;
+  const int i0 = ((f.S + 31) / 32 - 1 - int(blockIdx.x) / heads) * 32, iq = i0 + col;
+  if (tid == 0) *flag = 0;
+  __syncthreads();
+  const bool ok = iq < f.S;
+  const int2 qi = f32_query_info(a, iq);
+  const int4 qm = f32_query_meta(a, i0);
+  const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
+  float qf[16 * NDT];
+  f32_resident<T, VEC, NDT>(qf, (const T*)f.q + (int64_t(hq) * f.S + (ok ? iq : 0)) * d, ok, d, hb);
+  const T* K = (const T*)f.k + int64_t(hk) * f.L * d;
+  const T* V = (const T*)f.v + int64_t(hk) * f.L * d;
+  const F32Docs docs{a.m.kmeta, a.m.dock, qm.z, qm.w, qi.y, f.t.doc_q != nullptr};
+  f32_acc O[NDT];
+  float m, sum;
+  bool dirty = false;
+  f32_forward<T, VEC, NDT, true>(qf, iq + (f.L - f.S), qi.x, slope2, qm.x, K, V, [&](int j) { return int64_t(j) * d; }, f.L, w, 4,
+                           (qm.y + 31) / 32, d, a.score, docs, O, m, sum, dirty);
+  if (dirty) *flag = 1;
+  sum += __shfl_xor(sum, 32);
+  f32_put<NDT>(lds, O, w, col, hb);
+  if (hb == 0) ml[w * 32 + col] = make_float2(m, sum);
+  __syncthreads();
+  if (*flag) {  // values that are not finite, in tiles with masked places: a row at a time (terms.hpp)
+    const KeyRows<T> KR{K, nullptr, 0, 0, 0, d}, VR{V, nullptr, 0, 0, 0, d};
+    for (int i = i0 + w; i < min(i0 + 32, f.S); i += 4) {
+      const int64_t r = int64_t(hq) * f.S + i;
+      const QueryView qv = query_view(f.t, i, f.S, f.L, hq);
+      const RowState rs = f.t.softcap > 0.f
+                              ? row_forward<T, true>((const T*)f.q + r * d, KR, VR, qv, f.t.doc_k, 0, f.L, Score<true>(f.sm_scale, f.t.softcap))
+                              : row_forward<T, false>((const T*)f.q + r * d, KR, VR, qv, f.t.doc_k, 0, f.L, Score<false>(f.sm_scale, 0.f));
+      row_write(rs, d, (T*)f.out + r * d, f.lse + r);
+    }
+    return;
+  }
+  for (int i = w; i < 32 && i0 + i < f.S; i += 4) {  // a wave a query
+    const float2 st = f32_meet(ml, i);
+    float g[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) g[k] = f32_weight(ml, i, k, st.x);
+    const bool none = st.y == 0.f;
+    const float inv = none ? 0.f : 1.f / st.y;
+    const int64_t r = int64_t(hq) * f.S + i0 + i;
+    for (int c = l; c < d; c += 64) Elem<T>::store((T*)f.out + r * d + c, f32_get<NDT>(lds, i, c, g) * inv);
+    if (l == 0) f.lse[r] = none ? -FLT_MAX : (st.x + __builtin_amdgcn_logf(st.y)) * kLn2;
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------
+// {lse_i log2 e, D_i = do_i.o_i - dlse_i}, a wave per row
+template <typename T>
+__global__ __launch_bounds__(256) void terms_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout,
+                                                          const float* __restrict__ lse, const float* __restrict__ dlse,
+                                                          float2* __restrict__ rd, int d, int64_t rows) {
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  float s = 0.f;
+  for (int k = lane_id(); k < d; k += 64) s = fmaf(Elem<T>::load(dout + row * d + k), Elem<T>::load(out + row * d + k), s);
+  s = wave_sum(s);
+  if (lane_id() == 0) rd[row] = make_float2(lse[row] * kLog2e, s - (dlse ? dlse[row] : 0.f));
+}
+
+template <typename T, bool VEC, int NDT>
+__device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float* f32_lds) {
+  int* flag = reinterpret_cast<int*>(f32_lds);
+  float* lds = f32_lds + 64;
+  const FwdArgs& f = a.f;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
+  const int heads = f.H * f.G, bx = block % heads;
+  const int hk = bx % f.H, hq = hk * f.G + bx / f.H;
+  const int i0 = ((f.S + 31) / 32 - 1 - block / heads) * 32, iq = i0 + col;
+  if (tid == 0) *flag = 0;
+  __syncthreads();
+  const bool ok = iq < f.S;
+  const int2 qi = f32_query_info(a, iq);
+  const int4 qm = f32_query_meta(a, i0);
+  const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
+  const int64_t row = int64_t(hq) * f.S + (ok ? iq : 0);
+  float qf[16 * NDT], df[16 * NDT];
+  f32_resident<T, VEC, NDT>(qf, (const T*)f.q + row * d, ok, d, hb);
+  f32_resident<T, VEC, NDT>(df, (const T*)a.dout + row * d, ok, d, hb);
+  const float2 rd = ok ? a.rd[row] : make_float2(0.f, 0.f);
+  const T* K = (const T*)f.k + int64_t(hk) * f.L * d;
+  const T* V = (const T*)f.v + int64_t(hk) * f.L * d;
+  const F32Docs docs{a.m.kmeta, a.m.dock, qm.z, qm.w, qi.y, f.t.doc_q != nullptr};
+  const int pos = iq + (f.L - f.S);
+  f32_acc O[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) O[dt] = f32_zero();
+  bool dirty = false;
+  for (int t = w; t < (qm.y + 31) / 32; t += 4) {
+    const int kp0 = 32 * t;
+    bool masked = kp0 + 32 > qm.x;
+    if (!docs.meets(t, masked)) continue;
+    const int64_t at = int64_t(min(kp0 + col, f.L - 1)) * d;
+    const f32_acc s = f32_products<T, VEC, NDT>(K + at, qf, d, hb);
+    const f32_acc p = f32_products<T, VEC, NDT>(V + at, df, d, hb);
+    float g[16], slack[16];
+    f32_scores<true>(g, slack, s, a.score, slope2, pos - kp0 - 4 * hb, -1);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) g[r] = __builtin_amdgcn_exp2f(g[r] - rd.x) * (p[r] - rd.y) * slack[r];
+    if (masked) {
+      const unsigned seen = docs.seen(kp0 + 4 * hb, qi.x);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) g[r] = seen >> r & 1 ? g[r] : 0.f;
+    }
+    const int last = f.L - 1 - kp0;
+    f32_accumulate<T, NDT>(O, g, K + int64_t(kp0) * d, [&](int k) { return unsigned(min(k, last) * d); }, d, hb, col, masked, dirty);
+  }
+  if (dirty) *flag = 1;
+  f32_put<NDT>(lds, O, w, col, hb);
+  __syncthreads();
+  if (*flag) {
+    const KeyRows<T> KR{K, nullptr, 0, 0, 0, d}, VR{V, nullptr, 0, 0, 0, d};
+    for (int i = i0 + w; i < min(i0 + 32, f.S); i += 4) {
+      const int64_t r = int64_t(hq) * f.S + i;
+      const QueryView qv = query_view(f.t, i, f.S, f.L, hq);
+      const T *q = (const T*)f.q + r * d, *o = (const T*)a.dout + r * d;
+      T* to = (T*)a.dq + r * d;
+      if (f.t.softcap > 0.f)
+        row_dq<T, true>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, f.sm_scale, Score<true>(f.sm_scale, f.t.softcap), to);
+      else
+        row_dq<T, false>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, f.sm_scale, Score<false>(f.sm_scale, 0.f), to);
+    }
+    return;
+  }
+  const float one[4] = {1.f, 1.f, 1.f, 1.f};
+  for (int i = w; i < 32 && i0 + i < f.S; i += 4)
+    for (int c = l; c < d; c += 64)
+      Elem<T>::store((T*)a.dq + (int64_t(hq) * f.S + i0 + i) * d + c, f32_get<NDT>(lds, i, c, one) * f.sm_scale);
+}
+
+// dk and dv of 32 keys; PART as in terms_bwd.hpp (both sums and both operands of a padded dimension of 256 are 512 registers)
+constexpr int kF32Both = 0, kF32Dv = 1, kF32Dk = 2;
+
+template <typename T, bool VEC, int NDT, int PART>
+__device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float* f32_lds) {
+  constexpr bool kDk = PART != kF32Dv, kDv = PART != kF32Dk;
+  int* flag = reinterpret_cast<int*>(f32_lds);
+  float* lds = f32_lds + 64;
+  const FwdArgs& f = a.f;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
+  const int hk = block % f.H, j0 = block / f.H * 32, j = j0 + col;
+  if (tid == 0) *flag = 0;
+  __syncthreads();
+  const bool ok = j < f.L, has_docs = f.t.doc_q != nullptr;
+  const int doc = has_docs ? a.m.dock[j] : 0;
+  const int2 km = has_docs ? a.m.kmeta[j0 / 32] : make_int2(0, 0);
+  const int64_t row = (int64_t(hk) * f.L + (ok ? j : 0)) * d;
+  float kf[16 * NDT], vf[kDk ? 16 * NDT : 1];
+  f32_resident<T, VEC, NDT>(kf, (const T*)f.k + row, ok, d, hb);
+  if constexpr (kDk) f32_resident<T, VEC, NDT>(vf, (const T*)f.v + row, ok, d, hb);
+  f32_acc dK[kDk ? NDT : 1], dV[kDv ? NDT : 1];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    if constexpr (kDk) dK[dt] = f32_zero();
+    if constexpr (kDv) dV[dt] = f32_zero();
+  }
+  bool dirty = false;
+  const int nqt = (f.S + 31) / 32;
+  int step = w;  // of the (head, tile of queries) pairs, every fourth is this wave's
+  for (int g = 0; g < f.G; ++g) {
+    const int hq = hk * f.G + g;
+    const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
+    const T* Q = (const T*)f.q + int64_t(hq) * f.S * d;
+    const T* DO = (const T*)a.dout + int64_t(hq) * f.S * d;
+    const float2* RD = a.rd + int64_t(hq) * f.S;
+    for (; step < nqt; step += 4) {
+      const int i0 = (nqt - 1 - step) * 32;
+      const int4 qm = f32_query_meta(a, i0);
+      if (qm.y <= j0) {
+        if (!a.use_masks && f.t.causal) {  // (the tiles behind see still less)
+          step += (nqt - 1 - step) / 4 * 4;
+        }
+        continue;
+      }
+      bool masked = i0 + 32 > f.S || j0 + 32 > qm.x;
+      if (has_docs) {
+        if (km.y < 0 || km.y < qm.z || km.x > qm.w) continue;
+        masked |= km.x != km.y || qm.z != qm.w;
+      }
+      masked = wave_any(masked);
+      const int i = min(i0 + col, f.S - 1);
+      const float2 mine = RD[i];
+      const f32_acc s = f32_products<T, VEC, NDT>(Q + int64_t(i) * d, kf, d, hb);
+      float x[16], y[16];  // p; slack, then g
+      f32_scores<true>(x, y, s, a.score, slope2, i0 + 4 * hb + (f.L - f.S) - j, 1);
+      unsigned seen = 0xffff;
+      if (masked) {
+        seen = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int iq = i0 + f32_row(r) + 4 * hb;
+          const int2 qi = f32_query_info(a, iq);
+          seen |= unsigned(int(iq < f.S) & int(j < qi.x) & int(!has_docs | (qi.y == doc))) << r;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float e = __builtin_amdgcn_exp2f(x[r] - __shfl(mine.x, f32_row(r) + 4 * hb));
+        x[r] = seen >> r & 1 ? e : 0.f;
+      }
+      const int last = f.S - 1 - i0;
+      auto offset = [&](int k) { return unsigned(min(k, last) * d); };
+      if constexpr (kDv) f32_accumulate<T, NDT>(dV, x, DO + int64_t(i0) * d, offset, d, hb, col, masked, dirty);
+      if constexpr (kDk) {
+        const f32_acc p = f32_products<T, VEC, NDT>(DO + int64_t(i) * d, vf, d, hb);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = x[r] * y[r] * (p[r] - __shfl(mine.y, f32_row(r) + 4 * hb));
+          y[r] = seen >> r & 1 ? e : 0.f;
+        }
+        f32_accumulate<T, NDT>(dK, y, Q + int64_t(i0) * d, offset, d, hb, col, masked, dirty);
+      }
+    }
+    step -= nqt;
+  }
+  if (dirty) *flag = 1;
+  if constexpr (kDk) f32_put<NDT>(lds, dK, w, col, hb);
+  __syncthreads();
+  const int last = min(32, f.L - j0);
+  const float one[4] = {1.f, 1.f, 1.f, 1.f};
+  if (*flag) {
+    for (int jj = j0 + w; jj < j0 + last; jj += 4) {
+      const int64_t at = (int64_t(hk) * f.L + jj) * d;
+      KeyGrads kg;
+      key_grads_zero(kg);
+      for (int g = 0; g < f.G; ++g)
+        for (int ib = 0; ib < f.S; ib += kWave) {
+          const T *k = (const T*)f.k + at, *v = (const T*)f.v + at;
+          if (f.t.softcap > 0.f)
+            row_dkv_chunk<T, true>(k, v, jj, hk * f.G + g, ib, min(f.S, ib + kWave), f.S, f.L, d, (const T*)f.q, (const T*)a.dout, a.rd,
+                                   f.t, Score<true>(f.sm_scale, f.t.softcap), kg);
+          else
+            row_dkv_chunk<T, false>(k, v, jj, hk * f.G + g, ib, min(f.S, ib + kWave), f.S, f.L, d, (const T*)f.q, (const T*)a.dout, a.rd,
+                                    f.t, Score<false>(f.sm_scale, 0.f), kg);
+        }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int c = l + 64 * r;
+        if (c >= d) continue;
+        if constexpr (kDk) Elem<T>::store((T*)a.dk + at + c, kg.k[r] * f.sm_scale);
+        if constexpr (kDv) Elem<T>::store((T*)a.dv + at + c, kg.v[r]);
+      }
+    }
+    return;
+  }
+  if constexpr (kDk) {
+    for (int i = w; i < last; i += 4)
+      for (int c = l; c < d; c += 64)
+        Elem<T>::store((T*)a.dk + (int64_t(hk) * f.L + j0 + i) * d + c, f32_get<NDT>(lds, i, c, one) * f.sm_scale);
+  }
+  if constexpr (kDv) {
+    if constexpr (kDk) __syncthreads();
+    f32_put<NDT>(lds, dV, w, col, hb);
+    __syncthreads();
+    for (int i = w; i < last; i += 4)
+      for (int c = l; c < d; c += 64)
+        Elem<T>::store((T*)a.dv + (int64_t(hk) * f.L + j0 + i) * d + c, f32_get<NDT>(lds, i, c, one));
+  }
+}
+
+template <typename T, bool VEC, int NDT>
+__global__ __launch_bounds__(256, 1) void terms_f32_bwd_kernel(F32Args a, int dkv_blocks) {
+  extern __shared__ __attribute__((aligned(256))) float f32_lds[];
+  const int block = blockIdx.x;
+  if constexpr (NDT == 8) {
+    if (block < dkv_blocks) return f32_dkv_block<T, VEC, NDT, kF32Dk>(a, block, f32_lds);
+    if (block < 2 * dkv_blocks) return f32_dkv_block<T, VEC, NDT, kF32Dv>(a, block - dkv_blocks, f32_lds);
+    f32_dq_block<T, VEC, NDT>(a, block - 2 * dkv_blocks, f32_lds);
+  } else {
+    if (block < dkv_blocks) return f32_dkv_block<T, VEC, NDT, kF32Both>(a, block, f32_lds);
+    f32_dq_block<T, VEC, NDT>(a, block - dkv_blocks, f32_lds);
+  }
+}
+
+template <typename T, bool VEC, int NDT>
+static int launch_f32_fwd(const F32Args& a, hipStream_t st) {
+  FM_ALLOW_LDS((terms_f32_fwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_local_attn_terms_fwd(lds)");
+  hipLaunchKernelGGL((terms_f32_fwd_kernel<T, VEC, NDT>), dim3(unsigned(a.f.H * a.f.G * ceil_div(a.f.S, 32))), dim3(256),
+                     f32_lds_bytes<NDT>(1), st, a);
+  return launch_status("fm_local_attn_terms_fwd(f32)");
+}
+template <typename T>
+static int launch_delta(const BwdArgs& a, float2* rd, hipStream_t st) {
+  const int64_t rows = int64_t(a.f.H) * a.f.G * a.f.S;
+  hipLaunchKernelGGL(terms_delta_kernel<T>, dim3(unsigned(ceil_div(rows, 4))), dim3(256), 0, st, (const T*)a.f.out,
+                     (const T*)a.dout, a.f.lse, a.dlse, rd, a.f.d, rows);
+  return launch_status("fm_local_attn_terms_bwd(delta)");
+}
+
+template <typename T, bool VEC, int NDT>
+static int launch_f32_bwd(const F32Args& a, hipStream_t st) {
+  FM_ALLOW_LDS((terms_f32_bwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_local_attn_terms_bwd(lds)");
+  const int dkv = int(a.f.H * ceil_div(a.f.L, 32)), dq = int(a.f.H * a.f.G * ceil_div(a.f.S, 32));
+  hipLaunchKernelGGL((terms_f32_bwd_kernel<T, VEC, NDT>), dim3(unsigned((NDT == 8 ? 2 : 1) * dkv + dq)), dim3(256),
+                     f32_lds_bytes<NDT>(1), st, a, dkv);
+  return launch_status("fm_local_attn_terms_bwd(f32)");
+}
+
+// rows of d elements that can be read four at a time
+template <typename T>
+static bool f32_vec(int d, std::initializer_list<const void*> ptrs) {
+  bool ok = d % 4 == 0;
+  for (const void* p : ptrs) ok = ok && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0;
+  return ok;
+}
+#define FM_F32_BY_DIM(d, vec, F)             \
+  ((d) <= 64    ? ((vec) ? F(true, 2) : F(false, 2)) \
+   : (d) <= 128 ? ((vec) ? F(true, 4) : F(false, 4)) \
+                : ((vec) ? F(true, 8) : F(false, 8)))
+
+template <typename T>
+int terms_f32_fwd(const F32Args& a, hipStream_t st) {
+  const bool vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v});
+#define FM_F(V, N) launch_f32_fwd<T, V, N>(a, st)
+  return FM_F32_BY_DIM(a.f.d, vec, FM_F);
+#undef FM_F
+}
+template <typename T>
+int terms_f32_bwd(const F32Args& a, const BwdArgs& b, float2* rd, hipStream_t st) {
+  const int rc = launch_delta<T>(b, rd, st);
+  if (rc) return rc;
+  const bool vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v, a.dout});
+#define FM_F(V, N) launch_f32_bwd<T, V, N>(a, st)
+  return FM_F32_BY_DIM(a.f.d, vec, FM_F);
+#undef FM_F
+}
+
+}  // namespace fm

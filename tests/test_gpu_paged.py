@@ -311,6 +311,14 @@ def test_long_rows_are_split_and_joined():
     attend_case(28, [6000, 3], [1, 1], 1, 2, 128, 16, torch.float32, {})
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 2, 33, 50]])
+def test_short_rows_beside_a_long_one(dtype, new):
+    # the pieces are cut by the widest row: a short row has fewer tiles of keys than pieces, some of its pieces have none
+    attend_case(32, [5200, 2, 130, 300], new, 1, 2, 64, 16, dtype, {}, max_new=max(new))
+    attend_case(33, [5200, 70, 1025, 65], new, 1, 1, 128, 32, dtype, dict(softcap=20.0))
+
+
 def test_bad_page_numbers_stay_inside_the_pool():
     cache, q, cu, terms, out, lse = attend_case(29, [100, 70], [1, 30], 1, 2, 128, 16, torch.bfloat16, {})
     cache.table[0, 2] = 1 << 30

@@ -536,12 +536,14 @@ def _same_device(*ts) -> None:
 
 
 def _call(fn, like: torch.Tensor, *args) -> None:
-    """One C call on the current stream of ``like``'s device, which need not be the current device."""
-    if like.device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    """One C call on the current stream of ``like``'s device, which need not be the current device.  (The handle is asked
+    for as such: building a Stream object around it takes 5 us, a third of the smallest calls.)"""
+    index = like.device.index
+    if index == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
-        with torch.cuda.device(like.device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _row_ints(t: torch.Tensor, n: int, like: torch.Tensor, what: str) -> torch.Tensor:

@@ -453,8 +453,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_many_kernel(Paged
   const TileDocs docs{nullptr, nullptr, make_int2(0, 0), make_int2(0, 0)};
   typename M::f16v O[D / 32];
   TileState st;
-  const bool again = tile_sweep<F16, D, MODE, false>(src, qf, qy, lim_lo, lim_hi, wg_lo, j0 / KT, (j1 + KT - 1) / KT, docs, a.score, lds,
-                                              flag, O, st);
+  int t0 = j0 / KT, t1 = (j1 + KT - 1) / KT;
+  const bool again = tile_sweep<F16, D, MODE, false>(src, qf, qy, lim_lo, lim_hi, wg_lo, t0, t1, 0, 1, docs, a.score, lds, flag, O, st);
   if (again) {
     for (int rr = wr0; rr < min(wr0 + 32, n_rows); ++rr)
       paged_row_again<E>(a, pr, pr.q0 + rr / a.p.G, hk * a.p.G + rr % a.p.G, j0, j1, piece, a.many_pieces);
@@ -465,16 +465,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_many_kernel(Paged
                        a.p.lse + t * a.p.l_token + hq * a.p.l_head);
     return;
   }
-  const float lsum = st.l + __shfl_xor(st.l, 32);
   if (!ok) return;
   const int64_t at = part_index(a, t, hq, piece);
-#pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-    for (int rq = 0; rq < 4; ++rq)
-      *reinterpret_cast<float4*>(a.part_o + at * D + dt * 32 + 8 * rq + 4 * hb) =
-          make_float4(O[dt][4 * rq], O[dt][4 * rq + 1], O[dt][4 * rq + 2], O[dt][4 * rq + 3]);
-  if (hb == 0) a.part_ml[at] = make_float2(st.m, lsum);
+  tile_write_part<D>(O, st, a.part_o + at * D, a.part_ml + at);
 }
 
 // ---- the pieces of a query row, in order: 16 lanes a row, D / 16 dimensions each -----------------------------------------
@@ -483,39 +476,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedTileArgs a) {
   using M = Mma<F16>;
   const int HG = a.p.H * a.p.G;
   const int64_t unit = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const int t = int(unit / HG), hq = int(unit - int64_t(t) * HG), part = threadIdx.x & 15;
+  const int t = int(unit / HG), hq = int(unit - int64_t(t) * HG);
   if (t >= a.p.T) return;
   const PagedRow pr = paged_row_of_token(a.p, t);
   if (pr.row < 0) return;  // (written where nobody's tokens are)
   const int pieces = (pr.q1 - pr.q0) * a.p.G <= a.few_rows ? a.few_pieces : a.many_pieces;
   if (pieces == 1) return;
-  const float2* ml = a.part_ml + part_index(a, t, hq, 0);
-  const float* po = a.part_o + part_index(a, t, hq, 0) * D;
-  float mt = -INFINITY;
-  for (int i = 0; i < pieces; ++i) mt = fmaxf(mt, ml[i].x);
-  const float base = mt == -INFINITY ? 0.f : mt;
-  float lt = 0.f, o[D / 16];
-#pragma unroll
-  for (int k = 0; k < D / 16; ++k) o[k] = 0.f;
-  for (int i = 0; i < pieces; ++i) {
-    const float2 x = ml[i];
-    const float f = __builtin_amdgcn_exp2f(x.x - base);
-    lt = fmaf(x.y, f, lt);
-#pragma unroll
-    for (int u = 0; u < D / 64; ++u) {
-      const float4 v = *reinterpret_cast<const float4*>(po + int64_t(i) * D + 64 * u + 4 * part);
-      o[4 * u] = fmaf(v.x, f, o[4 * u]), o[4 * u + 1] = fmaf(v.y, f, o[4 * u + 1]);
-      o[4 * u + 2] = fmaf(v.z, f, o[4 * u + 2]), o[4 * u + 3] = fmaf(v.w, f, o[4 * u + 3]);
-    }
-  }
-  const bool none = lt == 0.f;
-  const float inv = none ? 0.f : 1.f / lt;
-  bf16_t* out = (bf16_t*)a.p.out + t * a.p.o_token + hq * a.p.o_head;
-#pragma unroll
-  for (int u = 0; u < D / 64; ++u)
-    *reinterpret_cast<uint2*>(out + 64 * u + 4 * part) =
-        make_uint2(M::pack2(o[4 * u] * inv, o[4 * u + 1] * inv), M::pack2(o[4 * u + 2] * inv, o[4 * u + 3] * inv));
-  if (part == 0) a.p.lse[t * a.p.l_token + hq * a.p.l_head] = none ? -FLT_MAX : (mt + __builtin_amdgcn_logf(lt)) * kLn2;
+  tile_join<F16, D>(a.part_o + part_index(a, t, hq, 0) * D, a.part_ml + part_index(a, t, hq, 0), pieces,
+                    (bf16_t*)a.p.out + t * a.p.o_token + hq * a.p.o_head, a.p.lse + t * a.p.l_token + hq * a.p.l_head);
 }
 
 // ---- host: which launches, how many pieces -----------------------------------------------------------------------------

@@ -174,16 +174,17 @@ __device__ __forceinline__ void row_write(const RowState& st, int d, T* __restri
   if (lane == 0) *lse = none ? -FLT_MAX : (st.m + __builtin_amdgcn_logf(st.l)) * kLn2;
 }
 
-// dq of one query; rd = {lse log2 e, D}
-template <typename T, bool CAP>
+// what keys [j0, j1) leave in dq of one query; rd = {lse log2 e, D}
+template <typename T, bool CAP, typename TO>
 __device__ __forceinline__ void row_dq(const T* __restrict__ q, const T* __restrict__ dout, float2 rd, const KeyRows<T>& K, const KeyRows<T>& V, const QueryView& qv,
-                                       const int32_t* __restrict__ doc_k, float sm_scale, const Score<CAP>& score,
-                                       T* __restrict__ dq) {
+                                       const int32_t* __restrict__ doc_k, int j0, int j1, float sm_scale, const Score<CAP>& score,
+                                       TO* __restrict__ dq) {
   const int lane = lane_id(), d = K.d;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int jb = 0; jb < qv.lim; jb += kWave) {
+  j1 = min(j1, qv.lim);
+  for (int jb = j0; jb < j1; jb += kWave) {
     const int j = jb + lane;
-    const bool ok = j < qv.lim && qv.sees(j, doc_k);
+    const bool ok = j < j1 && qv.sees(j, doc_k);
     float g = 0.f;
     if (ok) {
       float slack;
@@ -203,7 +204,7 @@ __device__ __forceinline__ void row_dq(const T* __restrict__ q, const T* __restr
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (lane + 64 * r < d) Elem<T>::store(dq + lane + 64 * r, acc[r] * sm_scale);
+    if (lane + 64 * r < d) Elem<TO>::store(dq + lane + 64 * r, acc[r] * sm_scale);
 }
 
 // The share of the at most 64 queries [i0, i1) of head hq in one key's gradients (not yet times sm_scale): lane = query, then dimension.

@@ -38,9 +38,34 @@ static bool tiles_take(int d, int dtype) {
   return g_force_generic != 1 && dtype != FM_F32 && (d == 64 || d == 128 || d == 256);
 }
 
+// Into how many pieces the keys of a block of 128 queries are cut: until there are 512 workgroups, two a compute unit, none of
+// less than 8 tiles of 64 keys.  (Blocks that fill half the card stay whole: the partial sums cost more than they gain.)
+static int sweep_pieces(int H, int G, int S, int L, int d, int dtype) {
+  if (!tiles_take(d, dtype)) return 1;
+  const int64_t blocks = int64_t(H) * G * ceil_div(S, kTQ);
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / blocks, ceil_div(L, 512)), 16)));
+}
+
+struct FwdLayout {
+  int pieces;
+  size_t part_o, part_ml, total;
+};
+static FwdLayout fwd_layout(int H, int G, int S, int L, int d, int dtype) {
+  FwdLayout y;
+  y.pieces = sweep_pieces(H, G, S, L, d, dtype);
+  const size_t units = y.pieces > 1 ? size_t(H) * G * S * y.pieces : 0;
+  y.part_o = masks_layout(nullptr, S, L).bytes;
+  y.part_ml = y.part_o + align_up(units * d * 4, 256);
+  y.total = y.part_ml + align_up(units * 8, 256);
+  return y;
+}
+
 static int terms_fwd_run(const FwdArgs& a, void* ws, hipStream_t st) {
+  const FwdLayout y = fwd_layout(a.H, a.G, a.S, a.L, a.d, a.dtype);
+  char* p = static_cast<char*>(ws);
   FwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (bf16_t*)a.out, a.lse, a.t, masks_layout(ws, a.S, a.L),
-                a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, a.sm_scale, tile_score(a.sm_scale, a.t.softcap)};
+                a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, a.sm_scale, tile_score(a.sm_scale, a.t.softcap), y.pieces, reinterpret_cast<float*>(p + y.part_o),
+                reinterpret_cast<float2*>(p + y.part_ml)};
   if (t.use_masks) {
     const int rc = make_masks(t.m, a.t, a.S, a.L, st);
     if (rc) return rc;
@@ -101,8 +126,8 @@ static size_t row_data_bytes(int H, int G, int S) { return align_up(size_t(H) * 
 
 // The workspace of a backward: {lse log2 e, D} | masks | norms | partial sums.
 struct BwdLayout {
-  size_t masks, norms, part, total;
-  int n_q_norms, n_k_norms, splits;
+  size_t masks, norms, part, part_dq, total;
+  int n_q_norms, n_k_norms, splits, dq_pieces;
 };
 
 // Into how many pieces the sweeps over the queries are cut: two workgroups a compute unit at least (512 in all), and four
@@ -123,7 +148,9 @@ static BwdLayout bwd_layout(int H, int G, int S, int L, int d, int dtype) {
   b.n_k_norms = int(ceil_div(int64_t(H) * L, kNormRows));
   b.part = b.norms + align_up(size_t(2 * b.n_q_norms + b.n_k_norms) * 4, 256);
   b.splits = (dtype != FM_F32 && (d == 64 || d == 128 || d == 256)) ? dkv_splits(H, G, S, L) : 1;
-  b.total = b.part + (b.splits > 1 ? size_t(b.splits) * 2 * H * L * d * 4 : 0);
+  b.dq_pieces = sweep_pieces(H, G, S, L, d, dtype);
+  b.part_dq = b.part + (b.splits > 1 ? size_t(b.splits) * 2 * H * L * d * 4 : 0);
+  b.total = b.part_dq + (b.dq_pieces > 1 ? size_t(b.dq_pieces) * H * G * S * d * 4 : 0);
   return b;
 }
 
@@ -136,7 +163,7 @@ static int terms_bwd_run(const BwdArgs& b, void* ws, hipStream_t st) {
   BwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (const bf16_t*)b.dout, rd, norms, y.n_q_norms,
                 y.n_k_norms, (bf16_t*)b.dq, (bf16_t*)b.dk, (bf16_t*)b.dv, reinterpret_cast<float*>(p + y.part), a.t,
                 masks_layout(p + y.masks, a.S, a.L), a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, y.splits, a.sm_scale,
-                tile_score(a.sm_scale, a.t.softcap)};
+                tile_score(a.sm_scale, a.t.softcap), y.dq_pieces, reinterpret_cast<float*>(p + y.part_dq)};
   if (t.use_masks) {
     const int rc = make_masks(t.m, a.t, a.S, a.L, st);
     if (rc) return rc;
@@ -151,8 +178,7 @@ static int terms_bwd_run(const BwdArgs& b, void* ws, hipStream_t st) {
 
 extern "C" size_t fm_local_attn_terms_fwd_workspace(int H, int G, int S, int L, int d, int dtype) {
   if (H < 1 || G < 1 || S < 1 || L < 1 || d < 1) return 0;
-  (void)dtype;
-  return fm::masks_layout(nullptr, S, L).bytes;
+  return fm::fwd_layout(H, G, S, L, d, dtype).total;
 }
 
 extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void* v, void* out, float* lse, float softcap,
@@ -166,7 +192,7 @@ extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void*
   const size_t need = fm_local_attn_terms_fwd_workspace(H, G, S, L, d, dtype);
   FM_REQUIRE(ws, FM_ERR_ARG, "fm_local_attn_terms_fwd: null pointer");
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_fwd: workspace %zu < %zu", ws_bytes, need);
-  if (tiles_take(d, dtype) && aligned16({q, k, v, out})) return terms_fwd_run(a, ws, as_stream(stream));
+  if (tiles_take(d, dtype) && aligned16({q, k, v, out, ws})) return terms_fwd_run(a, ws, as_stream(stream));
   return terms_fwd_f32(a, ws, as_stream(stream));
 }
 

@@ -41,6 +41,8 @@ struct BwdTileArgs {
   int use_masks, H, G, S, L, splits;
   float sm_scale;
   TileScore score;
+  int dq_pieces;
+  float* part_dq;      // [dq_pieces][H G][S][D], where dq_pieces > 1
 };
 
 // 2^e for the fp16 gradients of the call, the same in every workgroup
@@ -223,7 +225,7 @@ __device__ __forceinline__ void dq_block(const BwdTileArgs& a, int block, bf16_t
   __syncthreads();
   const int heads = a.H * a.G, bx = block % heads;
   const int hk = bx % a.H, hq = hk * a.G + bx / a.H;
-  const int qb = (a.S + kTQ - 1) / kTQ - 1 - block / heads;
+  const int rest = block / heads, piece = rest % a.dq_pieces, qb = (a.S + kTQ - 1) / kTQ - 1 - rest / a.dq_pieces;
   const int i0 = qb * kTQ, wq0 = i0 + 32 * w, iq = wq0 + col;
   const bool q_ok = iq < a.S;
   const int pos = iq + (a.L - a.S);
@@ -279,7 +281,7 @@ __device__ __forceinline__ void dq_block(const BwdTileArgs& a, int block, bf16_t
     for (int r = 0; r < 16; ++r) O[dt][r] = 0.f;
 
   FlatSource<D, KT> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
-  const int t_end = __builtin_amdgcn_readfirstlane((wg_hi + KT - 1) / KT);
+  int t_end = __builtin_amdgcn_readfirstlane((wg_hi + KT - 1) / KT);
   int mask_at = -64;
   unsigned long long mask = 0;
   auto next = [&](int t) {
@@ -355,7 +357,12 @@ __device__ __forceinline__ void dq_block(const BwdTileArgs& a, int block, bf16_t
       }
     }
   };
-  int t = next(0);
+  int t = next(0), t_begin = 0;
+  if (a.dq_pieces > 1) {
+    tile_piece(t, t_end, piece, a.dq_pieces);
+    t_begin = t;
+    t = next(t);
+  }
   if (t < t_end) {
     src.issue(t, lds0, lds0 + T::kBytes, w, l);
     if constexpr (DOCS) issue_docs<KT>(a.m.dock, t, lds_docs, w, l);
@@ -395,6 +402,16 @@ __device__ __forceinline__ void dq_block(const BwdTileArgs& a, int block, bf16_t
   if (*flag == 0) {
     if (!q_ok) return;
     const float f = a.sm_scale / g_scale;
+    if (a.dq_pieces > 1) {
+      float* to = a.part_dq + (int64_t(piece) * a.H * a.G * a.S + row) * D;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq)
+          *reinterpret_cast<float4*>(to + dt * 32 + 8 * rq + 4 * hb) =
+              make_float4(O[dt][4 * rq] * f, O[dt][4 * rq + 1] * f, O[dt][4 * rq + 2] * f, O[dt][4 * rq + 3] * f);
+      return;
+    }
     bf16_t* to = a.dq + row * D;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
@@ -413,7 +430,13 @@ __device__ __forceinline__ void dq_block(const BwdTileArgs& a, int block, bf16_t
   const Score<(MODE & kModeCap) != 0> score(a.sm_scale, a.t.softcap);
   for (int i = wq0; i < min(wq0 + 32, a.S); ++i) {
     const int64_t r = int64_t(hq) * a.S + i;
-    row_dq<E, (MODE & kModeCap) != 0>((const E*)a.q + r * D, (const E*)a.dout + r * D, a.rd[r], K, V, query_view(a.t, i, a.S, a.L, hq), a.t.doc_k, a.sm_scale, score, (E*)a.dq + r * D);
+    const E *q = (const E*)a.q + r * D, *o = (const E*)a.dout + r * D;
+    const QueryView qv = query_view(a.t, i, a.S, a.L, hq);
+    if (a.dq_pieces > 1)
+      row_dq<E, (MODE & kModeCap) != 0>(q, o, a.rd[r], K, V, qv, a.t.doc_k, t_begin * KT, t_end * KT, a.sm_scale, score,
+                                        a.part_dq + (int64_t(piece) * a.H * a.G * a.S + r) * D);
+    else
+      row_dq<E, (MODE & kModeCap) != 0>(q, o, a.rd[r], K, V, qv, a.t.doc_k, 0, a.L, a.sm_scale, score, (E*)a.dq + r * D);
   }
 }
 
@@ -740,18 +763,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_bwd_kernel(BwdTil
   }
 }
 
-// the pieces' sums in order, each rounded once
+// The pieces' sums in order, each rounded once: dk and dv ([2][plane]) from `part`, then dq from `part_dq`, where they have any.
 template <bool F16>
-__global__ __launch_bounds__(256) void terms_dkv_join_kernel(const float* __restrict__ part, bf16_t* __restrict__ dk,
-                                                             bf16_t* __restrict__ dv, int64_t plane, int splits) {
-  const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
-  if (i >= 2 * plane) return;
-  float4 s = *reinterpret_cast<const float4*>(part + i);
-  for (int k = 1; k < splits; ++k) {
-    const float4 x = *reinterpret_cast<const float4*>(part + 2 * k * plane + i);
+__global__ __launch_bounds__(256) void terms_bwd_join_kernel(BwdTileArgs a, int64_t plane, int64_t plane_q) {
+  int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+  const int64_t kv = a.splits > 1 ? 2 * plane : 0;
+  const float* from = a.part + i;
+  int64_t step = 2 * plane;
+  int n = a.splits;
+  bf16_t* to = i < plane ? a.dk + i : a.dv + (i - plane);
+  if (i >= kv) {
+    i -= kv;
+    if (a.dq_pieces == 1 || i >= plane_q) return;
+    from = a.part_dq + i, step = plane_q, n = a.dq_pieces, to = a.dq + i;
+  }
+  float4 s = *reinterpret_cast<const float4*>(from);
+  for (int k = 1; k < n; ++k) {
+    const float4 x = *reinterpret_cast<const float4*>(from + k * step);
     s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
   }
-  bf16_t* to = i < plane ? dk + i : dv + (i - plane);
   *reinterpret_cast<uint2*>(to) = make_uint2(Mma<F16>::pack2(s.x, s.y), Mma<F16>::pack2(s.z, s.w));
 }
 
@@ -759,7 +789,7 @@ template <bool F16, int D, int MODE, bool DOCS>
 static int launch_terms_bwd_docs(const BwdTileArgs& a, hipStream_t st) {
   constexpr size_t lds = std::max(dq_lds_bytes<D>(), dkv_lds_bytes<D>());
   FM_ALLOW_LDS((terms_bwd_kernel<F16, D, MODE, DOCS>), lds, "fm_local_attn_terms_bwd(lds)");
-  const int dkv = int(a.H * a.splits * ceil_div(a.L, kDkvKeys)), dq = int(a.H * a.G * ceil_div(a.S, kTQ));
+  const int dkv = int(a.H * a.splits * ceil_div(a.L, kDkvKeys)), dq = int(a.H * a.G * ceil_div(a.S, kTQ) * a.dq_pieces);
   hipLaunchKernelGGL((terms_bwd_kernel<F16, D, MODE, DOCS>), dim3(unsigned((D == 256 ? 2 : 1) * dkv + dq)), dim3(256), lds, st, a, dkv);
   return launch_status("fm_local_attn_terms_bwd(tiles)");
 }
@@ -768,10 +798,10 @@ template <bool F16, int D, int MODE>
 static int launch_terms_bwd(const BwdTileArgs& a, hipStream_t st) {
   const int rc = a.t.doc_q ? launch_terms_bwd_docs<F16, D, MODE, true>(a, st) : launch_terms_bwd_docs<F16, D, MODE, false>(a, st);
   if (rc) return rc;
-  if (a.splits > 1) {
-    const int64_t plane = int64_t(a.H) * a.L * D;
-    hipLaunchKernelGGL((terms_dkv_join_kernel<F16>), dim3(unsigned(ceil_div(2 * plane, 1024))), dim3(256), 0, st, a.part, a.dk,
-                       a.dv, plane, a.splits);
+  if (a.splits > 1 || a.dq_pieces > 1) {
+    const int64_t plane = int64_t(a.H) * a.L * D, plane_q = int64_t(a.H) * a.G * a.S * D;
+    const int64_t n = (a.splits > 1 ? 2 * plane : 0) + (a.dq_pieces > 1 ? plane_q : 0);
+    hipLaunchKernelGGL((terms_bwd_join_kernel<F16>), dim3(unsigned(ceil_div(n, 1024))), dim3(256), 0, st, a, plane, plane_q);
   }
   return launch_status("fm_local_attn_terms_bwd(join)");
 }

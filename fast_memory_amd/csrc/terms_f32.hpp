@@ -422,9 +422,9 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
       const T *q = (const T*)f.q + r * d, *o = (const T*)a.dout + r * d;
       T* to = (T*)a.dq + r * d;
       if (f.t.softcap > 0.f)
-        row_dq<T, true>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, f.sm_scale, Score<true>(f.sm_scale, f.t.softcap), to);
+        row_dq<T, true>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, 0, f.L, f.sm_scale, Score<true>(f.sm_scale, f.t.softcap), to);
       else
-        row_dq<T, false>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, f.sm_scale, Score<false>(f.sm_scale, 0.f), to);
+        row_dq<T, false>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, 0, f.L, f.sm_scale, Score<false>(f.sm_scale, 0.f), to);
     }
     return;
   }

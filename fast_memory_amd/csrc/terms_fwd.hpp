@@ -5,6 +5,9 @@
 // (under a causal mask it sees the most keys), so that what starts last is short and the launch ends evenly; the heads
 // go KV head first, so that the G query heads of a KV head run on one XCD (workgroups go to the 8 XCDs in turn) and
 // share its K and V in that XCD's L2.
+//
+// Where the blocks are too few for the card (sweep_pieces, terms_api.hip) the tiles that a block sees are cut into pieces, each of
+// which leaves (m, l, O) in fp32, and a second launch joins them in order.
 #pragma once
 #include <type_traits>
 
@@ -27,6 +30,9 @@ struct FwdTileArgs {
   int use_masks, H, G, S, L;
   float sm_scale;
   TileScore score;
+  int pieces;
+  float* part_o;     // [H G S][pieces][D], where pieces > 1
+  float2* part_ml;   // [H G S][pieces] {m, l}, m in base 2
 };
 
 template <bool F16, int D, int MODE, bool DOCS>
@@ -40,7 +46,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
   __syncthreads();
   const int heads = a.H * a.G, bx = int(blockIdx.x) % heads;
   const int hk = bx % a.H, hq = hk * a.G + bx / a.H;
-  const int qb = (a.S + kTQ - 1) / kTQ - 1 - int(blockIdx.x) / heads;
+  const int rest = int(blockIdx.x) / heads, piece = rest % a.pieces, qb = (a.S + kTQ - 1) / kTQ - 1 - rest / a.pieces;
   const int i0 = qb * kTQ, wq0 = i0 + 32 * w, iq = wq0 + col;
   const bool q_ok = iq < a.S;
   TileQuery qy;
@@ -90,9 +96,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
   const FlatSource<D, KT> src{a.k + int64_t(hk) * a.L * D, a.v + int64_t(hk) * a.L * D, a.L};
   typename M::f16v O[D / 32];
   TileState st;
-  const bool again = tile_sweep<F16, D, MODE, DOCS>(src, qf, qy, lim_lo, lim_hi, wg_lo, 0, (wg_hi + KT - 1) / KT, docs, a.score,
-                                              lds, flag, O, st);
+  int t0 = 0, t1 = (wg_hi + KT - 1) / KT;
+  const bool again = tile_sweep<F16, D, MODE, DOCS>(src, qf, qy, lim_lo, lim_hi, wg_lo, t0, t1, piece, a.pieces, docs, a.score, lds,
+                                                    flag, O, st);
   if (!again) {
+    if (a.pieces > 1) {
+      if (q_ok) tile_write_part<D>(O, st, a.part_o + (row * a.pieces + piece) * D, a.part_ml + row * a.pieces + piece);
+      return;
+    }
     tile_write<F16, D>(O, st, q_ok ? a.out + row * D : nullptr, a.lse + row);
     return;
   }
@@ -104,15 +115,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void terms_fwd_kernel(FwdTil
   for (int i = wq0; i < min(wq0 + 32, a.S); ++i) {
     const int64_t r = int64_t(hq) * a.S + i;
     const RowState rs = row_forward<E, (MODE & kModeCap) != 0>((const E*)a.q + r * D, K, V, query_view(a.t, i, a.S, a.L, hq),
-                                                               a.t.doc_k, 0, a.L, score);
+                                                               a.t.doc_k, t0 * KT, t1 * KT, score);
+    if (a.pieces > 1) {
+      const int64_t at = r * a.pieces + piece;
+#pragma unroll
+      for (int u = 0; u < D / 64; ++u) a.part_o[at * D + l + 64 * u] = rs.acc[u];
+      if (l == 0) a.part_ml[at] = make_float2(rs.m, rs.l);
+      continue;
+    }
     row_write(rs, D, (E*)a.out + r * D, a.lse + r);
   }
+}
+
+// the pieces of a query, in order: 16 lanes a query, D / 16 dimensions each
+template <bool F16, int D>
+__global__ __launch_bounds__(256) void terms_fwd_join_kernel(FwdTileArgs a) {
+  const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  if (row >= int64_t(a.H) * a.G * a.S) return;
+  tile_join<F16, D>(a.part_o + row * a.pieces * D, a.part_ml + row * a.pieces, a.pieces, a.out + row * D, a.lse + row);
 }
 
 template <bool F16, int D, int MODE, bool DOCS>
 static int launch_terms_fwd_docs(const FwdTileArgs& a, hipStream_t st) {
   FM_ALLOW_LDS((terms_fwd_kernel<F16, D, MODE, DOCS>), tile_lds_bytes<D>(), "fm_local_attn_terms_fwd(lds)");
-  hipLaunchKernelGGL((terms_fwd_kernel<F16, D, MODE, DOCS>), dim3(unsigned(a.H * a.G * ceil_div(a.S, kTQ))), dim3(256),
+  hipLaunchKernelGGL((terms_fwd_kernel<F16, D, MODE, DOCS>), dim3(unsigned(a.H * a.G * ceil_div(a.S, kTQ) * a.pieces)), dim3(256),
                      tile_lds_bytes<D>(), st, a);
   return launch_status("fm_local_attn_terms_fwd(tiles)");
 }
@@ -131,9 +157,17 @@ static int launch_terms_fwd_mode(const FwdTileArgs& a, hipStream_t st) {
   }
 }
 
+template <bool F16, int D>
+static int launch_terms_fwd_pieces(const FwdTileArgs& a, hipStream_t st) {
+  const int rc = launch_terms_fwd_mode<F16, D>(a, st);
+  if (rc || a.pieces == 1) return rc;
+  hipLaunchKernelGGL((terms_fwd_join_kernel<F16, D>), dim3(unsigned(ceil_div(int64_t(a.H) * a.G * a.S, 16))), dim3(256), 0, st, a);
+  return launch_status("fm_local_attn_terms_fwd(join)");
+}
+
 template <int D>
 int terms_fwd_tiles(const FwdTileArgs& a, bool f16, hipStream_t st) {
-  return f16 ? launch_terms_fwd_mode<true, D>(a, st) : launch_terms_fwd_mode<false, D>(a, st);
+  return f16 ? launch_terms_fwd_pieces<true, D>(a, st) : launch_terms_fwd_pieces<false, D>(a, st);
 }
 
 }  // namespace fm

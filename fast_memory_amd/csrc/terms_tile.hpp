@@ -285,13 +285,20 @@ __device__ __forceinline__ void issue_docs(const int32_t* dock, int t, uint32_t 
   if (w == 3) ring_load4(lds_addr, uint32_t(min(lane, KT - 1)) * 4u, ring_uniform_ptr(dock + int64_t(t) * KT));
 }
 
+// piece i of n of the tiles [t, t_end); the last ones may be empty
+__device__ __forceinline__ void tile_piece(int& t, int& t_end, int i, int n) {
+  const int each = (max(t_end - t, 0) + n - 1) / n;
+  t = min(t + i * each, t_end);
+  t_end = min(t + each, t_end);
+}
+
 struct TileState {
   float m, l;
 };
 
 template <bool F16, int D, int MODE, bool DOCS, class Source>
 __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16], const TileQuery& qy, int lim_lo, int lim_hi,
-                                           int wg_lo, int t_begin, int t_end, const TileDocs& docs, const TileScore& score,
+                                           int wg_lo, int& t_begin, int& t_end, int piece, int pieces, const TileDocs& docs, const TileScore& score,
                                            lds_char_t* lds, int* dirty_flag, typename Mma<F16>::f16v (&O)[D / 32], TileState& st) {
   constexpr int KT = fwd_tile_keys<D>(), NB = KT / 32;
   typedef TileLds<D, KT> T;
@@ -417,6 +424,11 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
 
   const uint32_t lds_docs = lds0 + 4u * T::kBytes;
   int t = next(t_begin);
+  if (pieces > 1) {
+    tile_piece(t, t_end, piece, pieces);
+    t_begin = t;
+    t = next(t);
+  }
   if (t < t_end) {
     src.prefetch(t);
     src.issue(t, lds0, lds0 + T::kBytes, w, l);
@@ -479,6 +491,52 @@ __device__ __forceinline__ void tile_write(const typename Mma<F16>::f16v (&O)[D 
       *reinterpret_cast<uint2*>(out + dt * 32 + 8 * rq + 4 * hb) = o;
     }
   if (hb == 0) *lse = none ? -FLT_MAX : (st.m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// A piece's state of a query, in fp32 and not yet divided.
+template <int D, class Acc>
+__device__ __forceinline__ void tile_write_part(const Acc (&O)[D / 32], const TileState& st, float* o, float2* ml) {
+  const int hb = (threadIdx.x >> 5) & 1;
+  const float l = st.l + __shfl_xor(st.l, 32);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq)
+      *reinterpret_cast<float4*>(o + dt * 32 + 8 * rq + 4 * hb) =
+          make_float4(O[dt][4 * rq], O[dt][4 * rq + 1], O[dt][4 * rq + 2], O[dt][4 * rq + 3]);
+  if (hb == 0) *ml = make_float2(st.m, l);
+}
+
+// The pieces of a query, in order: 16 lanes a query, D / 16 dimensions each.
+template <bool F16, int D>
+__device__ __forceinline__ void tile_join(const float* __restrict__ po, const float2* __restrict__ ml, int pieces, bf16_t* __restrict__ out,
+                                          float* __restrict__ lse) {
+  using M = Mma<F16>;
+  const int part = threadIdx.x & 15;
+  float mt = -INFINITY;
+  for (int i = 0; i < pieces; ++i) mt = fmaxf(mt, ml[i].x);
+  const float base = mt == -INFINITY ? 0.f : mt;
+  float lt = 0.f, o[D / 16];
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) o[k] = 0.f;
+  for (int i = 0; i < pieces; ++i) {
+    const float2 x = ml[i];
+    const float f = __builtin_amdgcn_exp2f(x.x - base);
+    lt = fmaf(x.y, f, lt);
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+      const float4 v = *reinterpret_cast<const float4*>(po + int64_t(i) * D + 64 * u + 4 * part);
+      o[4 * u] = fmaf(v.x, f, o[4 * u]), o[4 * u + 1] = fmaf(v.y, f, o[4 * u + 1]);
+      o[4 * u + 2] = fmaf(v.z, f, o[4 * u + 2]), o[4 * u + 3] = fmaf(v.w, f, o[4 * u + 3]);
+    }
+  }
+  const bool none = lt == 0.f;
+  const float inv = none ? 0.f : 1.f / lt;
+#pragma unroll
+  for (int u = 0; u < D / 64; ++u)
+    *reinterpret_cast<uint2*>(out + 64 * u + 4 * part) =
+        make_uint2(M::pack2(o[4 * u] * inv, o[4 * u + 1] * inv), M::pack2(o[4 * u + 2] * inv, o[4 * u + 3] * inv));
+  if (part == 0) *lse = none ? -FLT_MAX : (mt + __builtin_amdgcn_logf(lt)) * kLn2;
 }
 
 }  // namespace fm

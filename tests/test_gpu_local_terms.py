@@ -97,6 +97,41 @@ def test_longer_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d,cap,slopes,docs,prefix,causal", [
+    (64, 0.0, False, 0, 0, True), (128, 20.0, True, 3, 60, True), (256, 0.0, False, 5, 0, False), (64, 25.0, True, 0, 1900, True)])
+def test_few_rows_over_many_keys(dtype, d, cap, slopes, docs, prefix, causal):
+    # too few blocks of queries for the card: their keys are cut into pieces and joined
+    H, G, S, L = 1, 2, 201, 2100
+    check(43, H, G, S, L, d, dtype, causal, terms_of(12, H, G, S, L, cap, slopes, docs, prefix, pad=11 if docs else 0))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_pieces_with_masked_places_that_are_not_finite(dtype, d, bad):
+    H, G, S, L = 1, 1, 70, 1300
+    q, k, v, do, dl = inputs(44, H, G, S, L, d, dtype)
+    doc_k = torch.zeros(L, dtype=torch.int32)
+    doc_k[40:50], doc_k[600:640], doc_k[1299:] = 1, 1, -1
+    t = dict(doc_q=torch.zeros(S, dtype=torch.int32), doc_k=doc_k, softcap=10.0)
+    t["doc_q"][5] = -1
+    scale = d ** -0.5
+    want, tol = O.local(q, k, v, scale, False, dout=do, dlse=dl, **t)
+    for x in (k, v):
+        x[:, 40:50] = bad
+        x[:, 600:640] = bad
+        x[:, 1299:] = bad
+    q[:, 5], do[:, 5], dl[:, 5] = bad, bad, bad
+    gq, gk, gv, gdo, gdl = (x.cuda() for x in (q, k, v, do, dl))
+    out, lse = ops.local_attn_terms_fwd(gq, gk, gv, scale, False, on_gpu(t))
+    dq, dk, dv = ops.local_attn_terms_bwd(gdo, gq, gk, gv, out, lse, scale, False, on_gpu(t), gdl)
+    seen = doc_k == 0
+    for n, x, rows in (("out", out, slice(None)), ("lse", lse, slice(None)), ("dq", dq, slice(None)), ("dk", dk, seen), ("dv", dv, seen)):
+        close(x[:, rows], want[n][:, rows], tol[n][:, rows], n)
+    assert (dk[:, ~seen] == 0).all() and (dv[:, ~seen] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_rows_that_see_nothing_and_padding(dtype, d):
     # more queries than keys (the first see nothing), padding behind the last document, a document without keys

@@ -39,7 +39,9 @@ static bool tiles_take(int d, int dtype) {
 }
 
 // Into how many pieces the keys of a block of 128 queries are cut: until there are 512 workgroups, two a compute unit, none of
-// less than 8 tiles of 64 keys.  (Blocks that fill half the card stay whole: the partial sums cost more than they gain.)
+// less than 8 tiles of 64 keys.  Measured, whole and in pieces, bf16: 2 heads x 4096, d = 256: forward 220 and 64 us, backward
+// 606 and 280; 8 heads x 128 over 4096 keys, d = 128: 122 and 28, 193 and 48; 16 x 2048: 66 and 52, 150 and 131; 32 x 1024
+// (256 blocks): 37 and 37, 93 and 88.
 static int sweep_pieces(int H, int G, int S, int L, int d, int dtype) {
   if (!tiles_take(d, dtype)) return 1;
   const int64_t blocks = int64_t(H) * G * ceil_div(S, kTQ);

@@ -24,8 +24,6 @@
 
 namespace fm {
 
-typedef int lds_int2 __attribute__((ext_vector_type(2)));
-
 constexpr float kPScaleF16 = 4096.f;
 constexpr int kNormRows = 64;   // rows whose norms a workgroup of the first launch takes the largest of
 
@@ -153,7 +151,7 @@ __device__ __forceinline__ void block_probs(float (&x)[16], float (&y)[16], cons
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float u = x[r] * k.in, z = u * capped_small(k, u);
+        const float z = x[r] * capped_small(k, x[r]);
         finish(r, z, fmaf(z * k.k2, -z, 1.f));
       }
     }
@@ -169,11 +167,13 @@ struct ColumnQuery {
   float l;
   __device__ __forceinline__ float lse2(int) const { return l; }
 };
-struct RowQueries {  // this lane's rows are queries 4 hb + 8 (r / 4) + r % 4 of the tile, 8 bytes each from `at`
+struct RowQueries {  // this lane's rows are queries 4 hb + 8 (r / 4) + r % 4 of the tile: 32 x lse log2 e, 32 x D from 4 hb on
   const lds_char_t* at;
-  __device__ __forceinline__ uint4 pair(int r) const { return lds_read16(at + (8 * (r >> 2) + (r & 2)) * 8); }
-  __device__ __forceinline__ float lse2(int r) const { return __uint_as_float(r & 1 ? pair(r).z : pair(r).x); }
-  __device__ __forceinline__ float delta(int r) const { return __uint_as_float(r & 1 ? pair(r).w : pair(r).y); }
+  __device__ __forceinline__ float pick(const uint4& u, int r) const {
+    return __uint_as_float((r & 3) == 0 ? u.x : (r & 3) == 1 ? u.y : (r & 3) == 2 ? u.z : u.w);
+  }
+  __device__ __forceinline__ float lse2(int r) const { return pick(lds_read16(at + 32 * (r >> 2)), r); }
+  __device__ __forceinline__ float delta(int r) const { return pick(lds_read16(at + 128 + 32 * (r >> 2)), r); }
 };
 
 // keys of a tile of the dq launch
@@ -465,7 +465,7 @@ __device__ __forceinline__ void dkv_block(const BwdTileArgs& a, int block, bf16_
   int* flag = reinterpret_cast<int*>(lds_all);
   lds_char_t* lds_v = (lds_char_t*)(lds_all + 256);
   lds_char_t* lds = lds_v + TV::kBytes;
-  lds_char_t* lds_row = lds + 4 * T::kBytes;  // [2]{ {lse log2 e, D}[32], {limit, document}[32] }
+  lds_char_t* lds_row = lds + 4 * T::kBytes;  // [2]{ lse log2 e [32], D [32], limit [32], document [32] }
   const uint32_t lds_v0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds_v)));
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds)));
   const uint32_t lds_row0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds_row)));
@@ -565,8 +565,9 @@ __device__ __forceinline__ void dkv_block(const BwdTileArgs& a, int block, bf16_
       tile_load(to + uint32_t(w + 4 * u) * 1024u, voff, bq);
       tile_load(to + T::kBytes + uint32_t(w + 4 * u) * 1024u, voff, bd);
     }
-    // 8 bytes a query: wave 0 {lse log2 e, D}, wave 1 {limit, document} where there are masks
-    const uint32_t voff = uint32_t(min(l >> 1, last)) * 8u + uint32_t(l & 1) * 4u;
+    // 8 bytes a query: wave 0 {lse log2 e, D}, wave 1 {limit, document} where there are masks; the halves of a wave take one each,
+    // so that four queries' are 16 consecutive bytes in LDS
+    const uint32_t voff = uint32_t(min(l & 31, last)) * 8u + uint32_t(l >> 5) * 4u;
     if (w == 0) ring_load4(lds_row0 + uint32_t(buf) * 512u, voff, ring_uniform_ptr(a.rd + row));
     if (w == 1 && a.use_masks) ring_load4(lds_row0 + uint32_t(buf) * 512u + 256u, voff, ring_uniform_ptr(a.m.qinfo + i0));
   };
@@ -612,22 +613,26 @@ __device__ __forceinline__ void dkv_block(const BwdTileArgs& a, int block, bf16_
     float x[16], y[16];  // p; p slack
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = sc[r];
-    const RowQueries rq{rows + 4 * hb * 8};
+    const RowQueries rq{rows + 4 * hb * 4};
     block_probs<MODE>(x, y, a.score, float(j - (i0 + 4 * hb + (a.L - a.S))), slope2, rq);
     const bool masked = mixed || ragged || wj0 + 32 > lo;
     if (masked) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int iq = 4 * hb + 8 * (r >> 2) + (r & 3), i = i0 + iq;
-        bool ok = i < a.S;
+      for (int q = 0; q < 4; ++q) {
+        const int iq = 4 * hb + 8 * q;
+        uint4 lim = make_uint4(0, 0, 0, 0), docs = lim;
         if (a.use_masks) {
-          const lds_int2 qi = *reinterpret_cast<const __attribute__((address_space(3))) lds_int2*>(rows + 256 + iq * 8);
-          ok = ok && j < qi.x;
-          if constexpr (DOCS) ok = ok && qi.y == doc;
-        } else {
-          ok = ok && j < seen_limit(i + (a.L - a.S), a.L, a.t.causal, 0);
+          lim = lds_read16(rows + 256 + iq * 4);
+          if constexpr (DOCS) docs = lds_read16(rows + 384 + iq * 4);
         }
-        if (!ok) x[r] = 0.f, y[r] = 0.f;
+        const int ll[4] = {int(lim.x), int(lim.y), int(lim.z), int(lim.w)}, dd[4] = {int(docs.x), int(docs.y), int(docs.z), int(docs.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = i0 + iq + e;
+          bool ok = i < a.S && j < (a.use_masks ? ll[e] : seen_limit(i + (a.L - a.S), a.L, a.t.causal, 0));
+          if constexpr (DOCS) ok = ok && dd[e] == doc;
+          if (!ok) x[4 * q + e] = 0.f, y[4 * q + e] = 0.f;
+        }
       }
     }
     if constexpr (PART != kDkOnly) {

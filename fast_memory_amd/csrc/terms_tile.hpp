@@ -130,11 +130,13 @@ struct TileLds {
   }
 };
 
-// Score arithmetic of a launch (base 2, see Score in terms.hpp): with y = raw in and w = y^2 the small-argument cap is
-// y (c0 + w (c1 + w (..))), the polynomial's coefficients times `out`; it serves |raw| <= zmax (|y| <= 1/2).
+// Score arithmetic of a launch (base 2, see Score in terms.hpp).  With w = raw^2 the small-argument cap is
+// raw (c0 + w (c1 + w (..))): terms.hpp's polynomial in y = raw in, its coefficients times out in^(2 i + 1), which spares the
+// product raw in (of about 12 instructions a score).  It serves |raw| <= zmax (|y| <= 1/2); zmax is -1, and every score goes the
+// general way, where the last coefficient would leave fp32's normal range (sm_scale / softcap below 1e-3 or above 1e3 or so).
 // 1 - tanh^2 = 1 - k2 x^2 from the capped score x.
 struct TileScore {
-  float in, out, c1, c2, c3, c4, c5, zmax, k2;
+  float in, out, c0, c1, c2, c3, c4, c5, zmax, k2;
 };
 
 inline TileScore tile_score(float sm_scale, float softcap) {
@@ -147,22 +149,26 @@ inline TileScore tile_score(float sm_scale, float softcap) {
   t.in = sm_scale / softcap;
   t.out = softcap * kLog2e;
   t.k2 = 1.f / t.out / t.out;
-  t.c1 = -0.333333328f * t.out;
-  t.c2 = 0.133332274f * t.out;
-  t.c3 = -0.0539337893f * t.out;
-  t.c4 = 0.021472721f * t.out;
-  t.c5 = -0.00694700312f * t.out;
-  t.zmax = kTanhSmall / t.in;
+  const double in = double(t.in), w = in * in, c0 = double(t.out) * in;
+  const double c5 = -0.00694700312 * c0 * w * w * w * w * w;
+  t.c0 = float(c0);
+  t.c1 = float(-0.333333328 * c0 * w);
+  t.c2 = float(0.133332274 * c0 * w * w);
+  t.c3 = float(-0.0539337893 * c0 * w * w * w);
+  t.c4 = float(0.021472721 * c0 * w * w * w * w);
+  t.c5 = float(c5);
+  const bool fits = -c5 >= 1e-36 && -c5 <= 1e36 && c0 >= 1e-36 && c0 <= 1e36;
+  t.zmax = fits ? kTanhSmall / t.in : -1.f;
   return t;
 }
 
-__device__ __forceinline__ float capped_small(const TileScore& k, float y) {
-  const float w = y * y;
+__device__ __forceinline__ float capped_small(const TileScore& k, float x) {
+  const float w = x * x;
   float p = fmaf(w, k.c5, k.c4);
   p = fmaf(w, p, k.c3);
   p = fmaf(w, p, k.c2);
   p = fmaf(w, p, k.c1);
-  return fmaf(w, p, k.out);  // times y
+  return fmaf(w, p, k.c0);  // times x
 }
 
 typedef float tile_f16v __attribute__((__vector_size__(16 * sizeof(float))));
@@ -207,8 +213,8 @@ __device__ __forceinline__ void block_scores(float (&x)[16], const TileScore& k,
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float y = x[r] * k.in, p = capped_small(k, y);
-        x[r] = (MODE & kModeBias) ? fmaf(y, p, -slope2 * dist(r)) : y * p;
+        const float p = capped_small(k, x[r]);
+        x[r] = (MODE & kModeBias) ? fmaf(x[r], p, -slope2 * dist(r)) : x[r] * p;
       }
     }
   } else if constexpr (MODE & kModeBias) {

@@ -132,6 +132,13 @@ def test_pieces_with_masked_places_that_are_not_finite(dtype, d, bad):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("cap", [1e-3, 0.05, 1.0, 300.0, 1e5, 1e20])
+def test_caps_of_every_size(dtype, cap):
+    # small caps bind every score, large ones none; both ends leave the range of the small-argument polynomial's coefficients
+    check(46, 1, 2, 80, 100, 64, dtype, True, dict(softcap=cap))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_rows_that_see_nothing_and_padding(dtype, d):
     # more queries than keys (the first see nothing), padding behind the last document, a document without keys

@@ -265,7 +265,8 @@ class _LocalAttentionFunc(torch.autograd.Function):
 def local_attention(q, k, v, sm_scale: float, causal: bool = True, terms: Optional[ops.ScoreTerms] = None):
     """The local attention (call site memory.py:302-304) with :class:`ops.ScoreTerms`, differentiable in ``q``, ``k`` and
     ``v`` through ``out`` and ``lse``: ``q [H*G,S,d]``, ``k, v [H,L,d]`` -> ``(out [H*G,S,d], lse [H*G,S] fp32)``.  The
-    gradients do not depend on scheduling."""
+    gradients do not depend on scheduling.  A step that is recorded into a graph calls ``ops.local_attn_terms_fwd`` and
+    :func:`local_attention_backward`, which build no autograd graph of their own."""
     t = ops.ScoreTerms() if terms is None else terms
     if t.slopes is not None and t.slopes.requires_grad:
         raise ValueError("slopes receive no gradient: pass them detached")

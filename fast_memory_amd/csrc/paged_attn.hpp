@@ -29,14 +29,20 @@ struct PagedTileArgs {
   TileScore score;
   int few_rows;              // rows with at most that many query rows are the few-kernel's, the others the other's
   int few_pieces, many_pieces;
-  float* part_o;             // [T][H G][pieces][D], pieces = max of the two
-  float2* part_ml;           // [T][H G][pieces] {m, l}, m in base 2
-  int pieces;
+  float* part_o;             // [units][D]
+  float2* part_ml;           // [units] {m, l}, m in base 2
+  int64_t many_base;         // the first unit of the many-kernel's
   int many_slots;
 };
 
-__device__ __forceinline__ int64_t part_index(const PagedTileArgs& a, int t, int hq, int piece) {
-  return (int64_t(t) * a.p.H * a.p.G + hq) * a.pieces + piece;
+// Where a query row's pieces lie.  Beside a many-kernel the few-kernel's rows are counted within their row of the batch, of which
+// each has kFewRows at most: by token there would be units for all the others' too, gigabytes where a long prompt comes along.
+__device__ __forceinline__ int64_t few_index(const PagedTileArgs& a, int row, int r, int hk, int t, int hq) {
+  const int64_t u = a.few_rows == kFewRows ? (int64_t(row) * kFewRows + r) * a.p.H + hk : int64_t(t) * a.p.H * a.p.G + hq;
+  return u * a.few_pieces;
+}
+__device__ __forceinline__ int64_t many_index(const PagedTileArgs& a, int t, int hq) {
+  return a.many_base + (int64_t(t) * a.p.H * a.p.G + hq) * a.many_pieces;
 }
 
 // Where a page number leads: clamped into the pool.
@@ -44,26 +50,30 @@ __device__ __forceinline__ int64_t page_offset(const PagedArgs& p, int page, int
   return int64_t(min(max(page, 0), p.n_pages - 1)) * p.H * p.page * d;
 }
 
-// tokens behind the last row's, and those of rows with a broken cu: nothing to see
+// tokens in front of the first row's and behind the last row's: nothing to see
 template <typename E>
 __device__ void paged_nobody(const PagedTileArgs& a, int first, int step) {
-  const int HG = a.p.H * a.p.G;
-  for (int t = max(a.p.cu[a.p.R], 0) + first; t < a.p.T; t += step)
+  const int HG = a.p.H * a.p.G, c0 = a.p.cu[0], c1 = max(a.p.cu[a.p.R], 0);
+  for (int t = first; t < a.p.T; t += step) {
+    if (t >= c0 && t < c1) {
+      t += (c1 - 1 - t) / step * step;
+      continue;
+    }
     for (int u = threadIdx.x; u < HG * a.p.d; u += 256) {
       const int hq = u / a.p.d, c = u - hq * a.p.d;
       Elem<E>::store((E*)a.p.out + t * a.p.o_token + hq * a.p.o_head + c, 0.f);
       if (c == 0) a.p.lse[t * a.p.l_token + hq * a.p.l_head] = -FLT_MAX;
     }
+  }
 }
 
 // One query row's result: final where the keys are in one piece, else its piece's.  `o`: 64 lanes, dimensions l + 64 r.
 template <typename E>
-__device__ __forceinline__ void paged_row_result(const PagedTileArgs& a, const RowState& st, int t, int hq, int piece, int pieces) {
+__device__ __forceinline__ void paged_row_result(const PagedTileArgs& a, const RowState& st, int t, int hq, int64_t at, int pieces) {
   if (pieces == 1) {
     row_write(st, a.p.d, (E*)a.p.out + t * a.p.o_token + hq * a.p.o_head, a.p.lse + t * a.p.l_token + hq * a.p.l_head);
     return;
   }
-  const int64_t at = part_index(a, t, hq, piece);
   const int lane = lane_id();
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -72,7 +82,7 @@ __device__ __forceinline__ void paged_row_result(const PagedTileArgs& a, const R
 }
 
 template <typename E>
-__device__ __forceinline__ void paged_row_again(const PagedTileArgs& a, const PagedRow& pr, int t, int hq, int j0, int j1, int piece,
+__device__ __forceinline__ void paged_row_again(const PagedTileArgs& a, const PagedRow& pr, int t, int hq, int j0, int j1, int64_t at,
                                                 int pieces) {
   QueryView qv;
   qv.pos = pr.len - (pr.q1 - t);
@@ -87,7 +97,7 @@ __device__ __forceinline__ void paged_row_again(const PagedTileArgs& a, const Pa
   const RowState st = a.p.softcap > 0.f
                           ? row_forward<E, true>(q, K, V, qv, nullptr, j0, j1, Score<true>(a.p.sm_scale, a.p.softcap))
                           : row_forward<E, false>(q, K, V, qv, nullptr, j0, j1, Score<false>(a.p.sm_scale, 0.f));
-  paged_row_result<E>(a, st, t, hq, piece, pieces);
+  paged_row_result<E>(a, st, t, hq, at, pieces);
 }
 
 // the keys of piece i of n, in whole tiles of `tile`; a piece behind the last tile has j0 >= j1 and no tile j0 / tile .. either
@@ -303,7 +313,8 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
     const bool again = *flag != 0;
     if (again) {
       for (int r = r0 + w; r < min(r0 + 16 * NQ, n_rows); r += 4)
-        paged_row_again<E>(a, pr, pr.q0 + r / a.p.G, hk * a.p.G + r % a.p.G, j0, j1, piece, a.few_pieces);
+        paged_row_again<E>(a, pr, pr.q0 + r / a.p.G, hk * a.p.G + r % a.p.G, j0, j1,
+                           few_index(a, row, r, hk, pr.q0 + r / a.p.G, hk * a.p.G + r % a.p.G) + piece, a.few_pieces);
       __syncthreads();
       continue;
     }
@@ -341,7 +352,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
         const int tok = r / a.p.G, hq = hk * a.p.G + (r - tok * a.p.G), t = pr.q0 + tok;
         const bool none = lt == 0.f;
         const float inv = a.few_pieces > 1 ? 1.f : none ? 0.f : 1.f / lt;
-        const int64_t at = a.few_pieces > 1 ? part_index(a, t, hq, piece) : 0;
+        const int64_t at = a.few_pieces > 1 ? few_index(a, row, r, hk, t, hq) + piece : 0;
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) {
           const int d0 = 64 * u + 4 * part;
@@ -457,7 +468,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_many_kernel(Paged
   const bool again = tile_sweep<F16, D, MODE, false>(src, qf, qy, lim_lo, lim_hi, wg_lo, t0, t1, 0, 1, docs, a.score, lds, flag, O, st);
   if (again) {
     for (int rr = wr0; rr < min(wr0 + 32, n_rows); ++rr)
-      paged_row_again<E>(a, pr, pr.q0 + rr / a.p.G, hk * a.p.G + rr % a.p.G, j0, j1, piece, a.many_pieces);
+      paged_row_again<E>(a, pr, pr.q0 + rr / a.p.G, hk * a.p.G + rr % a.p.G, j0, j1,
+                         many_index(a, pr.q0 + rr / a.p.G, hk * a.p.G + rr % a.p.G) + piece, a.many_pieces);
     return;
   }
   if (a.many_pieces == 1) {
@@ -466,7 +478,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_many_kernel(Paged
     return;
   }
   if (!ok) return;
-  const int64_t at = part_index(a, t, hq, piece);
+  const int64_t at = many_index(a, t, hq) + piece;
   tile_write_part<D>(O, st, a.part_o + at * D, a.part_ml + at);
 }
 
@@ -480,16 +492,20 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedTileArgs a) {
   if (t >= a.p.T) return;
   const PagedRow pr = paged_row_of_token(a.p, t);
   if (pr.row < 0) return;  // (written where nobody's tokens are)
-  const int pieces = (pr.q1 - pr.q0) * a.p.G <= a.few_rows ? a.few_pieces : a.many_pieces;
+  const bool few = (pr.q1 - pr.q0) * a.p.G <= a.few_rows;
+  const int pieces = few ? a.few_pieces : a.many_pieces;
   if (pieces == 1) return;
-  tile_join<F16, D>(a.part_o + part_index(a, t, hq, 0) * D, a.part_ml + part_index(a, t, hq, 0), pieces,
+  const int hk = hq / a.p.G;
+  const int64_t at = few ? few_index(a, pr.row, (t - pr.q0) * a.p.G + hq - hk * a.p.G, hk, t, hq) : many_index(a, t, hq);
+  tile_join<F16, D>(a.part_o + at * D, a.part_ml + at, pieces,
                     (bf16_t*)a.p.out + t * a.p.o_token + hq * a.p.o_head, a.p.lse + t * a.p.l_token + hq * a.p.l_head);
 }
 
 // ---- host: which launches, how many pieces -----------------------------------------------------------------------------
 struct PagedPlan {
   bool few, many;
-  int few_rows, few_pieces, many_pieces, pieces, slots;
+  int few_rows, few_pieces, many_pieces, slots;
+  int64_t many_base;  // units of the few-kernel's pieces
   size_t part_ml, total;
 };
 
@@ -504,10 +520,11 @@ inline PagedPlan paged_plan(int rows, int T, int max_new, int H, int G, int d, i
   y.slots = int(int64_t(T) * G / kTQ) + rows;
   const int64_t most = std::min<int64_t>(ceil_div(keys, 512), 64);
   auto pieces = [&](int64_t groups) { return int(std::max<int64_t>(1, std::min(most, ceil_div(1024, groups)))); };
-  y.few_pieces = y.few ? pieces(int64_t(rows) * H) : 1;
+  // (where every row is the few-kernel's, by T as well: a max_new that is too small is no wrong answer, nor a large workspace)
+  y.few_pieces = y.few ? pieces(std::max<int64_t>(rows, y.many ? 0 : int64_t(T) * G / kFewRows) * H) : 1;
   y.many_pieces = y.many ? pieces(std::max<int64_t>(1, int64_t(T) * G / kTQ) * H) : 1;
-  y.pieces = std::max(y.few_pieces, y.many_pieces);
-  const size_t units = y.pieces > 1 ? size_t(T) * H * G * y.pieces : 0;
+  y.many_base = y.few_pieces > 1 ? int64_t(y.many ? int64_t(rows) * kFewRows : int64_t(T) * G) * H * y.few_pieces : 0;
+  const size_t units = size_t(y.many_base) + (y.many_pieces > 1 ? size_t(T) * H * G * y.many_pieces : 0);
   y.part_ml = align_up(units * d * 4, 256);
   y.total = y.part_ml + align_up(units * 8, 256);
   return y;
@@ -521,8 +538,8 @@ inline PagedPlan paged_f32_plan(int rows, int T, int H, int G, int d, int64_t ke
   y.slots = int(int64_t(T) * G / 32) + rows;
   const int64_t groups = std::max<int64_t>(std::min<int64_t>(rows, T), int64_t(T) * G / 32) * H;
   y.few_pieces = 1;
-  y.pieces = y.many_pieces = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(keys, 512), 64), ceil_div(1024, groups))));
-  const size_t units = y.pieces > 1 ? size_t(T) * H * G * y.pieces : 0;
+  y.many_pieces = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(keys, 512), 64), ceil_div(1024, groups))));
+  const size_t units = y.many_pieces > 1 ? size_t(T) * H * G * y.many_pieces : 0;
   y.part_ml = align_up(units * d * 4, 256);
   y.total = y.part_ml + align_up(units * 8, 256);
   return y;
@@ -563,7 +580,7 @@ static int launch_paged(const PagedTileArgs& a, const PagedPlan& y, int max_new,
     }
     if (rc) return rc;
   }
-  if (a.pieces > 1) {
+  if (a.few_pieces > 1 || a.many_pieces > 1) {
     const int64_t units = int64_t(a.p.T) * a.p.H * a.p.G;
     hipLaunchKernelGGL((paged_join_kernel<F16, D>), dim3(unsigned(ceil_div(units, 16))), dim3(256), 0, st, a);
   }

@@ -61,7 +61,8 @@ __global__ __launch_bounds__(256, 1) void paged_f32_kernel(PagedTileArgs a, F32S
   __syncthreads();
   if (*flag) {
     for (int rr = r0 + w; rr < min(r0 + kF32Rows, n_rows); rr += 4)
-      paged_row_again<T>(a, pr, pr.q0 + rr / p.G, hk * p.G + rr % p.G, j0, j1, piece, a.many_pieces);
+      paged_row_again<T>(a, pr, pr.q0 + rr / p.G, hk * p.G + rr % p.G, j0, j1,
+                         many_index(a, pr.q0 + rr / p.G, hk * p.G + rr % p.G) + piece, a.many_pieces);
     return;
   }
   for (int i = w; i < kF32Rows && r0 + i < n_rows; i += 4) {
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(256, 1) void paged_f32_kernel(PagedTileArgs a, F32S
     for (int k = 0; k < 4; ++k) g[k] = f32_weight(ml, i, k, st.x);
     const int rt = (r0 + i) / p.G, rq = hk * p.G + (r0 + i - rt * p.G), tt = pr.q0 + rt;
     if (a.many_pieces > 1) {
-      const int64_t at = part_index(a, tt, rq, piece);
+      const int64_t at = many_index(a, tt, rq) + piece;
       for (int c = l; c < d; c += 64) a.part_o[at * d + c] = f32_get<NDT>(lds, i, c, g);
       if (l == 0) a.part_ml[at] = st;
     } else {
@@ -92,8 +93,8 @@ __global__ __launch_bounds__(256) void paged_f32_join_kernel(PagedTileArgs a) {
   if (t >= a.p.T) return;
   const PagedRow pr = paged_row_of_token(a.p, t);
   if (pr.row < 0) return;  // (written where nobody's tokens are)
-  const float2* ml = a.part_ml + part_index(a, t, hq, 0);
-  const float* po = a.part_o + part_index(a, t, hq, 0) * a.p.d;
+  const float2* ml = a.part_ml + many_index(a, t, hq);
+  const float* po = a.part_o + many_index(a, t, hq) * a.p.d;
   RowState st;
   st.m = -INFINITY;
   st.l = 0.f;
@@ -126,7 +127,7 @@ int paged_f32(const PagedTileArgs& a, const PagedPlan& y, hipStream_t st) {
 #define FM_F(V, N) launch_paged_f32<T, V, N>(a, st)
   const int rc = FM_F32_BY_DIM(a.p.d, vec, FM_F);
 #undef FM_F
-  if (rc || y.pieces == 1) return rc;
+  if (rc || y.many_pieces == 1) return rc;
   const int64_t units = int64_t(a.p.T) * a.p.H * a.p.G;
   hipLaunchKernelGGL(paged_f32_join_kernel<T>, dim3(unsigned(ceil_div(units, 4))), dim3(256), 0, st, a);
   return launch_status("fm_paged_attn_fwd(join)");

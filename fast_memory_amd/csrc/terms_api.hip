@@ -260,7 +260,7 @@ extern "C" int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head,
   FM_REQUIRE(groups <= 0x7fffffffLL, FM_ERR_UNSUPPORTED, "fm_paged_attn_fwd: %lld workgroups", (long long)groups);
   char* w = static_cast<char*>(ws);
   const PagedTileArgs t{a, tile_score(sm_scale, softcap), y.few_rows, y.few_pieces, y.many_pieces, reinterpret_cast<float*>(w),
-                        reinterpret_cast<float2*>(w + y.part_ml), y.pieces, y.slots};
+                        reinterpret_cast<float2*>(w + y.part_ml), y.many_base, y.slots};
   hipStream_t st = as_stream(stream);
   if (!tiles) return dtype == FM_F32 ? paged_f32<float>(t, y, st) : dtype == FM_BF16 ? paged_f32<bf16_t>(t, y, st) : paged_f32<f16_t>(t, y, st);
   return d == 64 ? paged_tiles<64>(t, y, max_new, st) : d == 128 ? paged_tiles<128>(t, y, max_new, st) : paged_tiles<256>(t, y, max_new, st);

@@ -605,6 +605,8 @@ class ScoreTerms(NamedTuple):
       document is padding: it sees nothing and nobody sees it);
     * ``prefix [S]`` int: query i sees the keys ``j < prefix[i]`` whatever the causal mask says (of its own document,
       where there are any).  Over a paged cache it is ``[n_rows]``, and a row is a document of its own.
+
+    int64 tensors are cast: their values have to fit 32 bits.
     """
     softcap: float = 0.0
     slopes: Optional[torch.Tensor] = None

@@ -339,6 +339,13 @@ def test_tokens_of_no_row():
     assert o.shape == (0, 2, 64) and l.shape == (0, 2)
 
 
+def test_tokens_in_front_of_the_first_row():
+    cache, q, cu, terms, out, lse = attend_case(34, [40, 50], [3, 4], 1, 2, 64, 16, torch.bfloat16, {})
+    o, l = cache.attend(torch.cat([q[:2], q]), cu + 2, 64 ** -0.5, terms)
+    assert torch.equal(o[2:], out) and torch.equal(l[2:], lse)
+    assert (o[:2] == 0).all() and (l[:2] == O.EMPTY).all()
+
+
 def test_a_decoding_run_over_a_forked_cache_and_a_memory():
     """Prompt, fork, decode, drop what the memory takes over, compact: every step against the plain form, merged with the
     memory's attention; the batch of memories takes the same path."""

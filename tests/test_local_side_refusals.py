@@ -108,3 +108,10 @@ def test_python_refusals_on_the_gpu():
         with pytest.raises(ValueError):
             bad()
     c.check()
+
+
+def test_a_long_prompt_beside_single_tokens_needs_no_large_workspace():
+    lib = _lib.load()
+    for dt in (_lib.FM_BF16, _lib.FM_F32):
+        for rows, T, max_new in ((2, 8192, 0), (64, 8192, 0), (1, 8192, 1), (1, 8192, 8192), (2048, 2048, 1)):
+            assert 0 < lib.fm_paged_attn_fwd_workspace(rows, T, max_new, 8, 8, 128, 4096, 16, dt) <= 100 << 20, (rows, T, max_new)

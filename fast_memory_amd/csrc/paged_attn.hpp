@@ -483,22 +483,35 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_many_kernel(Paged
 }
 
 // ---- the pieces of a query row, in order: 16 lanes a row, D / 16 dimensions each -----------------------------------------
-template <bool F16, int D>
+// FEW: only the few-kernel's rows were cut, beside rows of many queries that are done; the launch counts as few_index does.
+template <bool F16, int D, bool FEW>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedTileArgs a) {
-  using M = Mma<F16>;
-  const int HG = a.p.H * a.p.G;
   const int64_t unit = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const int t = int(unit / HG), hq = int(unit - int64_t(t) * HG);
-  if (t >= a.p.T) return;
-  const PagedRow pr = paged_row_of_token(a.p, t);
-  if (pr.row < 0) return;  // (written where nobody's tokens are)
-  const bool few = (pr.q1 - pr.q0) * a.p.G <= a.few_rows;
-  const int pieces = few ? a.few_pieces : a.many_pieces;
+  PagedRow pr;
+  int t, hk, r;
+  if constexpr (FEW) {
+    const int64_t u = unit / a.p.H;
+    hk = int(unit - u * a.p.H), r = int(u % kFewRows);
+    if (u / kFewRows >= a.p.R) return;
+    pr = paged_row(a.p, int(u / kFewRows));
+    const int n_rows = (pr.q1 - pr.q0) * a.p.G;
+    if (n_rows > a.few_rows || r >= n_rows) return;
+    t = pr.q0 + r / a.p.G;
+  } else {
+    const int HG = a.p.H * a.p.G;
+    t = int(unit / HG);
+    if (t >= a.p.T) return;
+    const int hq = int(unit - int64_t(t) * HG);
+    pr = paged_row_of_token(a.p, t);
+    if (pr.row < 0) return;  // (written where nobody's tokens are)
+    hk = hq / a.p.G, r = (t - pr.q0) * a.p.G + hq - hk * a.p.G;
+  }
+  const bool few = FEW || (pr.q1 - pr.q0) * a.p.G <= a.few_rows;
+  const int pieces = few ? a.few_pieces : a.many_pieces, hq = hk * a.p.G + r % a.p.G;
   if (pieces == 1) return;
-  const int hk = hq / a.p.G;
-  const int64_t at = few ? few_index(a, pr.row, (t - pr.q0) * a.p.G + hq - hk * a.p.G, hk, t, hq) : many_index(a, t, hq);
-  tile_join<F16, D>(a.part_o + at * D, a.part_ml + at, pieces,
-                    (bf16_t*)a.p.out + t * a.p.o_token + hq * a.p.o_head, a.p.lse + t * a.p.l_token + hq * a.p.l_head);
+  const int64_t at = few ? few_index(a, pr.row, r, hk, t, hq) : many_index(a, t, hq);
+  tile_join<F16, D>(a.part_o + at * D, a.part_ml + at, pieces, (bf16_t*)a.p.out + t * a.p.o_token + hq * a.p.o_head,
+                    a.p.lse + t * a.p.l_token + hq * a.p.l_head);
 }
 
 // ---- host: which launches, how many pieces -----------------------------------------------------------------------------
@@ -580,9 +593,12 @@ static int launch_paged(const PagedTileArgs& a, const PagedPlan& y, int max_new,
     }
     if (rc) return rc;
   }
-  if (a.few_pieces > 1 || a.many_pieces > 1) {
+  if (a.many_pieces > 1 || (a.few_pieces > 1 && a.few_rows != kFewRows)) {
     const int64_t units = int64_t(a.p.T) * a.p.H * a.p.G;
-    hipLaunchKernelGGL((paged_join_kernel<F16, D>), dim3(unsigned(ceil_div(units, 16))), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_join_kernel<F16, D, false>), dim3(unsigned(ceil_div(units, 16))), dim3(256), 0, st, a);
+  } else if (a.few_pieces > 1) {
+    const int64_t units = int64_t(a.p.R) * kFewRows * a.p.H;
+    hipLaunchKernelGGL((paged_join_kernel<F16, D, true>), dim3(unsigned(ceil_div(units, 16))), dim3(256), 0, st, a);
   }
   return launch_status("fm_paged_attn_fwd(join)");
 }

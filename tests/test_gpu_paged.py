@@ -319,6 +319,32 @@ def test_short_rows_beside_a_long_one(dtype, new):
     attend_case(33, [5200, 70, 1025, 65], new, 1, 1, 128, 32, dtype, dict(softcap=20.0))
 
 
+def test_a_single_token_beside_a_long_prompt():
+    """The prompt's blocks fill the card and stay whole, the single token's long row is cut into pieces."""
+    H, G, d, P, dtype = 64, 1, 64, 64, torch.bfloat16
+    lengths, new = [2100, 5200, 0], [2100, 1, 0]
+    g = gen(35)
+    k, v = (torch.randn(120, H, P, d, generator=g).to(dtype) for _ in range(2))
+    cache = PagedCache(3, 120, P, H, d, dtype)
+    cache.k_pages.copy_(k), cache.v_pages.copy_(v)
+    pages = torch.randperm(120, generator=g)
+    rows = [pages[:33], pages[33:115], pages[:0]]
+    for r, at in enumerate(rows):
+        cache.table[r, :len(at)] = at.int().cuda()
+    cache.length.copy_(i32(lengths))
+    q = torch.randn(sum(new), H, d, generator=g).to(dtype)
+    out, lse = cache.attend(q.cuda(), cu_of(new), d ** -0.5)
+    for r, start, tokens in ((0, 0, [0, 1, 127, 128, 1500, 2099]), (1, 2100, [0])):
+        n, m = lengths[r], new[r]
+        kr, vr = (x[rows[r]].transpose(0, 1).reshape(H, -1, d)[:, :n] for x in (k, v))
+        seen = O.seen_mask(m, n, True, None)[tokens]
+        at = torch.tensor(tokens) + start
+        for h in range(0, H, 7):
+            f = O.attention(q[at, h], kr[h], vr[h], d ** -0.5, seen, 0.0, 0.0, t=dtype)
+            close(out[at.cuda(), h], f["out"], f["out_tol"], f"row {r} head {h} out")
+            close(lse[at.cuda(), h], f["lse"], f["lse_tol"], f"row {r} head {h} lse")
+
+
 def test_bad_page_numbers_stay_inside_the_pool():
     cache, q, cu, terms, out, lse = attend_case(29, [100, 70], [1, 30], 1, 2, 128, 16, torch.bfloat16, {})
     cache.table[0, 2] = 1 << 30

@@ -15,6 +15,9 @@
 // Bound: HBM for the rows that move (each read once and written once, 16 bytes per lane).  For a decode step
 // (some hundred kilobytes) the two launches and the search for free pages are all of it; the search starts at a
 // page number below which nothing is free, kept with the bookkeeping, and ends with the last page it needs.
+// Measured (16-bit, 8 heads, d = 128): compact of 1.07 GB 217 us = 4.9 TB/s, what a copy of 2 GiB reaches here, behind 13 us of
+// bookkeeping; 96 MB of prompts 17 us = 5.8 TB/s behind 10; a token for each of 64 rows 4 us behind 7; a fork 6 behind 8: the
+// deciding workgroup's chain of scans and dependent loads (a launch alone is 2).
 #include <algorithm>
 #include <initializer_list>
 

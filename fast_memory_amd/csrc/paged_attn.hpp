@@ -21,7 +21,10 @@
 
 namespace fm {
 
-constexpr int kFewRows = 32;   // query rows of a KV head up to which a row is `few`
+// Query rows of a KV head up to which a row is `few`.  Measured, 8 KV heads, d = 128, bf16, few and many at 32 query rows: one row
+// of 4096 keys 21.8 and 22.5 us, of 32 768 53.1 and 49.9, 16 rows of 4096 59.1 and 62.1, 64 of 512 28.6 and 29.4; at 40 query
+// rows 16 of 4096 138 and 64.
+constexpr int kFewRows = 32;
 constexpr int kFewKeys = 32;   // keys of a tile of a wave
 
 struct PagedTileArgs {

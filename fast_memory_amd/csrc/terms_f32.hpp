@@ -12,6 +12,11 @@
 //   second product       register r of both halves is the operand of one instruction: rows k and k + 4; its partner is
 //                        one element per lane of those two rows, 32 neighbouring dimensions
 // Head dimensions are padded with zeros to Dp = 32 NDT in registers only.
+//
+// Measured in fp32 (a product of 8192 reaches 154 TFLOP/s): 16 heads x 2048 causal, d = 64 0.13 ms forward = 67 TFLOP/s and 0.45
+// backward, d = 128 0.26 and 0.79, d = 256 (1024 tokens) 0.14 and 0.58; one head of 512 tokens 24 and 39 us.  Bound: the loads'
+// latency between the products, at one wave a SIMD (d > 64) or two.  Eight waves a workgroup instead of four: 20 and 54 us for
+// 8 heads x 512, where four take 22 and 42 (the backward's registers no longer hold).
 #pragma once
 #include <type_traits>
 

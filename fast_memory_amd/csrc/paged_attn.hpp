@@ -526,7 +526,9 @@ struct PagedPlan {
 };
 
 // Pieces until there are about 1024 workgroups (four a compute unit), but none of less than 512 keys by the table's
-// width.
+// width.  Measured, 512 and 1024 workgroups (8 KV heads, d = 128): 32 ragged rows of up to 32 768 keys 623 and 607 us, ragged chunks of
+// 1024 tokens 1075 and 1001 (finer pieces end more evenly); 16 equal rows of 4096 under 32 query rows each 53.5 and 59.3.
+// 2048: as 1024.
 inline PagedPlan paged_plan(int rows, int T, int max_new, int H, int G, int d, int64_t keys) {
   PagedPlan y{};
   const bool known = max_new > 0 && max_new <= T;

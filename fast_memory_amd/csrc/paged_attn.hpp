@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
         for (int r = 1; r < 8; ++r) mx = fmaxf(mx, y[r]);
         mx = st_max_lane_groups(mx);
         const float m_new = fmaxf(m[i], mx);
-        if (__any(m_new > m[i] + 8.f)) {
+        if (__any(m_new > m[i] + kPLazy<F16>)) {
           const float m_to = m_new == -INFINITY ? 0.f : m_new;
           const float alpha = __builtin_amdgcn_exp2f(m[i] - m_to);
           sum[i] *= alpha;
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
             for (int r = 0; r < 4; ++r) O[i][k][r] *= alpha;
           m[i] = m_new;
         }
-        const float base = m[i] == -INFINITY ? 0.f : m[i];
+        const float base = m[i] == -INFINITY ? 0.f : m[i] - kPUp<F16>;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           y[r] = __builtin_amdgcn_exp2f(y[r] - base);
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
         for (int r = 0; r < 4; ++r)
           *reinterpret_cast<float4*>(mine + 64 * j + 16 * g + 4 * r) =
               make_float4(O[i][4 * j][r], O[i][4 * j + 1][r], O[i][4 * j + 2][r], O[i][4 * j + 3][r]);
-      if (g == 0) lds_ml[w * 16 + c] = make_float2(m[i], ls);
+      if (g == 0) lds_ml[w * 16 + c] = make_float2(m[i] - kPUp<F16>, ls);
       __syncthreads();
       // 16 threads a query, each D / 16 dimensions
       const int q = tid >> 4, r = r0 + 16 * i + q, part = tid & 15;

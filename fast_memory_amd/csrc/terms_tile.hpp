@@ -30,6 +30,16 @@ constexpr int kTQ = 128;  // query rows of a workgroup
 template <int D>
 constexpr int fwd_tile_keys() { return D == 256 ? 32 : 64; }
 
+// The probabilities of the product with the values are held times 2^kPUp in fp16, and against a running maximum that is at most
+// 2^kPLazy behind the true one: at most 2^15 of fp16's 65504, and a key that weighs 2^-37 of the largest is half the smallest number
+// fp16 holds, so that what falls below is off by at most 2^-37 of it a key: 2^-13 in all for the 2^24 keys a row may have, under the
+// rounding of the result.  (Unscaled, 65 535 keys 17.5 under one key without a value gave 0 where 1.6e-3 is right.)  bf16 has fp32's
+// range.  The factor costs nothing: it sits in the maximum that the exponents are taken against, and in the sums as well.
+template <bool F16>
+constexpr float kPUp = F16 ? 12.f : 0.f;
+template <bool F16>
+constexpr float kPLazy = F16 ? 3.f : 8.f;
+
 // what the scores have, beside the product: bit 0 the cap, bit 1 the distance bias
 constexpr int kModeCap = 1, kModeBias = 2;
 
@@ -310,7 +320,7 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
   typedef TileLds<D, KT> T;
   using M = Mma<F16>;
   constexpr int NKS = D / 16, NDT = D / 32;
-  constexpr float kLazyGrow = 8.f;  // growth of a running maximum (in powers of two) that is left unfollowed
+  constexpr float kLazyGrow = kPLazy<F16>;  // growth of a running maximum (in powers of two) that is left unfollowed
   const int tid = threadIdx.x, l = tid & 63, hb = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(lds)));
@@ -408,7 +418,7 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
         for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
       st.m = m_new;
     }
-    const float m_sub = st.m == -INFINITY ? 0.f : st.m;
+    const float m_sub = st.m == -INFINITY ? 0.f : st.m - kPUp<F16>;
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
       uint4 pf[2];
@@ -473,6 +483,7 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
       step(1);
     }
   }
+  st.m -= kPUp<F16>;  // what the sums are against (-inf stays)
   if (dirty) *dirty_flag = 1;  // (every writer writes the same)
   __syncthreads();
   return *dirty_flag != 0;

@@ -1,0 +1,62 @@
+"""The local side at its edges: what lies far below the largest score, tokens that a caller did not announce, infinities in
+the last key, refusals around a snapshot, integers beyond 32 bits (bounds derived in oracle/local_side.py)."""
+import pytest
+import torch
+
+from fast_memory_amd import PagedCache, ops
+from oracle import local_side as O
+from tests.test_gpu_local_terms import close
+from tests.test_gpu_paged import cu_of, i32
+from tests.util import gen
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+# ------------------------------------------------------------------ keys far below the largest score
+def tail(seed, L, d, dtype, below, dominant=0):
+    """One key at score 0 whose value is 0, and L - 1 keys `below` under it with values in [1/2, 1): their weights are small one by
+    one and not together.  The query is the first unit vector times sqrt(d), so that the scale d^-1/2 leaves k's first element."""
+    q = torch.zeros(d)
+    q[0] = d ** 0.5
+    k = torch.zeros(L, d)
+    k[:, 0] = -below
+    k[dominant] = 0
+    v = 0.5 + 0.5 * torch.rand(L, d, generator=gen(seed)) * (1 - 2 ** -7)
+    v[dominant] = 0
+    return q.to(dtype), k.to(dtype), v.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("S,L,dominant", [(1, 65536, 0), (33000, 32768, 0), (33000, 32768, 20000)])
+def test_a_long_tail_under_one_key(dtype, d, S, L, dominant):
+    if dtype == torch.float32 and S > 1:
+        S = 300
+    q, k, v = tail(3, L, d, dtype, 17.5, dominant)
+    out, lse = ops.local_attn_terms_fwd(q.expand(1, S, d).contiguous().cuda(), k[None].cuda(), v[None].cuda(), d ** -0.5, False)
+    f = O.attention(q[None], k, v, d ** -0.5, torch.ones(1, L, dtype=torch.bool), t=dtype)
+    assert f["out"].min() > 2 ** -11                        # (the tail is most of the answer)
+    close(out[0], f["out"].expand(S, d), f["out_tol"].expand(S, d), "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,new,G", [(128, 1, 1), (128, 3, 4), (16, 80, 8)])
+def test_a_long_tail_in_a_cache(dtype, d, rows, new, G):
+    # all rows name the same pages; as many rows as it takes that a row's keys stay in one piece
+    H, P, L = 8, 16, 32768
+    if dtype == torch.float32:
+        rows, new = 4, min(new, 4)
+    q, k, v = tail(5, L, d, dtype, 17.5)
+    pages = lambda x: x.view(L // P, 1, P, d).expand(L // P, H, P, d).contiguous().cuda()
+    book = torch.zeros(16 + rows + L // P + rows * (L // P), dtype=torch.int32)
+    book[16:16 + rows] = L
+    book[16 + rows:16 + rows + L // P] = rows
+    book[16 + rows + L // P:] = torch.arange(L // P, dtype=torch.int32).repeat(rows)
+    c = PagedCache.over(pages(k), pages(v), book.cuda(), rows)
+    out, lse = c.attend(q.expand(rows * new, H * G, d).contiguous().cuda(), cu_of([new] * rows), d ** -0.5, max_new=new)
+    f = O.attention(q[None].expand(new, d), k, v, d ** -0.5, O.seen_mask(new, L, True), t=dtype)
+    whole = lambda x: x.unsqueeze(1).expand(new, H * G, *x.shape[1:]).repeat(rows, *[1] * x.dim())
+    close(out, whole(f["out"]), whole(f["out_tol"]), "out")

@@ -269,11 +269,13 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
           m[i] = m_new;
         }
         const float base = m[i] == -INFINITY ? 0.f : m[i] - kPUp<F16>;
+        float s_tile = 0.f;  // (by itself first, see tile_sweep)
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           y[r] = __builtin_amdgcn_exp2f(y[r] - base);
-          sum[i] += y[r];
+          s_tile += y[r];
         }
+        sum[i] += s_tile;
         pf[i] = make_uint4(M::pack2(y[0], y[1]), M::pack2(y[2], y[3]), M::pack2(y[4], y[5]), M::pack2(y[6], y[7]));
       }
       // values that 0 x would not erase, where some query does not see some key

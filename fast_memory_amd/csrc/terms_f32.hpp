@@ -258,11 +258,13 @@ __device__ __forceinline__ void f32_forward(const float (&qf)[16 * NDT], int pos
         for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
     }
     m = m_new;
+    float s_tile = 0.f;  // (by itself first, see tile_sweep)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = __builtin_amdgcn_exp2f(x[r] - base);
-      sum += x[r];
+      s_tile += x[r];
     }
+    sum += s_tile;
     if constexpr (FLAT) {
       const int last = n - 1 - kp0;
       f32_accumulate<T, NDT>(O, x, V + int64_t(kp0) * d, [&](int k) { return unsigned(min(k, last) * d); }, d, hb, col, masked, dirty);

@@ -419,13 +419,15 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
       st.m = m_new;
     }
     const float m_sub = st.m == -INFINITY ? 0.f : st.m - kPUp<F16>;
+    // (a tile's probabilities are summed by themselves first: one by one a large sum would swallow small ones)
+    float l_tile = 0.f;
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
       uint4 pf[2];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         x[sb][r] = __builtin_amdgcn_exp2f(MODE == 0 ? fmaf(x[sb][r], score.in, -m_sub) : x[sb][r] - m_sub);
-        st.l += x[sb][r];
+        l_tile += x[sb][r];
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -436,6 +438,7 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bV, at.cols, 32 * sb + 16 * h, dt), pf[h], O[dt]);
     }
+    st.l += l_tile;
   };
 
   const uint32_t lds_docs = lds0 + 4u * T::kBytes;

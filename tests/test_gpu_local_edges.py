@@ -28,6 +28,14 @@ def tail(seed, L, d, dtype, below, dominant=0):
     return q.to(dtype), k.to(dtype), v.to(dtype)
 
 
+def sum_tol(f, L):
+    """The oracle's bound of the log-sum-exp leaves out the rounding of the sum itself.  A tile of at least 16 of a lane's keys is
+    summed first (one of 32 keys, 8 of them a lane's, in the kernel for few rows, whose four waves take every fourth), then added:
+    at most L / 32 + 32 additions of positive numbers follow one another, each off by 2^-24 of a sum that is at most the whole, and
+    at most 64 pieces are joined.  The logarithm is off by the sum's relative error."""
+    return f["lse_tol"] + (L / 32 + 96) * O.W
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("S,L,dominant", [(1, 65536, 0), (33000, 32768, 0), (33000, 32768, 20000)])
@@ -39,6 +47,7 @@ def test_a_long_tail_under_one_key(dtype, d, S, L, dominant):
     f = O.attention(q[None], k, v, d ** -0.5, torch.ones(1, L, dtype=torch.bool), t=dtype)
     assert f["out"].min() > 2 ** -11                        # (the tail is most of the answer)
     close(out[0], f["out"].expand(S, d), f["out_tol"].expand(S, d), "out")
+    close(lse[0], f["lse"].expand(S), sum_tol(f, L).expand(S), "lse")
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -60,3 +69,4 @@ def test_a_long_tail_in_a_cache(dtype, d, rows, new, G):
     f = O.attention(q[None].expand(new, d), k, v, d ** -0.5, O.seen_mask(new, L, True), t=dtype)
     whole = lambda x: x.unsqueeze(1).expand(new, H * G, *x.shape[1:]).repeat(rows, *[1] * x.dim())
     close(out, whole(f["out"]), whole(f["out_tol"]), "out")
+    close(lse, whole(f["lse"]), whole(sum_tol(f, L)), "lse")

@@ -198,7 +198,6 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
     }
     int j0, j1;
     piece_keys(lim_hi, kFewKeys, piece, a.few_pieces, j0, j1);
-    const bool one_limit = lim_lo == lim_hi;
 
     f4 O[NQ][NM];
     float m[NQ], sum[NQ];
@@ -278,8 +277,9 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
         sum[i] += s_tile;
         pf[i] = make_uint4(M::pack2(y[0], y[1]), M::pack2(y[2], y[3]), M::pack2(y[4], y[5]), M::pack2(y[6], y[7]));
       }
-      // values that 0 x would not erase, where some query does not see some key
-      if (masked && !one_limit) {
+      // values that 0 x would not erase, where some query does not see some key (the row's last key, repeated behind its end, is such
+      // a place too: an infinite value of it is not NaN)
+      if (masked) {
 #pragma unroll
         for (int r = 0; r < 8; ++r)
 #pragma unroll

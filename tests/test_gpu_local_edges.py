@@ -70,3 +70,48 @@ def test_a_long_tail_in_a_cache(dtype, d, rows, new, G):
     whole = lambda x: x.unsqueeze(1).expand(new, H * G, *x.shape[1:]).repeat(rows, *[1] * x.dim())
     close(out, whole(f["out"]), whole(f["out_tol"]), "out")
     close(lse, whole(f["lse"]), whole(sum_tol(f, L)), "lse")
+
+
+# ------------------------------------------------------------------ values that are not finite
+def one_row(seed, n, new, H, G, d, P, dtype):
+    """A cache of one row of n tokens in order, and queries of its last `new`."""
+    g = gen(seed)
+    k, v = (torch.randn(n, H, d, generator=g).to(dtype) for _ in range(2))
+    c = PagedCache(1, -(-n // P), P, H, d, dtype)
+    q = torch.randn(new, H * G, d, generator=g).to(dtype)
+    return c, k, v, q
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("G,new,max_new", [(16, 2, 1), (32, 2, 1), (16, 3, 2), (8, 5, 1), (1, 40, 3), (16, 2, 2), (16, 2, 0), (32, 4, 0)])
+@pytest.mark.parametrize("n", [100, 128, 1100])
+def test_more_new_tokens_than_announced(dtype, G, new, max_new, n):
+    """max_new shapes the launch only: with too small a one the results are right, and a later token's NaN stays out of earlier ones."""
+    H, d, P = 2, 64, 16
+    c, k, v, q = one_row(11, n, new, H, G, d, P, dtype)
+    v[-1] = float("nan")
+    c.append(k.cuda(), v.cuda(), i32([0, n]))
+    out, lse = c.attend(q.cuda(), i32([0, new]), d ** -0.5, max_new=max_new)
+    for h in range(H * G):
+        f = O.attention(q[:, h], k[:, h // G], v[:, h // G], d ** -0.5, O.seen_mask(new, n, True), t=dtype)
+        f["out_tol"] = f["out_tol"].nan_to_num(0)
+        close(out[:-1, h], f["out"][:-1], f["out_tol"][:-1], f"head {h} out")
+        close(lse[:, h], f["lse"], f["lse_tol"], f"head {h} lse")
+    assert torch.isnan(out[-1]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n,new,G", [(1, 1, 4), (33, 1, 4), (97, 1, 1), (100, 3, 4), (100, 60, 2), (1500, 1, 8)])
+def test_an_infinite_value_in_the_last_key(dtype, d, n, new, G):
+    # the last token sees it and comes out infinite, where its probability is not zero: no NaN from the places behind it
+    H, P = 1, 16
+    c, k, v, q = one_row(13, n, new, H, G, d, P, dtype)
+    v[-1, :, ::2] = float("inf")
+    v[-1, :, 1::4] = -float("inf")
+    c.append(k.cuda(), v.cuda(), i32([0, n]))
+    out, _ = c.attend(q.cuda(), i32([0, new]), d ** -0.5, max_new=new)
+    assert torch.equal(out[-1], v[-1].cuda().expand(G, d)) if n == 1 else \
+        torch.equal(out[-1][:, ~torch.isfinite(v[-1, 0])].cpu(), v[-1][:, ~torch.isfinite(v[-1, 0])].expand(G, -1))
+    finite = torch.isfinite(v[-1, 0])
+    assert torch.isfinite(out[-1][:, finite]).all() and torch.isfinite(out[:-1]).all()

@@ -115,3 +115,21 @@ def test_an_infinite_value_in_the_last_key(dtype, d, n, new, G):
         torch.equal(out[-1][:, ~torch.isfinite(v[-1, 0])].cpu(), v[-1][:, ~torch.isfinite(v[-1, 0])].expand(G, -1))
     finite = torch.isfinite(v[-1, 0])
     assert torch.isfinite(out[-1][:, finite]).all() and torch.isfinite(out[:-1]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_gradient_that_is_not_finite_is_not_lost(dtype, d):
+    """Key 7 weighs nothing (its score is 1e4 under the others'), and D of every query that sees it is not finite: its gradient is 0
+    times that, in a tile with masked places as in one without.  Queries that see no such value keep theirs."""
+    S = 40
+    g = gen(17)
+    q, k, v, do = (torch.randn(1, S, d, generator=g).to(dtype) for _ in range(4))
+    q[..., 0] = d ** 0.5
+    k[..., 0] = 0
+    k[:, 7, 0] = -1e4
+    v[:, 7:9] = float("inf")
+    q, k, v, do = (x.cuda() for x in (q, k, v, do))
+    out, lse = ops.local_attn_terms_fwd(q, k, v, d ** -0.5, True)
+    dq, dk, dv = ops.local_attn_terms_bwd(do, q, k, v, out, lse, d ** -0.5, True)
+    assert not torch.isfinite(dk[0, 7]).any() and torch.isfinite(dq[0, :7]).all() and not torch.isfinite(dq[0, 8:]).any()

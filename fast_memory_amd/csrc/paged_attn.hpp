@@ -256,9 +256,8 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
 #pragma unroll
         for (int r = 1; r < 8; ++r) mx = fmaxf(mx, y[r]);
         mx = st_max_lane_groups(mx);
-        const float m_new = fmaxf(m[i], mx);
-        if (__any(m_new > m[i] + kPLazy<F16>)) {
-          const float m_to = m_new == -INFINITY ? 0.f : m_new;
+        if (__any(mx > m[i] + (kPUp<F16> + kPLazy<F16>))) {  // (m is held kPUp below the maximum)
+          const float m_new = fmaxf(m[i], mx - kPUp<F16>), m_to = m_new == -INFINITY ? 0.f : m_new;
           const float alpha = __builtin_amdgcn_exp2f(m[i] - m_to);
           sum[i] *= alpha;
 #pragma unroll
@@ -267,7 +266,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
             for (int r = 0; r < 4; ++r) O[i][k][r] *= alpha;
           m[i] = m_new;
         }
-        const float base = m[i] == -INFINITY ? 0.f : m[i] - kPUp<F16>;
+        const float base = m[i] == -INFINITY ? 0.f : m[i];
         float s_tile = 0.f;  // (by itself first, see tile_sweep)
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -335,7 +334,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
         for (int r = 0; r < 4; ++r)
           *reinterpret_cast<float4*>(mine + 64 * j + 16 * g + 4 * r) =
               make_float4(O[i][4 * j][r], O[i][4 * j + 1][r], O[i][4 * j + 2][r], O[i][4 * j + 3][r]);
-      if (g == 0) lds_ml[w * 16 + c] = make_float2(m[i] - kPUp<F16>, ls);
+      if (g == 0) lds_ml[w * 16 + c] = make_float2(m[i], ls);
       __syncthreads();
       // 16 threads a query, each D / 16 dimensions
       const int q = tid >> 4, r = r0 + 16 * i + q, part = tid & 15;

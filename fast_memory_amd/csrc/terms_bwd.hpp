@@ -622,7 +622,7 @@ __device__ __forceinline__ void dkv_block(const BwdTileArgs& a, int block, bf16_
     const RowQueries rq{rows + 4 * hb * 4};
     block_probs<MODE>(x, y, a.score, float(j - (i0 + 4 * hb + (a.L - a.S))), slope2, rq);
     const bool masked = mixed || ragged || wj0 + 32 > lo;
-    unsigned unseen = 0;  // bit r: this lane's key is not seen by the query of register r
+    constexpr float kUnseen = -4.f;  // in the place of p slack, which is 0 or (rounded) -2^-21 p at the least
     if (masked) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -638,8 +638,7 @@ __device__ __forceinline__ void dkv_block(const BwdTileArgs& a, int block, bf16_
           const int i = i0 + iq + e;
           bool ok = i < a.S && j < (a.use_masks ? ll[e] : seen_limit(i + (a.L - a.S), a.L, a.t.causal, 0));
           if constexpr (DOCS) ok = ok && dd[e] == doc;
-          unseen |= unsigned(!ok) << (4 * q + e);
-          x[4 * q + e] = ok ? x[4 * q + e] : 0.f;
+          if (!ok) x[4 * q + e] = 0.f, y[4 * q + e] = kUnseen;
         }
       }
     }
@@ -667,9 +666,10 @@ __device__ __forceinline__ void dkv_block(const BwdTileArgs& a, int block, bf16_
       gr[r] = (pr[r] - rq.delta(r)) * y[r];
       if constexpr (F16) gr[r] *= g_scale;
     }
-    if (masked) {  // (by the mask, not by p: a seen pair's p may be 0 beside a gradient that is not finite)
+    if (masked) {  // (where the mask is, not where p is 0: a seen pair's may be, beside a gradient that is not finite)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) gr[r] = (unseen >> r & 1) ? 0.f : gr[r];
+      for (int r = 0; r < 16; ++r)
+        if (y[r] == kUnseen) gr[r] = 0.f;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {

@@ -34,7 +34,8 @@ constexpr int fwd_tile_keys() { return D == 256 ? 32 : 64; }
 // 2^kPLazy behind the true one: at most 2^15 of fp16's 65504, and a key that weighs 2^-37 of the largest is half the smallest number
 // fp16 holds, so that what falls below is off by at most 2^-37 of it a key: 2^-13 in all for the 2^24 keys a row may have, under the
 // rounding of the result.  (Unscaled, 65 535 keys 17.5 under one key without a value gave 0 where 1.6e-3 is right.)  bf16 has fp32's
-// range.  The factor costs nothing: it sits in the maximum that the exponents are taken against, and in the sums as well.
+// range.  The factor costs nothing: it sits in the maximum that the exponents are taken against, and in the sums as well.  (A
+// maximum followed from 2^5 or 2^8 on instead of 2^3 is no faster.)
 template <bool F16>
 constexpr float kPUp = F16 ? 12.f : 0.f;
 template <bool F16>
@@ -407,9 +408,9 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
     // The running maximum follows only when some query's grew by more than 2^kLazyGrow (or it sees its first key): until
     // then p stays below 2^kLazyGrow against the older maximum, which neither the fp32 sums nor the relative rounding
     // of p notice, and the accumulator's multiplications are spared in most tiles.
-    const float m_new = fmaxf(st.m, mx);
-    if (__any(m_new > st.m + kLazyGrow)) {
-      const float m_to = m_new == -INFINITY ? 0.f : m_new;
+    // (st.m is held kPUp below the maximum it stands for: what the exponents are taken against)
+    if (__any(mx > st.m + (kPUp<F16> + kLazyGrow))) {
+      const float m_new = fmaxf(st.m, mx - kPUp<F16>), m_to = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = __builtin_amdgcn_exp2f(st.m - m_to);
       st.l *= alpha;
 #pragma unroll
@@ -418,17 +419,17 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
         for (int r = 0; r < 16; ++r) O[dt][r] *= alpha;
       st.m = m_new;
     }
-    const float m_sub = st.m == -INFINITY ? 0.f : st.m - kPUp<F16>;
-    // (a tile's probabilities are summed by themselves first: one by one a large sum would swallow small ones)
-    float l_tile = 0.f;
+    const float m_sub = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb) {
       uint4 pf[2];
+      float l_block;  // (a block's probabilities are summed by themselves first: one by one a large sum would swallow small ones)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         x[sb][r] = __builtin_amdgcn_exp2f(MODE == 0 ? fmaf(x[sb][r], score.in, -m_sub) : x[sb][r] - m_sub);
-        l_tile += x[sb][r];
+        l_block = r == 0 ? x[sb][0] : l_block + x[sb][r];
       }
+      st.l += l_block;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         pf[h] = make_uint4(M::pack2(x[sb][8 * h + 0], x[sb][8 * h + 1]), M::pack2(x[sb][8 * h + 2], x[sb][8 * h + 3]),
@@ -438,7 +439,6 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) O[dt] = M::m32(T::cols32(bV, at.cols, 32 * sb + 16 * h, dt), pf[h], O[dt]);
     }
-    st.l += l_tile;
   };
 
   const uint32_t lds_docs = lds0 + 4u * T::kBytes;
@@ -486,7 +486,6 @@ __device__ __forceinline__ bool tile_sweep(Source src, const uint4 (&qf)[D / 16]
       step(1);
     }
   }
-  st.m -= kPUp<F16>;  // what the sums are against (-inf stays)
   if (dirty) *dirty_flag = 1;  // (every writer writes the same)
   __syncthreads();
   return *dirty_flag != 0;

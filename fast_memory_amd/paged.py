@@ -25,7 +25,8 @@ class PagedCache:
     record into a graph; a request that cannot be met (:data:`REFUSALS`) changes nothing and is counted, and
     :meth:`check`, called wherever waiting costs nothing, raises.  The calls of one cache follow each other on one
     stream, or are ordered by events.  ``snapshot`` / ``restore`` take the bookkeeping back (speculative tokens that
-    were not accepted); a page that a call after the snapshot freed, or moved, may hold other rows by then.
+    were not accepted), but not the count of refused calls; a page that a call after the snapshot freed, or moved, may
+    hold other rows by then.
     """
 
     def __init__(self, n_rows: int, n_pages: int, page_size: int, n_heads: int, d: int,
@@ -96,7 +97,9 @@ class PagedCache:
         return self.book.clone()
 
     def restore(self, book: torch.Tensor) -> None:
-        self.book.copy_(book)
+        if book.shape != self.book.shape:
+            raise ValueError(f"PagedCache.restore: {tuple(book.shape)} is no snapshot of this cache ({tuple(self.book.shape)})")
+        self.book[2:].copy_(book[2:])  # (what check() counts stays: a refused call stays refused)
 
     def check(self) -> None:
         """Raises when a call since the last check was refused (synchronises)."""

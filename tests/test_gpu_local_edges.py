@@ -133,3 +133,30 @@ def test_a_gradient_that_is_not_finite_is_not_lost(dtype, d):
     out, lse = ops.local_attn_terms_fwd(q, k, v, d ** -0.5, True)
     dq, dk, dv = ops.local_attn_terms_bwd(do, q, k, v, out, lse, d ** -0.5, True)
     assert not torch.isfinite(dk[0, 7]).any() and torch.isfinite(dq[0, :7]).all() and not torch.isfinite(dq[0, 8:]).any()
+
+
+# ------------------------------------------------------------------ the cache
+def test_a_refusal_outlives_a_restore():
+    c = PagedCache(2, 3, 4, 1, 8, torch.float32)
+    k = torch.randn(16, 1, 8, device="cuda")
+    c.append(k, k, i32([0, 4, 5]))
+    saved = c.snapshot()
+    c.append(k, k, i32([0, 9, 9]))                           # a fourth page for a row of three
+    c.restore(saved)
+    assert c.length.tolist() == [4, 1]
+    with pytest.raises(RuntimeError, match="1 call.*outgrow its table"):
+        c.check()
+    # and one that was told about is not told again
+    c.append(k, k, i32([0, 9, 9]))
+    saved = c.snapshot()
+    with pytest.raises(RuntimeError, match="1 call"):
+        c.check()
+    c.append(k, k, i32([0, 1, 2]))
+    c.restore(saved)
+    c.check()
+    assert c.length.tolist() == [4, 1] and c.table.tolist() == [[0, -1, -1], [1, -1, -1]] and c.refs.tolist() == [1, 1, 0]
+    c.append(k, k, i32([0, 2, 3]))                           # the page that came back is found again
+    c.check()
+    assert c.table.tolist() == [[0, 2, -1], [1, -1, -1]]
+    with pytest.raises(ValueError, match="no snapshot"):
+        c.restore(saved[:1])

@@ -547,11 +547,14 @@ def _call(fn, like: torch.Tensor, *args) -> None:
 
 
 def _row_ints(t: torch.Tensor, n: int, like: torch.Tensor, what: str) -> torch.Tensor:
-    """An int32 vector of n entries on ``like``'s device (int64 is cast at the edge)."""
+    """An int32 vector of n entries on ``like``'s device.  int64 is cast at the edge, what does not fit to the nearest that does: a
+    limit or an offset too large stays too large."""
     if t.shape != (n,) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: {n} integers, got {tuple(t.shape)} {t.dtype}")
     _same_device(like, t)
-    return t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+    return t.contiguous()
 
 
 def cache_append_(cache, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor) -> None:
@@ -606,7 +609,7 @@ class ScoreTerms(NamedTuple):
     * ``prefix [S]`` int: query i sees the keys ``j < prefix[i]`` whatever the causal mask says (of its own document,
       where there are any).  Over a paged cache it is ``[n_rows]``, and a row is a document of its own.
 
-    int64 tensors are cast: their values have to fit 32 bits.
+    int64 tensors are cast, what does not fit 32 bits to the nearest that does: documents' numbers have to fit.
     """
     softcap: float = 0.0
     slopes: Optional[torch.Tensor] = None

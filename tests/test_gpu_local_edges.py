@@ -3,7 +3,7 @@ the last key, refusals around a snapshot, integers beyond 32 bits (bounds derive
 import pytest
 import torch
 
-from fast_memory_amd import PagedCache, ops
+from fast_memory_amd import PagedCache, ScoreTerms, ops
 from oracle import local_side as O
 from tests.test_gpu_local_terms import close
 from tests.test_gpu_paged import cu_of, i32
@@ -160,3 +160,29 @@ def test_a_refusal_outlives_a_restore():
     assert c.table.tolist() == [[0, 2, -1], [1, -1, -1]]
     with pytest.raises(ValueError, match="no snapshot"):
         c.restore(saved[:1])
+
+
+def test_integers_beyond_32_bits():
+    """int64 arguments: what does not fit 32 bits does not come back as another number."""
+    i64 = lambda x: torch.tensor(x, dtype=torch.int64, device="cuda")
+    H, d, P = 1, 64, 4
+    c = PagedCache(2, 8, P, H, d, torch.float32)
+    k, v = (torch.randn(6, H, d, generator=gen(21)).cuda() for _ in range(2))
+    c.append(k, v, i64([0, (1 << 32) + 1, 1 << 33]))          # (as 32 bits: 0, 1, 0 and 0, 1, ..)
+    c.fork(i64([1 << 32, -1]))                               # (from row 0)
+    with pytest.raises(RuntimeError, match="2 call"):
+        c.check()
+    assert c.length.tolist() == [0, 0] and c.refs.sum() == 0
+    c.append(k, v, i64([0, 6, 6]))
+    q = torch.randn(2, H, d, generator=gen(22)).cuda()
+    want = c.attend(q, i32([0, 2, 2]), 0.1, ScoreTerms(prefix=i32([6, 0])))
+    got = c.attend(q, i64([0, 2, 2]), 0.1, ScoreTerms(prefix=i64([1 << 40, -(1 << 40)])))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    c.drop(i64([1 << 40, -(1 << 32) + 1]))
+    c.check()
+    assert c.length.tolist() == [0, 0] and c.refs.sum() == 0
+    x = torch.randn(1, 5, d, generator=gen(23)).cuda()
+    doc = [0, 0, -(1 << 32), 0, 0]                             # (as 32 bits: 0, no padding)
+    a = ops.local_attn_terms_fwd(x, x, x, 0.1, True, ScoreTerms(doc_q=i64(doc), doc_k=i64(doc)))
+    b = ops.local_attn_terms_fwd(x, x, x, 0.1, True, ScoreTerms(doc_q=i32([0, 0, -1, 0, 0]), doc_k=i32([0, 0, -1, 0, 0])))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -29,9 +29,9 @@ __host__ __device__ __forceinline__ Book book_of(int32_t* b, int n_pages, int R)
   return k;
 }
 
-// P is a power of two
+// P is a power of two; a row may hold up to 2^31 - 1 tokens
 __host__ __device__ __forceinline__ int pages_of(int tokens, int log2p) {
-  return (tokens + (1 << log2p) - 1) >> log2p;
+  return (tokens >> log2p) + ((tokens & ((1 << log2p) - 1)) != 0);
 }
 
 static inline int log2_exact(int x) {  // -1: no power of two

@@ -186,3 +186,25 @@ def test_integers_beyond_32_bits():
     a = ops.local_attn_terms_fwd(x, x, x, 0.1, True, ScoreTerms(doc_q=i64(doc), doc_k=i64(doc)))
     b = ops.local_attn_terms_fwd(x, x, x, 0.1, True, ScoreTerms(doc_q=i32([0, 0, -1, 0, 0]), doc_k=i32([0, 0, -1, 0, 0])))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_a_row_near_2_to_the_31_tokens():
+    """The page count of a row whose last page ends behind 2^31 - 1."""
+    P, width = 4096, 1 << 19
+    c = PagedCache(1, 4, P, 1, 8, torch.bfloat16, max_tokens=width * P)
+    c.length.fill_((width - 1) * P)                           # all but one page of the table, as if they were held
+    k = torch.randn(3, 1, 8, generator=gen(25)).to(torch.bfloat16).cuda()
+    c.append(k[:1], k[:1], i32([0, 1]))
+    c.append(k[1:], k[1:], i32([0, 2]))
+    c.check()
+    assert c.length.tolist() == [(width - 1) * P + 3] and c.table[0, -2:].tolist() == [-1, 0] and c.refs.tolist() == [1, 0, 0, 0]
+    assert torch.equal(c.k_pages[0, 0, :3], k[:, 0])
+    c.append(k[:1].expand(P - 4, 1, 8), k[:1].expand(P - 4, 1, 8), i32([0, P - 4]))
+    c.check()
+    c.append(k[:1], k[:1], i32([0, 1]))                       # 2^31
+    with pytest.raises(RuntimeError, match="outgrow"):
+        c.check()
+    c.drop(i32([width - 1]))
+    assert c.length.tolist() == [P - 1] and c.table[0, :2].tolist() == [0, -1]
+    c.drop(i32([1]))
+    assert c.length.tolist() == [0] and c.refs.tolist() == [0, 0, 0, 0]

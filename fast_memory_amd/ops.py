@@ -701,6 +701,8 @@ def paged_attn_fwd(q: torch.Tensor, cache, cu: torch.Tensor, sm_scale: float, te
         raise ValueError(f"attend: q is [T, {cache.n_heads} G, {cache.d}] {kp.dtype}, got {tuple(q.shape)} {q.dtype}")
     if not q.is_cuda:
         raise RuntimeError("libfastmem operators take GPU tensors only (there is no CPU path)")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise ValueError("attend has no backward: pass q detached, or call it under torch.no_grad()")
     _same_device(kp, q)
     T, HG, d = q.shape
     t = _NO_TERMS if terms is None else terms

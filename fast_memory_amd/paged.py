@@ -70,7 +70,8 @@ class PagedCache:
 
     # ------------------------------------------------------------------ rows come, are forked, and leave
     def append(self, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor) -> None:
-        """Row r receives tokens ``cu[r] .. cu[r+1]`` of ``k, v [T, n_heads, d]`` at its end; ``cu [n_rows+1]`` int32."""
+        """Row r receives tokens ``cu[r] .. cu[r+1]`` of ``k, v [T, n_heads, d]`` at its end; ``cu [n_rows+1]`` int32.
+        The cache holds values: no gradient reaches ``k`` or ``v`` through it."""
         ops.cache_append_(self, k, v, cu)
 
     def fork(self, src: torch.Tensor) -> None:
@@ -116,5 +117,5 @@ class PagedCache:
         fp32)``, to be merged with a memory's by ``merge``.  Query head ``h*G + g`` reads KV head h.  ``terms``: cap,
         slopes, and ``prefix [n_rows]`` (the first keys of a row that all its new tokens see); a row is a document of
         its own.  ``max_new``: the largest number of new tokens of a row where the caller knows it (it only shapes the
-        launch)."""
+        launch).  There is no backward: a ``q`` that asks for gradients is refused."""
         return ops.paged_attn_fwd(q, self, cu, sm_scale, terms, max_new)

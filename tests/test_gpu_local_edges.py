@@ -208,3 +208,16 @@ def test_a_row_near_2_to_the_31_tokens():
     assert c.length.tolist() == [P - 1] and c.table[0, :2].tolist() == [0, -1]
     c.drop(i32([1]))
     assert c.length.tolist() == [0] and c.refs.tolist() == [0, 0, 0, 0]
+
+
+def test_no_gradient_is_dropped_in_silence():
+    c = PagedCache(1, 2, 16, 1, 64)
+    k = torch.randn(3, 1, 64, device="cuda").to(torch.bfloat16)
+    c.append(k, k, i32([0, 3]))
+    q = k[:1].clone().requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        c.attend(q, i32([0, 1]), 0.1)
+    with torch.no_grad():
+        a = c.attend(q, i32([0, 1]), 0.1)
+    b = c.attend(q.detach(), i32([0, 1]), 0.1)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -38,10 +38,37 @@ struct PagedTileArgs {
   int many_slots;
 };
 
-// Where a query row's pieces lie.  Beside a many-kernel the few-kernel's rows are counted within their row of the batch, of which
+// ---- rows by the tokens there are ------------------------------------------------------------------------------------
+// A cache may have many more rows than a call has tokens.  Workgroups and workspace are handed out over slots, of which there are
+// min(R, T) a head (and piece) and one more for every full block of query rows: which rows have tokens is only known on the device.
+// One token for one row of 32 768 keys, 8 KV heads, d = 128, bf16: 50 us in a cache of 1 to 512 rows (387 with a workgroup for every
+// row of 128 or more, whose number leaves each a single piece), fp32 137 (340 to 1109).
+
+// The last row i with first(i) <= s, first ascending: 64 candidates at a time, one load a lane and round.  All lanes call it.
+template <class First>
+__device__ __forceinline__ int last_row(int R, int s, const First& first) {
+  int lo = 0, n = R;  // it is among rows lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave, at = lane_id() * step;
+    const unsigned long long m = __ballot(at < n && first(lo + at) <= s);
+    const int k = m ? 63 - __clzll((long long)m) : 0;
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// The slot of a row with tokens, its first at q0, among min(R, T): no two rows have the same.  With a token for each row and more
+// it is the row itself, and no search is needed.
+__device__ __forceinline__ int few_slot(const PagedArgs& p, int row, int q0) { return p.T >= p.R ? row : min(row, q0); }
+__device__ __forceinline__ int few_row(const PagedArgs& p, int slot) {
+  return p.T >= p.R ? slot : last_row(p.R, slot, [&](int i) { return min(i, max(p.cu[i], 0)); });
+}
+
+// Where a query row's pieces lie.  Beside a many-kernel the few-kernel's rows are counted within their row's slot, of which
 // each has kFewRows at most: by token there would be units for all the others' too, gigabytes where a long prompt comes along.
-__device__ __forceinline__ int64_t few_index(const PagedTileArgs& a, int row, int r, int hk, int t, int hq) {
-  const int64_t u = a.few_rows == kFewRows ? (int64_t(row) * kFewRows + r) * a.p.H + hk : int64_t(t) * a.p.H * a.p.G + hq;
+__device__ __forceinline__ int64_t few_index(const PagedTileArgs& a, int slot, int r, int hk, int t, int hq) {
+  const int64_t u = a.few_rows == kFewRows ? (int64_t(slot) * kFewRows + r) * a.p.H + hk : int64_t(t) * a.p.H * a.p.G + hq;
   return u * a.few_pieces;
 }
 __device__ __forceinline__ int64_t many_index(const PagedTileArgs& a, int t, int hq) {
@@ -111,19 +138,14 @@ __device__ __forceinline__ void piece_keys(int keys, int tile, int i, int n, int
 }
 
 // The row and its first query row that slot s of ROWS query rows stands for: row i owns slots first(i) .. first(i + 1) - 1,
-// first(i) = cu[i] G / ROWS + i: at least as many as it has blocks.
+// first(i) = cu[i] G / ROWS + min(i, cu[i]): at least as many as it has blocks, and none before the first token.
 template <int ROWS>
 __device__ __forceinline__ void paged_slot(const PagedArgs& p, int s, int& row, int& r0) {
-  auto first = [&](int i) { return int(int64_t(max(p.cu[i], 0)) * p.G / ROWS) + i; };
-  int lo = 0, hi = p.R - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first(mid) <= s)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  row = __builtin_amdgcn_readfirstlane(lo);
+  auto first = [&](int i) {
+    const int c = max(p.cu[i], 0);
+    return int(int64_t(c) * p.G / ROWS) + min(i, c);
+  };
+  row = last_row(p.R, s, first);
   r0 = (s - first(row)) * ROWS;
 }
 
@@ -157,14 +179,14 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
   float* lds_o = reinterpret_cast<float*>(lds_all + 128);             // [4][16][LD]
   float2* lds_ml = reinterpret_cast<float2*>(lds_o + 4 * 16 * LD);     // [4][16]
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, c = l & 15, g = l >> 4;
-  const int units = a.p.R * a.p.H * a.few_pieces;
+  const int units = min(a.p.R, a.p.T) * a.p.H * a.few_pieces;
   if (int(blockIdx.x) >= units) return paged_nobody<E>(a, int(blockIdx.x) - units, int(gridDim.x) - units);
   // pieces of a row side by side, then its heads: the pages of a row are read at one time
   const int piece = int(blockIdx.x) % a.few_pieces, rh = int(blockIdx.x) / a.few_pieces;
-  const int hk = rh % a.p.H, row = rh / a.p.H;
+  const int hk = rh % a.p.H, slot = rh / a.p.H, row = few_row(a.p, slot);
   const PagedRow pr = paged_row(a.p, row);
   const int n = pr.q1 - pr.q0, n_rows = n * a.p.G;
-  if (n <= 0 || n_rows > a.few_rows) return;
+  if (n <= 0 || n_rows > a.few_rows || slot != few_slot(a.p, row, pr.q0)) return;
   const int prefix = a.p.prefix ? a.p.prefix[row] : 0;
   const int64_t head = int64_t(hk) * a.p.page * D;
   const bf16_t* K = (const bf16_t*)a.p.k + head;
@@ -318,7 +340,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
     if (again) {
       for (int r = r0 + w; r < min(r0 + 16 * NQ, n_rows); r += 4)
         paged_row_again<E>(a, pr, pr.q0 + r / a.p.G, hk * a.p.G + r % a.p.G, j0, j1,
-                           few_index(a, row, r, hk, pr.q0 + r / a.p.G, hk * a.p.G + r % a.p.G) + piece, a.few_pieces);
+                           few_index(a, slot, r, hk, pr.q0 + r / a.p.G, hk * a.p.G + r % a.p.G) + piece, a.few_pieces);
       __syncthreads();
       continue;
     }
@@ -356,7 +378,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
         const int tok = r / a.p.G, hq = hk * a.p.G + (r - tok * a.p.G), t = pr.q0 + tok;
         const bool none = lt == 0.f;
         const float inv = a.few_pieces > 1 ? 1.f : none ? 0.f : 1.f / lt;
-        const int64_t at = a.few_pieces > 1 ? few_index(a, row, r, hk, t, hq) + piece : 0;
+        const int64_t at = a.few_pieces > 1 ? few_index(a, slot, r, hk, t, hq) + piece : 0;
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) {
           const int d0 = 64 * u + 4 * part;
@@ -495,11 +517,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedTileArgs a) {
   int t, hk, r;
   if constexpr (FEW) {
     const int64_t u = unit / a.p.H;
+    const int64_t slot = u / kFewRows;  // (the same in a wave: its four units are neighbours among 32 H)
     hk = int(unit - u * a.p.H), r = int(u % kFewRows);
-    if (u / kFewRows >= a.p.R) return;
-    pr = paged_row(a.p, int(u / kFewRows));
+    if (slot >= min(a.p.R, a.p.T)) return;
+    pr = paged_row(a.p, few_row(a.p, int(slot)));
     const int n_rows = (pr.q1 - pr.q0) * a.p.G;
-    if (n_rows > a.few_rows || r >= n_rows) return;
+    if (n_rows > a.few_rows || r >= n_rows || slot != few_slot(a.p, pr.row, pr.q0)) return;
     t = pr.q0 + r / a.p.G;
   } else {
     const int HG = a.p.H * a.p.G;
@@ -513,7 +536,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedTileArgs a) {
   const bool few = FEW || (pr.q1 - pr.q0) * a.p.G <= a.few_rows;
   const int pieces = few ? a.few_pieces : a.many_pieces, hq = hk * a.p.G + r % a.p.G;
   if (pieces == 1) return;
-  const int64_t at = few ? few_index(a, pr.row, r, hk, t, hq) : many_index(a, t, hq);
+  const int64_t at = few ? few_index(a, few_slot(a.p, pr.row, pr.q0), r, hk, t, hq) : many_index(a, t, hq);
   tile_join<F16, D>(a.part_o + at * D, a.part_ml + at, pieces, (bf16_t*)a.p.out + t * a.p.o_token + hq * a.p.o_head,
                     a.p.lse + t * a.p.l_token + hq * a.p.l_head);
 }
@@ -536,13 +559,14 @@ inline PagedPlan paged_plan(int rows, int T, int max_new, int H, int G, int d, i
   y.few = !(known && rows == 1 && max_new == T && int64_t(T) * G > kFewRows);
   y.many = !(known && int64_t(max_new) * G <= kFewRows) && int64_t(T) * G > kFewRows;
   y.few_rows = !y.many ? 0x7fffffff : y.few ? kFewRows : 0;
-  y.slots = int(int64_t(T) * G / kTQ) + rows;
+  const int filled = std::min(rows, T);  // rows that may have tokens
+  y.slots = int(int64_t(T) * G / kTQ) + filled;
   const int64_t most = std::min<int64_t>(ceil_div(keys, 512), 64);
   auto pieces = [&](int64_t groups) { return int(std::max<int64_t>(1, std::min(most, ceil_div(1024, groups)))); };
   // (where every row is the few-kernel's, by T as well: a max_new that is too small is no wrong answer, nor a large workspace)
-  y.few_pieces = y.few ? pieces(std::max<int64_t>(rows, y.many ? 0 : int64_t(T) * G / kFewRows) * H) : 1;
+  y.few_pieces = y.few ? pieces(std::max<int64_t>(filled, y.many ? 0 : int64_t(T) * G / kFewRows) * H) : 1;
   y.many_pieces = y.many ? pieces(std::max<int64_t>(1, int64_t(T) * G / kTQ) * H) : 1;
-  y.many_base = y.few_pieces > 1 ? int64_t(y.many ? int64_t(rows) * kFewRows : int64_t(T) * G) * H * y.few_pieces : 0;
+  y.many_base = y.few_pieces > 1 ? int64_t(y.many ? int64_t(filled) * kFewRows : int64_t(T) * G) * H * y.few_pieces : 0;
   const size_t units = size_t(y.many_base) + (y.many_pieces > 1 ? size_t(T) * H * G * y.many_pieces : 0);
   y.part_ml = align_up(units * d * 4, 256);
   y.total = y.part_ml + align_up(units * 8, 256);
@@ -554,7 +578,7 @@ inline PagedPlan paged_plan(int rows, int T, int max_new, int H, int G, int d, i
 inline PagedPlan paged_f32_plan(int rows, int T, int H, int G, int d, int64_t keys) {
   PagedPlan y{};
   y.many = true;
-  y.slots = int(int64_t(T) * G / 32) + rows;
+  y.slots = int(int64_t(T) * G / 32) + std::min(rows, T);
   const int64_t groups = std::max<int64_t>(std::min<int64_t>(rows, T), int64_t(T) * G / 32) * H;
   y.few_pieces = 1;
   y.many_pieces = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(keys, 512), 64), ceil_div(1024, groups))));
@@ -567,7 +591,7 @@ inline PagedPlan paged_f32_plan(int rows, int T, int H, int G, int d, int64_t ke
 template <bool F16, int D, int NQ>
 static int launch_few(const PagedTileArgs& a, int extra, hipStream_t st) {
   FM_ALLOW_LDS((paged_few_kernel<F16, D, NQ>), (few_lds_bytes<D, NQ>()), "fm_paged_attn_fwd(lds)");
-  hipLaunchKernelGGL((paged_few_kernel<F16, D, NQ>), dim3(unsigned(a.p.R * a.p.H * a.few_pieces + extra)), dim3(256),
+  hipLaunchKernelGGL((paged_few_kernel<F16, D, NQ>), dim3(unsigned(std::min(a.p.R, a.p.T) * a.p.H * a.few_pieces + extra)), dim3(256),
                      (few_lds_bytes<D, NQ>()), st, a);
   return launch_status("fm_paged_attn_fwd(few)");
 }
@@ -603,7 +627,7 @@ static int launch_paged(const PagedTileArgs& a, const PagedPlan& y, int max_new,
     const int64_t units = int64_t(a.p.T) * a.p.H * a.p.G;
     hipLaunchKernelGGL((paged_join_kernel<F16, D, false>), dim3(unsigned(ceil_div(units, 16))), dim3(256), 0, st, a);
   } else if (a.few_pieces > 1) {
-    const int64_t units = int64_t(a.p.R) * kFewRows * a.p.H;
+    const int64_t units = int64_t(std::min(a.p.R, a.p.T)) * kFewRows * a.p.H;
     hipLaunchKernelGGL((paged_join_kernel<F16, D, true>), dim3(unsigned(ceil_div(units, 16))), dim3(256), 0, st, a);
   }
   return launch_status("fm_paged_attn_fwd(join)");

@@ -6,7 +6,7 @@ import torch
 from fast_memory_amd import PagedCache, ScoreTerms, ops
 from oracle import local_side as O
 from tests.test_gpu_local_terms import close
-from tests.test_gpu_paged import cu_of, i32
+from tests.test_gpu_paged import attend_case, cu_of, i32
 from tests.util import gen
 
 pytestmark = pytest.mark.gpu
@@ -221,3 +221,29 @@ def test_no_gradient_is_dropped_in_silence():
         a = c.attend(q, i32([0, 1]), 0.1)
     b = c.attend(q.detach(), i32([0, 1]), 0.1)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# ------------------------------------------------------------------ rows without new tokens
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("G,active", [(1, {37: 1}), (4, {69: 1}), (4, {0: 1, 1: 1, 64: 2, 69: 1}), (2, {5: 40, 6: 1, 66: 1}), (8, {3: 3, 12: 20, 68: 1}),
+                                      (1, {i: 1 for i in range(0, 70, 2)}), (2, {10: 70}), (1, {20: 33, 64: 33, 65: 1, 66: 3}), (1, {1: 66, 69: 5})])
+def test_few_rows_with_tokens_among_many(dtype, G, active):
+    """70 rows of which a few have new tokens, long and short ones: fewer tokens than rows, as many, more."""
+    lengths = [(37 * r) % 90 for r in range(70)]
+    for at, r in enumerate(active):
+        lengths[r] = max(active[r], (5200, 33, 700, 64)[at % 4])
+    new = [active.get(r, 0) for r in range(70)]
+    attend_case(37, lengths, new, 2, G, 64, 16, dtype, {}, max_new=max(new))
+    attend_case(38, lengths, new, 1, G, 64, 16, dtype, dict(softcap=20.0), heads_first=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_offsets_that_do_not_fit_stay_inside(dtype):
+    """cu that does not ascend, or leaves the tokens there are: some result, and nothing outside of it is touched."""
+    cache, q, cu, terms, out, lse = attend_case(39, [40] * 9, [0, 0, 3, 0, 0, 0, 1, 0, 0], 1, 2, 64, 16, dtype, {})
+    for bad in ([9, 8, 7, 6, 5, 4, 3, 2, 1, 0], [0, 1 << 30, -5, 4, 1 << 30, 0, 0, 2, 4, 1 << 30], [4] * 10, [-3] * 10, [0] * 9 + [1 << 30]):
+        whole = torch.full((8, 2, 64), 7.0, dtype=q.dtype, device="cuda")
+        whole[2:6] = q
+        o, l = cache.attend(whole[2:6], i32(bad), 0.1)
+        torch.cuda.synchronize()
+        assert o.shape == (4, 2, 64) and (whole[:2] == 7).all() and (whole[6:] == 7).all()

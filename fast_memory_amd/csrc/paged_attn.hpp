@@ -80,21 +80,37 @@ __device__ __forceinline__ int64_t page_offset(const PagedArgs& p, int page, int
   return int64_t(min(max(page, 0), p.n_pages - 1)) * p.H * p.page * d;
 }
 
-// tokens in front of the first row's and behind the last row's: nothing to see
+// Tokens in front of the first row's and behind the last row's: nothing to see.  As many lanes a query row as it has groups of four
+// dimensions (a power of two, a wave at most); `first` of `step` workgroups.
 template <typename E>
 __device__ void paged_nobody(const PagedTileArgs& a, int first, int step) {
-  const int HG = a.p.H * a.p.G, c0 = a.p.cu[0], c1 = max(a.p.cu[a.p.R], 0);
-  for (int t = first; t < a.p.T; t += step) {
-    if (t >= c0 && t < c1) {
-      t += (c1 - 1 - t) / step * step;
-      continue;
+  const PagedArgs& p = a.p;
+  const int HG = p.H * p.G, c0 = min(max(p.cu[0], 0), p.T), c1 = min(max(p.cu[p.R], c0), p.T);
+  const unsigned n = unsigned(c0 + p.T - c1) * unsigned(HG);  // (T H G fits 31 bits)
+  const bool fours = ((p.d | p.o_token | p.o_head) & 3) == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(E)) == 0;
+  int log2l = 0;
+  while (log2l < 6 && (4 << log2l) < p.d) ++log2l;
+  const int lane = int(threadIdx.x) & ((1 << log2l) - 1), rows = 256 >> log2l;
+  for (unsigned i = unsigned(first * rows) + (threadIdx.x >> log2l); i < n; i += unsigned(step * rows)) {
+    int t = int(i / unsigned(HG));
+    const int hq = int(i - unsigned(t) * unsigned(HG));
+    if (t >= c0) t += c1 - c0;
+    E* out = (E*)p.out + t * p.o_token + hq * p.o_head;
+    for (int c = 4 * lane; c < p.d; c += 4 << log2l) {
+      if (fours) {
+        typename std::conditional<sizeof(E) == 4, uint4, uint2>::type zero{};
+        *reinterpret_cast<decltype(zero)*>(out + c) = zero;
+      } else {
+        for (int e = c; e < min(c + 4, p.d); ++e) Elem<E>::store(out + e, 0.f);
+      }
     }
-    for (int u = threadIdx.x; u < HG * a.p.d; u += 256) {
-      const int hq = u / a.p.d, c = u - hq * a.p.d;
-      Elem<E>::store((E*)a.p.out + t * a.p.o_token + hq * a.p.o_head + c, 0.f);
-      if (c == 0) a.p.lse[t * a.p.l_token + hq * a.p.l_head] = -FLT_MAX;
-    }
+    if (lane == 0) p.lse[t * p.l_token + hq * p.l_head] = -FLT_MAX;
   }
+}
+// Workgroups for them, behind the others': one per 64 query rows of the call, 1024 at most.  They leave at once where every token
+// is some row's.  A batch padded to 8192 tokens x 64 heads, d = 128, bf16, of which 4 are real: 62 us (7.8 ms with four workgroups).
+inline int nobody_groups(const PagedArgs& p) {
+  return int(std::min<int64_t>(1024, ceil_div(int64_t(p.T) * p.H * p.G, 64)));
 }
 
 // One query row's result: final where the keys are in one piece, else its piece's.  `o`: 64 lanes, dimensions l + 64 r.
@@ -606,7 +622,7 @@ static int launch_many(const PagedTileArgs& a, int extra, hipStream_t st) {
 
 template <bool F16, int D>
 static int launch_paged(const PagedTileArgs& a, const PagedPlan& y, int max_new, hipStream_t st) {
-  const int extra = 4;  // workgroups for tokens of no row
+  const int extra = nobody_groups(a.p);
   int rc = FM_OK;
   if (y.few) {
     const bool one = max_new > 0 && int64_t(max_new) * a.p.G <= 16;

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void paged_f32_join_kernel(PagedTileArgs a) {
 template <typename T, bool VEC, int NDT>
 static int launch_paged_f32(const PagedTileArgs& a, hipStream_t st) {
   FM_ALLOW_LDS((paged_f32_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_paged_attn_fwd(lds)");
-  hipLaunchKernelGGL((paged_f32_kernel<T, VEC, NDT>), dim3(unsigned(a.p.H * a.many_slots * a.many_pieces + 4)), dim3(256),
+  hipLaunchKernelGGL((paged_f32_kernel<T, VEC, NDT>), dim3(unsigned(a.p.H * a.many_slots * a.many_pieces + nobody_groups(a.p))), dim3(256),
                      f32_lds_bytes<NDT>(1), st, a, f32_score(a.p.sm_scale, a.p.softcap));
   return launch_status("fm_paged_attn_fwd(f32)");
 }

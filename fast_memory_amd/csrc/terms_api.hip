@@ -256,7 +256,7 @@ extern "C" int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head,
   const bool tiles = tiles_take(d, dtype) && page >= 16 && aligned16({q, k_pages, v_pages, out, ws}) && q_token * e % 16 == 0 &&
                      q_head * e % 16 == 0 && out_token * e % 8 == 0 && out_head * e % 8 == 0;
   const PagedPlan y = tiles ? paged_plan(rows, T, max_new, H, G, d, keys) : paged_f32_plan(rows, T, H, G, d, keys);
-  const int64_t groups = int64_t(H) * std::max(int64_t(std::min(rows, T)) * y.few_pieces, int64_t(y.slots) * y.many_pieces) + 4;
+  const int64_t groups = int64_t(H) * std::max(int64_t(std::min(rows, T)) * y.few_pieces, int64_t(y.slots) * y.many_pieces) + 1024;
   FM_REQUIRE(groups <= 0x7fffffffLL, FM_ERR_UNSUPPORTED, "fm_paged_attn_fwd: %lld workgroups", (long long)groups);
   char* w = static_cast<char*>(ws);
   const PagedTileArgs t{a, tile_score(sm_scale, softcap), y.few_rows, y.few_pieces, y.many_pieces, reinterpret_cast<float*>(w),

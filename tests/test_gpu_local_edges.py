@@ -247,3 +247,23 @@ def test_offsets_that_do_not_fit_stay_inside(dtype):
         o, l = cache.attend(whole[2:6], i32(bad), 0.1)
         torch.cuda.synchronize()
         assert o.shape == (4, 2, 64) and (whole[:2] == 7).all() and (whole[6:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("heads_first", [False, True])
+@pytest.mark.parametrize("front,back", [(0, 700), (300, 0), (257, 1000), (0, 0), (1, 1)])
+def test_a_padded_batch(dtype, heads_first, front, back):
+    """Tokens of no row on both sides: empty, whatever lay there, and the rows' results as without them."""
+    cache, q, cu, terms, out, lse = attend_case(40, [40, 50, 0], [3, 40, 0], 2, 3, 64, 16, dtype, {}, heads_first=heads_first)
+    pad = lambda n: torch.full((n, 6, 64), float("nan"), dtype=dtype, device="cuda")
+    more = torch.cat([pad(front), q, pad(back)])
+    if heads_first:
+        more = more.transpose(0, 1).contiguous().transpose(0, 1)
+    torch.empty(1 << 24, device="cuda").fill_(float("nan"))    # (what the results' memory holds beforehand)
+    o, l = cache.attend(more, cu + front, 64 ** -0.5)
+    mine = slice(front, front + 43)
+    # (the number of pieces follows the number of tokens: equal up to the rounding of the result and of the probabilities)
+    assert (o[mine].float() - out.float()).abs().max() <= 4 * torch.finfo(dtype).eps * out.float().abs().max()
+    assert (l[mine] - lse).abs().max() < 1e-5
+    for part in (slice(0, front), slice(front + 43, None)):
+        assert (o[part] == 0).all() and (l[part] == O.EMPTY).all()

@@ -88,30 +88,15 @@ __global__ __launch_bounds__(256, 1) void paged_f32_kernel(PagedTileArgs a, F32S
 // the pieces of a query row, in order: a wave a row
 template <typename T>
 __global__ __launch_bounds__(256) void paged_f32_join_kernel(PagedTileArgs a) {
-  const int HG = a.p.H * a.p.G, l = lane_id();
+  const int HG = a.p.H * a.p.G;
   const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int t = int(unit / HG), hq = int(unit - int64_t(t) * HG);
   if (t >= a.p.T) return;
   const PagedRow pr = paged_row_of_token(a.p, t);
   if (pr.row < 0) return;  // (written where nobody's tokens are)
-  const float2* ml = a.part_ml + many_index(a, t, hq);
-  const float* po = a.part_o + many_index(a, t, hq) * a.p.d;
-  RowState st;
-  st.m = -INFINITY;
-  st.l = 0.f;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) st.acc[r] = 0.f;
-  for (int i = 0; i < a.many_pieces; ++i) st.m = fmaxf(st.m, ml[i].x);
-  const float base = st.m == -INFINITY ? 0.f : st.m;
-  for (int i = 0; i < a.many_pieces; ++i) {
-    const float2 x = ml[i];
-    const float f = __builtin_amdgcn_exp2f(x.x - base);
-    st.l = fmaf(x.y, f, st.l);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (l + 64 * r < a.p.d) st.acc[r] = fmaf(po[int64_t(i) * a.p.d + l + 64 * r], f, st.acc[r]);
-  }
-  row_write(st, a.p.d, (T*)a.p.out + t * a.p.o_token + hq * a.p.o_head, a.p.lse + t * a.p.l_token + hq * a.p.l_head);
+  const int64_t at = many_index(a, t, hq);
+  f32_join_row(a.part_o + at * a.p.d, a.part_ml + at, a.many_pieces, a.p.d, (T*)a.p.out + t * a.p.o_token + hq * a.p.o_head,
+               a.p.lse + t * a.p.l_token + hq * a.p.l_head);
 }
 
 template <typename T, bool VEC, int NDT>

@@ -42,19 +42,33 @@ static bool tiles_take(int d, int dtype) {
 // less than 8 tiles of 64 keys.  Measured, whole and in pieces, bf16: 2 heads x 4096, d = 256: forward 220 and 64 us, backward
 // 606 and 280; 8 heads x 128 over 4096 keys, d = 128: 122 and 28, 193 and 48; 16 x 2048: 66 and 52, 150 and 131; 32 x 1024
 // (256 blocks): 37 and 37, 93 and 88.
-static int sweep_pieces(int H, int G, int S, int L, int d, int dtype) {
-  if (!tiles_take(d, dtype)) return 1;
+static int sweep_pieces(int H, int G, int S, int L) {
   const int64_t blocks = int64_t(H) * G * ceil_div(S, kTQ);
   return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / blocks, ceil_div(L, 512)), 16)));
 }
 
+// The same of the fp32 products' kernels, a workgroup a compute unit: a block of 32 queries over tiles of 32 keys, of which a piece
+// has four at least, one a wave ..
+static int f32_pieces(int H, int G, int S, int L) {
+  const int64_t blocks = int64_t(H) * G * ceil_div(S, 32);
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(256, blocks), ceil_div(L, 32) / 4), 16)));
+}
+// .. and a block of 32 keys over the tiles of 32 queries of its heads.  Measured, forward and backward in fp32, whole, in pieces for
+// 256 workgroups and for 512: 1 x 512 tokens d = 64: 65, 44 and 43 us; 1 x 8 heads x 1024, d = 64: 500, 124, 134; d = 128: 898, 209,
+// 220; d = 256: 1466, 456, 500; 8 heads x 512, d = 128: 105, 98, 132; 8 x 8 heads x 512, d = 64: 295, 209, 213.
+static int f32_splits(int H, int G, int S, int L) {
+  const int64_t blocks = int64_t(H) * ceil_div(L, 32), steps = int64_t(G) * ceil_div(S, 32);
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(256, blocks), steps / 4), 16)));
+}
+
+// The workspace of a forward: masks | partial sums.  `tiles`: of the 16-bit products' kernels.
 struct FwdLayout {
   int pieces;
   size_t part_o, part_ml, total;
 };
-static FwdLayout fwd_layout(int H, int G, int S, int L, int d, int dtype) {
+static FwdLayout fwd_layout(int H, int G, int S, int L, int d, bool tiles) {
   FwdLayout y;
-  y.pieces = sweep_pieces(H, G, S, L, d, dtype);
+  y.pieces = tiles ? sweep_pieces(H, G, S, L) : f32_pieces(H, G, S, L);
   const size_t units = y.pieces > 1 ? size_t(H) * G * S * y.pieces : 0;
   y.part_o = masks_layout(nullptr, S, L).bytes;
   y.part_ml = y.part_o + align_up(units * d * 4, 256);
@@ -63,7 +77,7 @@ static FwdLayout fwd_layout(int H, int G, int S, int L, int d, int dtype) {
 }
 
 static int terms_fwd_run(const FwdArgs& a, void* ws, hipStream_t st) {
-  const FwdLayout y = fwd_layout(a.H, a.G, a.S, a.L, a.d, a.dtype);
+  const FwdLayout y = fwd_layout(a.H, a.G, a.S, a.L, a.d, true);
   char* p = static_cast<char*>(ws);
   FwdTileArgs t{(const bf16_t*)a.q, (const bf16_t*)a.k, (const bf16_t*)a.v, (bf16_t*)a.out, a.lse, a.t, masks_layout(ws, a.S, a.L),
                 a.t.doc_q || a.t.prefix, a.H, a.G, a.S, a.L, a.sm_scale, tile_score(a.sm_scale, a.t.softcap), y.pieces, reinterpret_cast<float*>(p + y.part_o),
@@ -94,27 +108,21 @@ static int terms_check(const char* name, const FwdArgs& a) {
   return FM_OK;
 }
 
-static int terms_fwd_f32(const FwdArgs& f, void* ws, hipStream_t st) {
-  F32Args a{f, nullptr, nullptr, nullptr, nullptr, nullptr, masks_layout(ws, f.S, f.L), f.t.doc_q || f.t.prefix,
-            f32_score(f.sm_scale, f.t.softcap)};
+static int terms_fwd_f32(const FwdArgs& f, char* ws, hipStream_t st) {
+  const FwdLayout y = fwd_layout(f.H, f.G, f.S, f.L, f.d, false);
+  F32Args a{};
+  a.f = f;
+  a.m = masks_layout(ws, f.S, f.L);
+  a.use_masks = f.t.doc_q || f.t.prefix;
+  a.score = f32_score(f.sm_scale, f.t.softcap);
+  a.pieces = y.pieces;
+  a.part_o = reinterpret_cast<float*>(ws + y.part_o);
+  a.part_ml = reinterpret_cast<float2*>(ws + y.part_ml);
   if (a.use_masks) {
     const int rc = make_masks(a.m, f.t, f.S, f.L, st);
     if (rc) return rc;
   }
   return f.dtype == FM_F32 ? terms_f32_fwd<float>(a, st) : f.dtype == FM_BF16 ? terms_f32_fwd<bf16_t>(a, st) : terms_f32_fwd<f16_t>(a, st);
-}
-static int terms_bwd_f32(const BwdArgs& b, char* ws, size_t masks_at, hipStream_t st) {
-  const FwdArgs& f = b.f;
-  float2* rd = reinterpret_cast<float2*>(ws);
-  F32Args a{f, b.dout, rd, b.dq, b.dk, b.dv, masks_layout(ws + masks_at, f.S, f.L), f.t.doc_q || f.t.prefix,
-            f32_score(f.sm_scale, f.t.softcap)};
-  if (a.use_masks) {
-    const int rc = make_masks(a.m, f.t, f.S, f.L, st);
-    if (rc) return rc;
-  }
-  return f.dtype == FM_F32    ? terms_f32_bwd<float>(a, b, rd, st)
-         : f.dtype == FM_BF16 ? terms_f32_bwd<bf16_t>(a, b, rd, st)
-                              : terms_f32_bwd<f16_t>(a, b, rd, st);
 }
 
 // (the tiled kernels read rows of q, k, v in 16-byte pieces, 8 bytes at a time written)
@@ -142,23 +150,46 @@ static int dkv_splits(int H, int G, int S, int L) {
   return int(std::max<int64_t>(1, std::min<int64_t>(std::min(want, steps / 4), 16)));
 }
 
-static BwdLayout bwd_layout(int H, int G, int S, int L, int d, int dtype) {
+static BwdLayout bwd_layout(int H, int G, int S, int L, int d, bool tiles) {
   BwdLayout b;
   b.masks = row_data_bytes(H, G, S);
   b.norms = b.masks + masks_layout(nullptr, S, L).bytes;
   b.n_q_norms = int(ceil_div(int64_t(H) * G * S, kNormRows));
   b.n_k_norms = int(ceil_div(int64_t(H) * L, kNormRows));
   b.part = b.norms + align_up(size_t(2 * b.n_q_norms + b.n_k_norms) * 4, 256);
-  b.splits = (dtype != FM_F32 && (d == 64 || d == 128 || d == 256)) ? dkv_splits(H, G, S, L) : 1;
-  b.dq_pieces = sweep_pieces(H, G, S, L, d, dtype);
+  b.splits = tiles ? dkv_splits(H, G, S, L) : f32_splits(H, G, S, L);
+  b.dq_pieces = tiles ? sweep_pieces(H, G, S, L) : f32_pieces(H, G, S, L);
   b.part_dq = b.part + (b.splits > 1 ? size_t(b.splits) * 2 * H * L * d * 4 : 0);
   b.total = b.part_dq + (b.dq_pieces > 1 ? size_t(b.dq_pieces) * H * G * S * d * 4 : 0);
   return b;
 }
 
+static int terms_bwd_f32(const BwdArgs& b, char* ws, hipStream_t st) {
+  const FwdArgs& f = b.f;
+  const BwdLayout y = bwd_layout(f.H, f.G, f.S, f.L, f.d, false);
+  float2* rd = reinterpret_cast<float2*>(ws);
+  F32Args a{};
+  a.f = f;
+  a.dout = b.dout, a.rd = rd;
+  a.dq = b.dq, a.dk = b.dk, a.dv = b.dv;
+  a.m = masks_layout(ws + y.masks, f.S, f.L);
+  a.use_masks = f.t.doc_q || f.t.prefix;
+  a.score = f32_score(f.sm_scale, f.t.softcap);
+  a.pieces = y.dq_pieces, a.splits = y.splits;
+  a.part_kv = reinterpret_cast<float*>(ws + y.part);
+  a.part_dq = reinterpret_cast<float*>(ws + y.part_dq);
+  if (a.use_masks) {
+    const int rc = make_masks(a.m, f.t, f.S, f.L, st);
+    if (rc) return rc;
+  }
+  return f.dtype == FM_F32    ? terms_f32_bwd<float>(a, b, rd, st)
+         : f.dtype == FM_BF16 ? terms_f32_bwd<bf16_t>(a, b, rd, st)
+                              : terms_f32_bwd<f16_t>(a, b, rd, st);
+}
+
 static int terms_bwd_run(const BwdArgs& b, void* ws, hipStream_t st) {
   const FwdArgs& a = b.f;
-  const BwdLayout y = bwd_layout(a.H, a.G, a.S, a.L, a.d, a.dtype);
+  const BwdLayout y = bwd_layout(a.H, a.G, a.S, a.L, a.d, true);
   char* p = static_cast<char*>(ws);
   float2* rd = reinterpret_cast<float2*>(p);
   float* norms = reinterpret_cast<float*>(p + y.norms);
@@ -180,7 +211,9 @@ static int terms_bwd_run(const BwdArgs& b, void* ws, hipStream_t st) {
 
 extern "C" size_t fm_local_attn_terms_fwd_workspace(int H, int G, int S, int L, int d, int dtype) {
   if (H < 1 || G < 1 || S < 1 || L < 1 || d < 1) return 0;
-  return fm::fwd_layout(H, G, S, L, d, dtype).total;
+  // (rows that are not on 16 bytes go the fp32 products' way)
+  const size_t tiles = fm::tiles_take(d, dtype) ? fm::fwd_layout(H, G, S, L, d, true).total : 0;
+  return std::max(tiles, fm::fwd_layout(H, G, S, L, d, false).total);
 }
 
 extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void* v, void* out, float* lse, float softcap,
@@ -195,12 +228,13 @@ extern "C" int fm_local_attn_terms_fwd(const void* q, const void* k, const void*
   FM_REQUIRE(ws, FM_ERR_ARG, "fm_local_attn_terms_fwd: null pointer");
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_fwd: workspace %zu < %zu", ws_bytes, need);
   if (tiles_take(d, dtype) && aligned16({q, k, v, out, ws})) return terms_fwd_run(a, ws, as_stream(stream));
-  return terms_fwd_f32(a, ws, as_stream(stream));
+  return terms_fwd_f32(a, static_cast<char*>(ws), as_stream(stream));
 }
 
 extern "C" size_t fm_local_attn_terms_bwd_workspace(int H, int G, int S, int L, int d, int dtype) {
   if (H < 1 || G < 1 || S < 1 || L < 1 || d < 1) return 0;
-  return fm::bwd_layout(H, G, S, L, d, dtype).total;
+  const size_t tiles = fm::tiles_take(d, dtype) ? fm::bwd_layout(H, G, S, L, d, true).total : 0;
+  return std::max(tiles, fm::bwd_layout(H, G, S, L, d, false).total);
 }
 
 extern "C" int fm_local_attn_terms_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
@@ -218,7 +252,7 @@ extern "C" int fm_local_attn_terms_bwd(const void* q, const void* k, const void*
   const size_t need = fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dtype);
   FM_REQUIRE(ws_bytes >= need, FM_ERR_WORKSPACE, "fm_local_attn_terms_bwd: workspace %zu < %zu", ws_bytes, need);
   if (tiles_take(d, dtype) && aligned16({q, k, v, out, dout, dq, dk, dv, ws})) return terms_bwd_run(a, ws, as_stream(stream));
-  return terms_bwd_f32(a, static_cast<char*>(ws), bwd_layout(H, G, S, L, d, dtype).masks, as_stream(stream));
+  return terms_bwd_f32(a, static_cast<char*>(ws), as_stream(stream));
 }
 
 extern "C" size_t fm_paged_attn_fwd_workspace(int rows, int T, int max_new, int H, int G, int d, int width, int page, int dtype) {

@@ -6,8 +6,9 @@
 // owns 32 queries (or 32 keys) and its four waves take the tiles of 32 on the other side in turn; their sums meet in LDS
 // at the end, in wave order.  Short rows are spread over four waves this way, which is what bounds them.
 //
-//   operand of 32 rows   lane (row l % 32, half l / 32) holds half of the row's dimensions, [0, Dp / 2) or [Dp / 2, Dp): the
-//                        order of a contraction is free, and a lane then reads 16 consecutive bytes for four products
+//   operand of 32 rows   lane (row l % 32, half l / 32) holds half of the row's dimensions, four of eight: the order of a
+//                        contraction is free, a lane then reads 16 consecutive bytes for four products, and both halves the
+//                        same cache line
 //   scores               as in terms_tile.hpp: lane column = query (key), register r = row 8 (r / 4) + 4 (l / 32) + r % 4
 //   second product       register r of both halves is the operand of one instruction: rows k and k + 4; its partner is
 //                        one element per lane of those two rows, 32 neighbouring dimensions
@@ -58,42 +59,72 @@ __device__ __forceinline__ float4 f32_load4(const T* __restrict__ row, int c, in
   }
 }
 
-// this lane's half of a row, to stay in registers
+// this lane's half of a row (dimensions 8 j + 4 hb ..), to stay in registers
 template <typename T, bool VEC, int NDT>
 __device__ __forceinline__ void f32_resident(float (&x)[16 * NDT], const T* row, bool ok, int d, int hb) {
 #pragma unroll
   for (int j = 0; j < 4 * NDT; ++j) {
-    const float4 v = ok ? f32_load4<T, VEC>(row, 16 * NDT * hb + 4 * j, d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 v = ok ? f32_load4<T, VEC>(row, 8 * j + 4 * hb, d) : make_float4(0.f, 0.f, 0.f, 0.f);
     x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
   }
 }
 
+// The resident operand of a product, 4 NDT quads of a lane: registers, or LDS where there are two operands of 32 NDT = 256 dimensions
+// beside a sum of as many (registers for all spilled 455: 8 heads x 1024 d = 256, forward and backward, 2.86 ms against 2.56).  A row in
+// LDS has four words more than dimensions, so that eight neighbouring rows lie on different banks.
+template <int NDT>
+struct F32Regs {
+  const float (&x)[16 * NDT];
+  __device__ __forceinline__ float4 quad(int j) const { return make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]); }
+};
+template <int NDT>
+struct F32Lds {
+  static constexpr int kRow = 32 * NDT + 4;
+  const float* at;
+  __device__ __forceinline__ F32Lds(const float* lds, int col, int hb) : at(lds + col * kRow + 4 * hb) {}
+  __device__ __forceinline__ float4 quad(int j) const { return *reinterpret_cast<const float4*>(at + 8 * j); }
+  // 32 rows from `rows`, of which the first n are there; all threads of the workgroup
+  template <typename T, bool VEC>
+  __device__ static __forceinline__ void fill(float* lds, const T* rows, int n, int d) {
+    for (int i = threadIdx.x; i < 32 * 8 * NDT; i += 256) {
+      const int r = i / (8 * NDT), c = 4 * (i % (8 * NDT));
+      *reinterpret_cast<float4*>(lds + r * kRow + c) = r < n ? f32_load4<T, VEC>(rows + int64_t(r) * d, c, d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+};
+
 // products of 32 streamed rows (this lane's is `row`) with the resident ones.  Sixteen elements are in flight while the
 // products of the sixteen before them run (1024 cycles); the barriers keep the compiler from loading everything at once.
-template <typename T, bool VEC, int NDT>
-__device__ __forceinline__ f32_acc f32_products(const T* row, const float (&x)[16 * NDT], int d, int hb) {
+template <typename T, bool VEC, int NDT, class Resident>
+__device__ __forceinline__ f32_acc f32_products_of(const T* row, const Resident& x, int d, int hb) {
   f32_acc s = f32_zero();
-  float4 v[2][4];
+  float4 v[2][4], u[2][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[0][i] = f32_load4<T, VEC>(row, 16 * NDT * hb + 4 * i, d);
+  for (int i = 0; i < 4; ++i) v[0][i] = f32_load4<T, VEC>(row, 8 * i + 4 * hb, d), u[0][i] = x.quad(i);
 #pragma unroll
   for (int g = 0; g < NDT; ++g) {
     if (g + 1 < NDT)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[(g + 1) & 1][i] = f32_load4<T, VEC>(row, 16 * NDT * hb + 16 * (g + 1) + 4 * i, d);
+      for (int i = 0; i < 4; ++i) {
+        v[(g + 1) & 1][i] = f32_load4<T, VEC>(row, 32 * (g + 1) + 8 * i + 4 * hb, d);
+        u[(g + 1) & 1][i] = x.quad(4 * (g + 1) + i);
+      }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 u = v[g & 1][i];
-      const int j = 16 * g + 4 * i;
-      s = mfma_f32(u.x, x[j], s);
-      s = mfma_f32(u.y, x[j + 1], s);
-      s = mfma_f32(u.z, x[j + 2], s);
-      s = mfma_f32(u.w, x[j + 3], s);
+      const float4 a = v[g & 1][i], b = u[g & 1][i];
+      s = mfma_f32(a.x, b.x, s);
+      s = mfma_f32(a.y, b.y, s);
+      s = mfma_f32(a.z, b.z, s);
+      s = mfma_f32(a.w, b.w, s);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
   return s;
+}
+template <typename T, bool VEC, int NDT>
+__device__ __forceinline__ f32_acc f32_products(const T* row, const float (&x)[16 * NDT], int d, int hb) {
+  return f32_products_of<T, VEC, NDT>(row, F32Regs<NDT>{x}, d, hb);
 }
 
 // acc += sum over the 32 rows of a block of row^T w, w = 16 registers.  offset_of(k): of row k from base, in elements
@@ -167,6 +198,13 @@ struct F32Args {
   Masks m;
   int use_masks;
   F32Score score;
+  // where the blocks are too few for the card: pieces of a block's keys (forward, dq) and of its queries (dk dv), each of which
+  // leaves its sums, and a launch that joins them in order
+  int pieces, splits;
+  float* part_o;     // [H G S][pieces][d], forward
+  float2* part_ml;   // [H G S][pieces] {m, l}, m in base 2
+  float* part_kv;    // [splits][2][H][L][d]
+  float* part_dq;    // [pieces][H G][S][d]
 };
 
 // {fewest, most keys} and {smallest, largest document} of 32 queries
@@ -310,7 +348,8 @@ __global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
   const int heads = f.H * f.G, bx = int(blockIdx.x) % heads;
   const int hk = bx % f.H, hq = hk * f.G + bx / f.H;
-  const int i0 = ((f.S + 31) / 32 - 1 - int(blockIdx.x) / heads) * 32, iq = i0 + col;
+  const int rest = int(blockIdx.x) / heads, piece = rest % a.pieces;
+  const int i0 = ((f.S + 31) / 32 - 1 - rest / a.pieces) * 32, iq = i0 + col;
   if (tid == 0) *flag = 0;
   __syncthreads();
   const bool ok = iq < f.S;
@@ -325,8 +364,10 @@ __global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
   f32_acc O[NDT];
   float m, sum;
   bool dirty = false;
-  f32_forward<T, VEC, NDT, true>(qf, iq + (f.L - f.S), qi.x, slope2, qm.x, K, V, [&](int j) { return int64_t(j) * d; }, f.L, w, 4,
-                           (qm.y + 31) / 32, d, a.score, docs, O, m, sum, dirty);
+  int t0 = 0, t1 = (qm.y + 31) / 32;
+  tile_piece(t0, t1, piece, a.pieces);
+  f32_forward<T, VEC, NDT, true>(qf, iq + (f.L - f.S), qi.x, slope2, qm.x, K, V, [&](int j) { return int64_t(j) * d; }, f.L, t0 + w, 4,
+                           t1, d, a.score, docs, O, m, sum, dirty);
   if (dirty) *flag = 1;
   sum += __shfl_xor(sum, 32);
   f32_put<NDT>(lds, O, w, col, hb);
@@ -338,9 +379,17 @@ __global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
       const int64_t r = int64_t(hq) * f.S + i;
       const QueryView qv = query_view(f.t, i, f.S, f.L, hq);
       const RowState rs = f.t.softcap > 0.f
-                              ? row_forward<T, true>((const T*)f.q + r * d, KR, VR, qv, f.t.doc_k, 0, f.L, Score<true>(f.sm_scale, f.t.softcap))
-                              : row_forward<T, false>((const T*)f.q + r * d, KR, VR, qv, f.t.doc_k, 0, f.L, Score<false>(f.sm_scale, 0.f));
-      row_write(rs, d, (T*)f.out + r * d, f.lse + r);
+                              ? row_forward<T, true>((const T*)f.q + r * d, KR, VR, qv, f.t.doc_k, 32 * t0, 32 * t1, Score<true>(f.sm_scale, f.t.softcap))
+                              : row_forward<T, false>((const T*)f.q + r * d, KR, VR, qv, f.t.doc_k, 32 * t0, 32 * t1, Score<false>(f.sm_scale, 0.f));
+      if (a.pieces == 1) {
+        row_write(rs, d, (T*)f.out + r * d, f.lse + r);
+        continue;
+      }
+      const int64_t at = r * a.pieces + piece;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (l + 64 * u < d) a.part_o[at * d + l + 64 * u] = rs.acc[u];
+      if (l == 0) a.part_ml[at] = make_float2(rs.m, rs.l);
     }
     return;
   }
@@ -349,12 +398,48 @@ __global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
     float g[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) g[k] = f32_weight(ml, i, k, st.x);
+    const int64_t r = int64_t(hq) * f.S + i0 + i;
+    if (a.pieces > 1) {
+      const int64_t at = r * a.pieces + piece;
+      for (int c = l; c < d; c += 64) a.part_o[at * d + c] = f32_get<NDT>(lds, i, c, g);
+      if (l == 0) a.part_ml[at] = st;
+      continue;
+    }
     const bool none = st.y == 0.f;
     const float inv = none ? 0.f : 1.f / st.y;
-    const int64_t r = int64_t(hq) * f.S + i0 + i;
     for (int c = l; c < d; c += 64) Elem<T>::store((T*)f.out + r * d + c, f32_get<NDT>(lds, i, c, g) * inv);
     if (l == 0) f.lse[r] = none ? -FLT_MAX : (st.x + __builtin_amdgcn_logf(st.y)) * kLn2;
   }
+}
+
+// the pieces of a query row, in order: a wave a row
+template <typename T>
+__device__ __forceinline__ void f32_join_row(const float* __restrict__ po, const float2* __restrict__ ml, int pieces, int d, T* __restrict__ out,
+                                             float* __restrict__ lse) {
+  const int l = lane_id();
+  RowState st;
+  st.m = -INFINITY;
+  st.l = 0.f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) st.acc[r] = 0.f;
+  for (int i = 0; i < pieces; ++i) st.m = fmaxf(st.m, ml[i].x);
+  const float base = st.m == -INFINITY ? 0.f : st.m;
+  for (int i = 0; i < pieces; ++i) {
+    const float2 x = ml[i];
+    const float f = __builtin_amdgcn_exp2f(x.x - base);
+    st.l = fmaf(x.y, f, st.l);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (l + 64 * r < d) st.acc[r] = fmaf(po[int64_t(i) * d + l + 64 * r], f, st.acc[r]);
+  }
+  row_write(st, d, out, lse);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void terms_f32_join_kernel(F32Args a) {
+  const FwdArgs& f = a.f;
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= int64_t(f.H) * f.G * f.S) return;
+  f32_join_row(a.part_o + row * a.pieces * f.d, a.part_ml + row * a.pieces, a.pieces, f.d, (T*)f.out + row * f.d, f.lse + row);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
@@ -379,7 +464,8 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
   const int heads = f.H * f.G, bx = block % heads;
   const int hk = bx % f.H, hq = hk * f.G + bx / f.H;
-  const int i0 = ((f.S + 31) / 32 - 1 - block / heads) * 32, iq = i0 + col;
+  const int rest = block / heads, piece = rest % a.pieces;
+  const int i0 = ((f.S + 31) / 32 - 1 - rest / a.pieces) * 32, iq = i0 + col;
   if (tid == 0) *flag = 0;
   __syncthreads();
   const bool ok = iq < f.S;
@@ -387,9 +473,16 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
   const int4 qm = f32_query_meta(a, i0);
   const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
   const int64_t row = int64_t(hq) * f.S + (ok ? iq : 0);
-  float qf[16 * NDT], df[16 * NDT];
-  f32_resident<T, VEC, NDT>(qf, (const T*)f.q + row * d, ok, d, hb);
-  f32_resident<T, VEC, NDT>(df, (const T*)a.dout + row * d, ok, d, hb);
+  constexpr bool kLds = NDT == 8;  // both in LDS, where the waves' sums go at the end
+  float qf[kLds ? 1 : 16 * NDT], df[kLds ? 1 : 16 * NDT];
+  if constexpr (kLds) {
+    F32Lds<NDT>::template fill<T, VEC>(lds + 32 * F32Lds<NDT>::kRow, (const T*)f.q + (int64_t(hq) * f.S + i0) * d, f.S - i0, d);
+    F32Lds<NDT>::template fill<T, VEC>(lds, (const T*)a.dout + (int64_t(hq) * f.S + i0) * d, f.S - i0, d);
+    __syncthreads();
+  } else {
+    f32_resident<T, VEC, NDT>(qf, (const T*)f.q + row * d, ok, d, hb);
+    f32_resident<T, VEC, NDT>(df, (const T*)a.dout + row * d, ok, d, hb);
+  }
   const float2 rd = ok ? a.rd[row] : make_float2(0.f, 0.f);
   const T* K = (const T*)f.k + int64_t(hk) * f.L * d;
   const T* V = (const T*)f.v + int64_t(hk) * f.L * d;
@@ -399,13 +492,23 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) O[dt] = f32_zero();
   bool dirty = false;
-  for (int t = w; t < (qm.y + 31) / 32; t += 4) {
+  int t0 = 0, t1 = (qm.y + 31) / 32;
+  tile_piece(t0, t1, piece, a.pieces);
+  float* part = a.pieces > 1 ? a.part_dq + (int64_t(piece) * heads + hq) * f.S * d : nullptr;
+  for (int t = t0 + w; t < t1; t += 4) {
     const int kp0 = 32 * t;
     bool masked = kp0 + 32 > qm.x;
     if (!docs.meets(t, masked)) continue;
     const int64_t at = int64_t(min(kp0 + col, f.L - 1)) * d;
-    const f32_acc s = f32_products<T, VEC, NDT>(K + at, qf, d, hb);
-    const f32_acc p = f32_products<T, VEC, NDT>(V + at, df, d, hb);
+    f32_acc s, p;
+    if constexpr (kLds)
+      s = f32_products_of<T, VEC, NDT>(K + at, F32Lds<NDT>(lds + 32 * F32Lds<NDT>::kRow, col, hb), d, hb);
+    else
+      s = f32_products<T, VEC, NDT>(K + at, qf, d, hb);
+    if constexpr (kLds)
+      p = f32_products_of<T, VEC, NDT>(V + at, F32Lds<NDT>(lds, col, hb), d, hb);
+    else
+      p = f32_products<T, VEC, NDT>(V + at, df, d, hb);
     float g[16], slack[16];
     f32_scores<true>(g, slack, s, a.score, slope2, pos - kp0 - 4 * hb, -1);
 #pragma unroll
@@ -419,6 +522,7 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
     f32_accumulate<T, NDT>(O, g, K + int64_t(kp0) * d, [&](int k) { return unsigned(min(k, last) * d); }, d, hb, col, masked, dirty);
   }
   if (dirty) *flag = 1;
+  if constexpr (kLds) __syncthreads();
   f32_put<NDT>(lds, O, w, col, hb);
   __syncthreads();
   if (*flag) {
@@ -427,18 +531,28 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
       const int64_t r = int64_t(hq) * f.S + i;
       const QueryView qv = query_view(f.t, i, f.S, f.L, hq);
       const T *q = (const T*)f.q + r * d, *o = (const T*)a.dout + r * d;
-      T* to = (T*)a.dq + r * d;
-      if (f.t.softcap > 0.f)
-        row_dq<T, true>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, 0, f.L, f.sm_scale, Score<true>(f.sm_scale, f.t.softcap), to);
+      auto row = [&](auto* to) {
+        if (f.t.softcap > 0.f)
+          row_dq<T, true>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, 32 * t0, 32 * t1, f.sm_scale, Score<true>(f.sm_scale, f.t.softcap), to);
+        else
+          row_dq<T, false>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, 32 * t0, 32 * t1, f.sm_scale, Score<false>(f.sm_scale, 0.f), to);
+      };
+      if (part)
+        row(part + int64_t(i) * d);
       else
-        row_dq<T, false>(q, o, a.rd[r], KR, VR, qv, f.t.doc_k, 0, f.L, f.sm_scale, Score<false>(f.sm_scale, 0.f), to);
+        row((T*)a.dq + r * d);
     }
     return;
   }
   const float one[4] = {1.f, 1.f, 1.f, 1.f};
   for (int i = w; i < 32 && i0 + i < f.S; i += 4)
-    for (int c = l; c < d; c += 64)
-      Elem<T>::store((T*)a.dq + (int64_t(hq) * f.S + i0 + i) * d + c, f32_get<NDT>(lds, i, c, one) * f.sm_scale);
+    for (int c = l; c < d; c += 64) {
+      const float x = f32_get<NDT>(lds, i, c, one) * f.sm_scale;
+      if (part)
+        part[int64_t(i0 + i) * d + c] = x;
+      else
+        Elem<T>::store((T*)a.dq + (int64_t(hq) * f.S + i0 + i) * d + c, x);
+    }
 }
 
 // dk and dv of 32 keys; PART as in terms_bwd.hpp (both sums and both operands of a padded dimension of 256 are 512 registers)
@@ -451,16 +565,23 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
   float* lds = f32_lds + 64;
   const FwdArgs& f = a.f;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
-  const int hk = block % f.H, j0 = block / f.H * 32, j = j0 + col;
+  const int hk = block % f.H, part = block / f.H, split = part % a.splits, j0 = part / a.splits * 32, j = j0 + col;
   if (tid == 0) *flag = 0;
   __syncthreads();
   const bool ok = j < f.L, has_docs = f.t.doc_q != nullptr;
   const int doc = has_docs ? a.m.dock[j] : 0;
   const int2 km = has_docs ? a.m.kmeta[j0 / 32] : make_int2(0, 0);
   const int64_t row = (int64_t(hk) * f.L + (ok ? j : 0)) * d;
-  float kf[16 * NDT], vf[kDk ? 16 * NDT : 1];
-  f32_resident<T, VEC, NDT>(kf, (const T*)f.k + row, ok, d, hb);
-  if constexpr (kDk) f32_resident<T, VEC, NDT>(vf, (const T*)f.v + row, ok, d, hb);
+  constexpr bool kLds = kDk && NDT == 8;  // keys and values in LDS, as q and dout above
+  float kf[kLds ? 1 : 16 * NDT], vf[kDk && !kLds ? 16 * NDT : 1];
+  if constexpr (!kLds) f32_resident<T, VEC, NDT>(kf, (const T*)f.k + row, ok, d, hb);
+  if constexpr (kLds) {
+    F32Lds<NDT>::template fill<T, VEC>(lds + 32 * F32Lds<NDT>::kRow, (const T*)f.k + (int64_t(hk) * f.L + j0) * d, f.L - j0, d);
+    F32Lds<NDT>::template fill<T, VEC>(lds, (const T*)f.v + (int64_t(hk) * f.L + j0) * d, f.L - j0, d);
+    __syncthreads();
+  } else if constexpr (kDk) {
+    f32_resident<T, VEC, NDT>(vf, (const T*)f.v + row, ok, d, hb);
+  }
   f32_acc dK[kDk ? NDT : 1], dV[kDv ? NDT : 1];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) {
@@ -468,23 +589,23 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
     if constexpr (kDv) dV[dt] = f32_zero();
   }
   bool dirty = false;
-  const int nqt = (f.S + 31) / 32;
-  int step = w;  // of the (head, tile of queries) pairs, every fourth is this wave's
-  for (int g = 0; g < f.G; ++g) {
-    const int hq = hk * f.G + g;
+  // the (head, tile of queries) pairs from the last tile down to the first that can see the keys; of this workgroup's, every
+  // fourth is this wave's
+  const int nqt = (f.S + 31) / 32, qt0 = (f.t.causal && !a.use_masks) ? min(max(0, j0 - (f.L - f.S)) / 32, nqt) : 0, n = nqt - qt0;
+  const int64_t steps = int64_t(f.G) * n;
+  const int s0 = int(steps * split / a.splits), s1 = int(steps * (split + 1) / a.splits);
+  // (a loop over heads and one over tiles: as a single one over pairs it takes 100 registers more)
+  int g = n > 0 ? s0 / n : 0, step = s0 - g * n + w;
+  for (; g * n < s1; ++g) {
+    const int hq = hk * f.G + g, end = min(n, s1 - g * n);
     const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
     const T* Q = (const T*)f.q + int64_t(hq) * f.S * d;
     const T* DO = (const T*)a.dout + int64_t(hq) * f.S * d;
     const float2* RD = a.rd + int64_t(hq) * f.S;
-    for (; step < nqt; step += 4) {
+    for (; step < end; step += 4) {
       const int i0 = (nqt - 1 - step) * 32;
       const int4 qm = f32_query_meta(a, i0);
-      if (qm.y <= j0) {
-        if (!a.use_masks && f.t.causal) {  // (the tiles behind see still less)
-          step += (nqt - 1 - step) / 4 * 4;
-        }
-        continue;
-      }
+      if (qm.y <= j0) continue;
       bool masked = i0 + 32 > f.S || j0 + 32 > qm.x;
       if (has_docs) {
         if (km.y < 0 || km.y < qm.z || km.x > qm.w) continue;
@@ -493,7 +614,11 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
       masked = wave_any(masked);
       const int i = min(i0 + col, f.S - 1);
       const float2 mine = RD[i];
-      const f32_acc s = f32_products<T, VEC, NDT>(Q + int64_t(i) * d, kf, d, hb);
+      f32_acc s;
+      if constexpr (kLds)
+        s = f32_products_of<T, VEC, NDT>(Q + int64_t(i) * d, F32Lds<NDT>(lds + 32 * F32Lds<NDT>::kRow, col, hb), d, hb);
+      else
+        s = f32_products<T, VEC, NDT>(Q + int64_t(i) * d, kf, d, hb);
       float x[16], y[16];  // p; slack, then g
       f32_scores<true>(x, y, s, a.score, slope2, i0 + 4 * hb + (f.L - f.S) - j, 1);
       unsigned seen = 0xffff;
@@ -515,7 +640,11 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
       auto offset = [&](int k) { return unsigned(min(k, last) * d); };
       if constexpr (kDv) f32_accumulate<T, NDT>(dV, x, DO + int64_t(i0) * d, offset, d, hb, col, masked, dirty);
       if constexpr (kDk) {
-        const f32_acc p = f32_products<T, VEC, NDT>(DO + int64_t(i) * d, vf, d, hb);
+        f32_acc p;
+        if constexpr (kLds)
+          p = f32_products_of<T, VEC, NDT>(DO + int64_t(i) * d, F32Lds<NDT>(lds, col, hb), d, hb);
+        else
+          p = f32_products<T, VEC, NDT>(DO + int64_t(i) * d, vf, d, hb);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float e = x[r] * y[r] * (p[r] - __shfl(mine.y, f32_row(r) + 4 * hb));
@@ -524,51 +653,75 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
         f32_accumulate<T, NDT>(dK, y, Q + int64_t(i0) * d, offset, d, hb, col, masked, dirty);
       }
     }
-    step -= nqt;
+    step -= n;
   }
   if (dirty) *flag = 1;
+  if constexpr (kLds) __syncthreads();
   if constexpr (kDk) f32_put<NDT>(lds, dK, w, col, hb);
   __syncthreads();
   const int last = min(32, f.L - j0);
   const float one[4] = {1.f, 1.f, 1.f, 1.f};
+  // element c of key jj's gradients, x of dk (times sm_scale here) and of dv
+  const int64_t plane = int64_t(f.H) * f.L * d;
+  auto put = [&](bool dv, int jj, int c, float x) {
+    const int64_t at = (int64_t(hk) * f.L + jj) * d + c;
+    if (!dv) x *= f.sm_scale;
+    if (a.splits > 1)
+      a.part_kv[(2 * split + dv) * plane + at] = x;
+    else
+      Elem<T>::store((T*)(dv ? a.dv : a.dk) + at, x);
+  };
   if (*flag) {
     for (int jj = j0 + w; jj < j0 + last; jj += 4) {
       const int64_t at = (int64_t(hk) * f.L + jj) * d;
+      const T *k = (const T*)f.k + at, *v = (const T*)f.v + at;
       KeyGrads kg;
       key_grads_zero(kg);
-      for (int g = 0; g < f.G; ++g)
-        for (int ib = 0; ib < f.S; ib += kWave) {
-          const T *k = (const T*)f.k + at, *v = (const T*)f.v + at;
-          if (f.t.softcap > 0.f)
-            row_dkv_chunk<T, true>(k, v, jj, hk * f.G + g, ib, min(f.S, ib + kWave), f.S, f.L, d, (const T*)f.q, (const T*)a.dout, a.rd,
-                                   f.t, Score<true>(f.sm_scale, f.t.softcap), kg);
-          else
-            row_dkv_chunk<T, false>(k, v, jj, hk * f.G + g, ib, min(f.S, ib + kWave), f.S, f.L, d, (const T*)f.q, (const T*)a.dout, a.rd,
-                                    f.t, Score<false>(f.sm_scale, 0.f), kg);
-        }
+      for (int step = s0; step < s1; ++step) {
+        const int g = step / n, ib = (nqt - 1 - (step - g * n)) * 32;
+        if (f.t.softcap > 0.f)
+          row_dkv_chunk<T, true>(k, v, jj, hk * f.G + g, ib, min(f.S, ib + 32), f.S, f.L, d, (const T*)f.q, (const T*)a.dout, a.rd,
+                                 f.t, Score<true>(f.sm_scale, f.t.softcap), kg);
+        else
+          row_dkv_chunk<T, false>(k, v, jj, hk * f.G + g, ib, min(f.S, ib + 32), f.S, f.L, d, (const T*)f.q, (const T*)a.dout, a.rd,
+                                  f.t, Score<false>(f.sm_scale, 0.f), kg);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int c = l + 64 * r;
         if (c >= d) continue;
-        if constexpr (kDk) Elem<T>::store((T*)a.dk + at + c, kg.k[r] * f.sm_scale);
-        if constexpr (kDv) Elem<T>::store((T*)a.dv + at + c, kg.v[r]);
+        if constexpr (kDk) put(false, jj, c, kg.k[r]);
+        if constexpr (kDv) put(true, jj, c, kg.v[r]);
       }
     }
     return;
   }
   if constexpr (kDk) {
     for (int i = w; i < last; i += 4)
-      for (int c = l; c < d; c += 64)
-        Elem<T>::store((T*)a.dk + (int64_t(hk) * f.L + j0 + i) * d + c, f32_get<NDT>(lds, i, c, one) * f.sm_scale);
+      for (int c = l; c < d; c += 64) put(false, j0 + i, c, f32_get<NDT>(lds, i, c, one));
   }
   if constexpr (kDv) {
     if constexpr (kDk) __syncthreads();
     f32_put<NDT>(lds, dV, w, col, hb);
     __syncthreads();
     for (int i = w; i < last; i += 4)
-      for (int c = l; c < d; c += 64)
-        Elem<T>::store((T*)a.dv + (int64_t(hk) * f.L + j0 + i) * d + c, f32_get<NDT>(lds, i, c, one));
+      for (int c = l; c < d; c += 64) put(true, j0 + i, c, f32_get<NDT>(lds, i, c, one));
   }
+}
+
+// The pieces' sums in order, each rounded once: dk and dv from part_kv, then dq from part_dq, where they have any.
+template <typename T>
+__global__ __launch_bounds__(256) void terms_f32_bwd_join_kernel(F32Args a, int64_t plane, int64_t plane_q) {
+  int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t kv = a.splits > 1 ? 2 * plane : 0;
+  const bool is_q = i >= kv;
+  if (is_q) i -= kv;
+  if (is_q && (a.pieces == 1 || i >= plane_q)) return;
+  const float* from = (is_q ? a.part_dq : a.part_kv) + i;
+  const int64_t step = is_q ? plane_q : 2 * plane;
+  float x = *from;
+  for (int k = 1; k < (is_q ? a.pieces : a.splits); ++k) x += from[k * step];
+  Elem<T>::store(is_q ? (T*)a.dq + i : i < plane ? (T*)a.dk + i : (T*)a.dv + (i - plane), x);
 }
 
 template <typename T, bool VEC, int NDT>
@@ -588,7 +741,7 @@ __global__ __launch_bounds__(256, 1) void terms_f32_bwd_kernel(F32Args a, int dk
 template <typename T, bool VEC, int NDT>
 static int launch_f32_fwd(const F32Args& a, hipStream_t st) {
   FM_ALLOW_LDS((terms_f32_fwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_local_attn_terms_fwd(lds)");
-  hipLaunchKernelGGL((terms_f32_fwd_kernel<T, VEC, NDT>), dim3(unsigned(a.f.H * a.f.G * ceil_div(a.f.S, 32))), dim3(256),
+  hipLaunchKernelGGL((terms_f32_fwd_kernel<T, VEC, NDT>), dim3(unsigned(a.f.H * a.f.G * ceil_div(a.f.S, 32) * a.pieces)), dim3(256),
                      f32_lds_bytes<NDT>(1), st, a);
   return launch_status("fm_local_attn_terms_fwd(f32)");
 }
@@ -603,7 +756,7 @@ static int launch_delta(const BwdArgs& a, float2* rd, hipStream_t st) {
 template <typename T, bool VEC, int NDT>
 static int launch_f32_bwd(const F32Args& a, hipStream_t st) {
   FM_ALLOW_LDS((terms_f32_bwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_local_attn_terms_bwd(lds)");
-  const int dkv = int(a.f.H * ceil_div(a.f.L, 32)), dq = int(a.f.H * a.f.G * ceil_div(a.f.S, 32));
+  const int dkv = int(a.f.H * ceil_div(a.f.L, 32) * a.splits), dq = int(a.f.H * a.f.G * ceil_div(a.f.S, 32) * a.pieces);
   hipLaunchKernelGGL((terms_f32_bwd_kernel<T, VEC, NDT>), dim3(unsigned((NDT == 8 ? 2 : 1) * dkv + dq)), dim3(256),
                      f32_lds_bytes<NDT>(1), st, a, dkv);
   return launch_status("fm_local_attn_terms_bwd(f32)");
@@ -625,17 +778,25 @@ template <typename T>
 int terms_f32_fwd(const F32Args& a, hipStream_t st) {
   const bool vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v});
 #define FM_F(V, N) launch_f32_fwd<T, V, N>(a, st)
-  return FM_F32_BY_DIM(a.f.d, vec, FM_F);
+  const int rc = FM_F32_BY_DIM(a.f.d, vec, FM_F);
 #undef FM_F
+  if (rc || a.pieces == 1) return rc;
+  hipLaunchKernelGGL(terms_f32_join_kernel<T>, dim3(unsigned(ceil_div(int64_t(a.f.H) * a.f.G * a.f.S, 4))), dim3(256), 0, st, a);
+  return launch_status("fm_local_attn_terms_fwd(join)");
 }
 template <typename T>
 int terms_f32_bwd(const F32Args& a, const BwdArgs& b, float2* rd, hipStream_t st) {
-  const int rc = launch_delta<T>(b, rd, st);
+  int rc = launch_delta<T>(b, rd, st);
   if (rc) return rc;
   const bool vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v, a.dout});
 #define FM_F(V, N) launch_f32_bwd<T, V, N>(a, st)
-  return FM_F32_BY_DIM(a.f.d, vec, FM_F);
+  rc = FM_F32_BY_DIM(a.f.d, vec, FM_F);
 #undef FM_F
+  if (rc || (a.splits == 1 && a.pieces == 1)) return rc;
+  const int64_t plane = int64_t(a.f.H) * a.f.L * a.f.d, plane_q = int64_t(a.f.H) * a.f.G * a.f.S * a.f.d;
+  const int64_t n = (a.splits > 1 ? 2 * plane : 0) + (a.pieces > 1 ? plane_q : 0);
+  hipLaunchKernelGGL(terms_f32_bwd_join_kernel<T>, dim3(unsigned(ceil_div(n, 256))), dim3(256), 0, st, a, plane, plane_q);
+  return launch_status("fm_local_attn_terms_bwd(join)");
 }
 
 }  // namespace fm

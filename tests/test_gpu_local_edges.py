@@ -5,7 +5,7 @@ import torch
 
 from fast_memory_amd import PagedCache, ScoreTerms, ops
 from oracle import local_side as O
-from tests.test_gpu_local_terms import close
+from tests.test_gpu_local_terms import check, close, inputs, on_gpu, terms_of
 from tests.test_gpu_paged import attend_case, cu_of, i32
 from tests.util import gen
 
@@ -267,3 +267,43 @@ def test_a_padded_batch(dtype, heads_first, front, back):
     assert (l[mine] - lse).abs().max() < 1e-5
     for part in (slice(0, front), slice(front + 43, None)):
         assert (o[part] == 0).all() and (l[part] == O.EMPTY).all()
+
+
+# ------------------------------------------------------------------ fp32 products in pieces
+FP32_PRODUCTS = [(torch.float32, 64), (torch.float32, 128), (torch.float32, 256), (torch.bfloat16, 96), (torch.float16, 80), (torch.float32, 37)]
+
+
+@pytest.mark.parametrize("dtype,d", FP32_PRODUCTS, ids=str)
+@pytest.mark.parametrize("H,G,S,L,cap,slopes,docs,prefix,causal", [
+    (1, 8, 300, 300, 0.0, False, 0, 0, True), (1, 8, 301, 450, 20.0, True, 0, 0, True), (2, 5, 270, 270, 0.0, False, 4, 0, True),
+    (1, 3, 333, 200, 0.0, True, 0, 150, True), (1, 6, 257, 511, 15.0, False, 3, 40, False), (1, 1, 1500, 40, 0.0, False, 0, 0, False),
+    (1, 16, 33, 33, 5.0, True, 2, 9, True), (1, 40, 3, 700, 0.0, False, 0, 0, True)])
+def test_few_blocks_in_pieces(dtype, d, H, G, S, L, cap, slopes, docs, prefix, causal):
+    """Too few blocks of queries, or of keys, for the card: the others' tiles are cut into pieces, across heads as well."""
+    check(121, H, G, S, L, d, dtype, causal, terms_of(14, H, G, S, L, cap, slopes, docs, prefix, pad=7 if docs else 0))
+
+
+@pytest.mark.parametrize("dtype,d", FP32_PRODUCTS, ids=str)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_pieces_of_queries_with_masked_places_that_are_not_finite(dtype, d, bad):
+    H, G, S, L = 1, 7, 290, 150
+    q, k, v, do, dl = inputs(123, H, G, S, L, d, dtype)
+    doc_q, doc_k = torch.zeros(S, dtype=torch.int32), torch.zeros(L, dtype=torch.int32)
+    doc_q[20:40], doc_q[200:230], doc_q[280:] = 1, 2, -1
+    doc_k[40:50], doc_k[149:] = 1, -1
+    t = dict(doc_q=doc_q, doc_k=doc_k, softcap=10.0)
+    scale = d ** -0.5
+    want, tol = O.local(q, k, v, scale, False, dout=do, dlse=dl, **t)
+    for x in (q, do):                                       # document 2 has no keys, document 1's rows are finite
+        x[:, 200:230], x[:, 280:] = bad, bad
+    dl[:, 200:230], dl[:, 280:] = bad, bad
+    for x in (k, v):
+        x[:, 149:] = bad
+    gq, gk, gv, gdo, gdl = (x.cuda() for x in (q, k, v, do, dl))
+    out, lse = ops.local_attn_terms_fwd(gq, gk, gv, scale, False, on_gpu(t))
+    got = ops.local_attn_terms_bwd(gdo, gq, gk, gv, out, lse, scale, False, on_gpu(t), gdl)
+    for n, x in zip(("out", "lse", "dq", "dk", "dv"), (out, lse) + got):
+        close(x, want[n], tol[n], n)
+    again = ops.local_attn_terms_bwd(gdo, gq, gk, gv, out, lse, scale, False, on_gpu(t), gdl)
+    for x, y in zip(got, again):
+        assert torch.equal(x, y)

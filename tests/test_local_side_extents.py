@@ -18,3 +18,17 @@ def test_a_cache_of_many_rows_needs_no_large_workspace(dt, d):
                 # pieces until there are about 1024 workgroups of at most 128 query rows, twice over where ceilings add up, or
                 # one piece; d + 2 words a unit
                 assert 0 < need <= 2 * 2 * (1024 + H) * 128 * (d + 2) * 4, (rows, T, max_new, H, G)
+
+
+@pytest.mark.parametrize("dt", [_lib.FM_BF16, _lib.FM_F32])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_pieces_need_no_large_workspace(dt, d):
+    lib = _lib.load()
+    for H, G in ((1, 1), (1, 8), (8, 8), (64, 1)):
+        for S, L in ((1, 1), (1, 1 << 20), (512, 512), (4096, 4096), (1 << 20, 32)):
+            rows, keys = H * G * S, H * L
+            # pieces: fp32 rows of at most 512 + H G blocks of 128 queries; splits: two of at most 1024 + H blocks of 128 keys
+            small = 40 * (rows + keys) + (1 << 20)             # masks, {lse, D}, norms
+            assert 0 < lib.fm_local_attn_terms_fwd_workspace(H, G, S, L, d, dt) <= small + 2 * (512 + H * G) * 128 * (d + 2) * 4
+            assert 0 < lib.fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dt) <= \
+                small + 2 * (512 + H * G) * 128 * d * 4 + 2 * (1024 + H) * 2 * 128 * d * 4

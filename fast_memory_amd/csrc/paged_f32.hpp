@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256, 1) void paged_f32_kernel(PagedTileArgs a, F32S
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   int* flag = reinterpret_cast<int*>(f32_lds);
   float* lds = f32_lds + 64;
-  float2* ml = reinterpret_cast<float2*>(lds + 4 * 32 * (32 * NDT + 4));
+  float2* ml = reinterpret_cast<float2*>(lds + kMeetFloats<NDT>);
   const PagedArgs& p = a.p;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = p.d;
   const int units = p.H * a.many_slots * a.many_pieces;
@@ -53,11 +53,11 @@ __global__ __launch_bounds__(256, 1) void paged_f32_kernel(PagedTileArgs a, F32S
   f32_acc O[NDT];
   float m, sum;
   bool dirty = false;
-  f32_forward<T, VEC, NDT, false>(qf, pos, lim, slope2, lim_lo, (const T*)p.k + head, (const T*)p.v + head, row_of, pr.len, j0 / 32 + w,
+  f32_forward<T, VEC, NDT, false>(F32Regs<NDT>{qf}, pos, lim, slope2, lim_lo, (const T*)p.k + head, (const T*)p.v + head, row_of, pr.len, j0 / 32 + w,
                                   4, (j1 + 31) / 32, d, score, docs, O, m, sum, dirty);
   if (dirty) *flag = 1;
   sum += __shfl_xor(sum, 32);
-  f32_put<NDT>(lds, O, w, col, hb);
+  f32_put<NDT>(lds, O, 0, w, col, hb);
   if (hb == 0) ml[w * 32 + col] = make_float2(m, sum);
   __syncthreads();
   if (*flag) {
@@ -66,23 +66,30 @@ __global__ __launch_bounds__(256, 1) void paged_f32_kernel(PagedTileArgs a, F32S
                          many_index(a, pr.q0 + rr / p.G, hk * p.G + rr % p.G) + piece, a.many_pieces);
     return;
   }
-  for (int i = w; i < kF32Rows && r0 + i < n_rows; i += 4) {
-    const float2 st = f32_meet(ml, i);
-    float g[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) g[k] = f32_weight(ml, i, k, st.x);
-    const int rt = (r0 + i) / p.G, rq = hk * p.G + (r0 + i - rt * p.G), tt = pr.q0 + rt;
-    if (a.many_pieces > 1) {
-      const int64_t at = many_index(a, tt, rq) + piece;
-      for (int c = l; c < d; c += 64) a.part_o[at * d + c] = f32_get<NDT>(lds, i, c, g);
-      if (l == 0) a.part_ml[at] = st;
-    } else {
-      const bool none = st.y == 0.f;
-      const float inv = none ? 0.f : 1.f / st.y;
-      for (int c = l; c < d; c += 64) Elem<T>::store((T*)p.out + tt * p.o_token + rq * p.o_head + c, f32_get<NDT>(lds, i, c, g) * inv);
-      if (l == 0) p.lse[tt * p.l_token + rq * p.l_head] = none ? -FLT_MAX : (st.x + __builtin_amdgcn_logf(st.y)) * kLn2;
+  const int rows = min(kF32Rows, n_rows - r0);
+  auto place = [&](int i, int& tt, int& rq) {  // the token and query head of row i
+    const int rt = (r0 + i) / p.G;
+    tt = pr.q0 + rt, rq = hk * p.G + (r0 + i - rt * p.G);
+  };
+  if (l == 0)
+    for (int i = w; i < rows; i += 4) {
+      int tt, rq;
+      place(i, tt, rq);
+      const float2 st = f32_meet(ml, i);
+      if (a.many_pieces > 1)
+        a.part_ml[many_index(a, tt, rq) + piece] = st;
+      else
+        p.lse[tt * p.l_token + rq * p.l_head] = st.y == 0.f ? -FLT_MAX : (st.x + __builtin_amdgcn_logf(st.y)) * kLn2;
     }
-  }
+  f32_meet_all<NDT>(lds, O, w, col, hb, rows, d, [&](int i, float (&g)[4]) { f32_weights(ml, i, a.many_pieces == 1, g); },
+                    [&](int i, int c, float x) {
+                      int tt, rq;
+                      place(i, tt, rq);
+                      if (a.many_pieces > 1)
+                        a.part_o[(many_index(a, tt, rq) + piece) * d + c] = x;
+                      else
+                        Elem<T>::store((T*)p.out + tt * p.o_token + rq * p.o_head + c, x);
+                    });
 }
 
 // the pieces of a query row, in order: a wave a row
@@ -101,9 +108,9 @@ __global__ __launch_bounds__(256) void paged_f32_join_kernel(PagedTileArgs a) {
 
 template <typename T, bool VEC, int NDT>
 static int launch_paged_f32(const PagedTileArgs& a, hipStream_t st) {
-  FM_ALLOW_LDS((paged_f32_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_paged_attn_fwd(lds)");
+  FM_ALLOW_LDS((paged_f32_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(), "fm_paged_attn_fwd(lds)");
   hipLaunchKernelGGL((paged_f32_kernel<T, VEC, NDT>), dim3(unsigned(a.p.H * a.many_slots * a.many_pieces + nobody_groups(a.p))), dim3(256),
-                     f32_lds_bytes<NDT>(1), st, a, f32_score(a.p.sm_scale, a.p.softcap));
+                     f32_lds_bytes<NDT>(), st, a, f32_score(a.p.sm_scale, a.p.softcap));
   return launch_status("fm_paged_attn_fwd(f32)");
 }
 

@@ -47,18 +47,22 @@ static int sweep_pieces(int H, int G, int S, int L) {
   return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / blocks, ceil_div(L, 512)), 16)));
 }
 
-// The same of the fp32 products' kernels, a workgroup a compute unit: a block of 32 queries over tiles of 32 keys, of which a piece
-// has four at least, one a wave ..
-static int f32_pieces(int H, int G, int S, int L) {
+// Workgroups that the fp32 products' kernels are cut for: one a compute unit, three for every two where two fit one (d > 128).
+// Measured at d = 256, forward and backward, 256, 384, 512 workgroups: 8 query heads on one KV head x 1024: 470, 403, 414 us; 8 heads
+// x 1024: 452, 416, 419; 4 x 4 heads x 1024: 645, 706, 701; x 2048: 2295, 2085, 2089.
+static int64_t f32_want(int d) { return d > 128 ? 384 : 256; }
+
+// Into how many pieces theirs are cut: a block of 32 queries over tiles of 32 keys, of which a piece has four at least, one a wave ..
+static int f32_pieces(int H, int G, int S, int L, int d) {
   const int64_t blocks = int64_t(H) * G * ceil_div(S, 32);
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(256, blocks), ceil_div(L, 32) / 4), 16)));
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), ceil_div(L, 32) / 4), 16)));
 }
 // .. and a block of 32 keys over the tiles of 32 queries of its heads.  Measured, forward and backward in fp32, whole, in pieces for
 // 256 workgroups and for 512: 1 x 512 tokens d = 64: 65, 44 and 43 us; 1 x 8 heads x 1024, d = 64: 500, 124, 134; d = 128: 898, 209,
-// 220; d = 256: 1466, 456, 500; 8 heads x 512, d = 128: 105, 98, 132; 8 x 8 heads x 512, d = 64: 295, 209, 213.
-static int f32_splits(int H, int G, int S, int L) {
+// 220; 8 heads x 512, d = 128: 105, 98, 132; 8 x 8 heads x 512, d = 64: 295, 209, 213.
+static int f32_splits(int H, int G, int S, int L, int d) {
   const int64_t blocks = int64_t(H) * ceil_div(L, 32), steps = int64_t(G) * ceil_div(S, 32);
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(256, blocks), steps / 4), 16)));
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), steps / 4), 16)));
 }
 
 // The workspace of a forward: masks | partial sums.  `tiles`: of the 16-bit products' kernels.
@@ -68,7 +72,7 @@ struct FwdLayout {
 };
 static FwdLayout fwd_layout(int H, int G, int S, int L, int d, bool tiles) {
   FwdLayout y;
-  y.pieces = tiles ? sweep_pieces(H, G, S, L) : f32_pieces(H, G, S, L);
+  y.pieces = tiles ? sweep_pieces(H, G, S, L) : f32_pieces(H, G, S, L, d);
   const size_t units = y.pieces > 1 ? size_t(H) * G * S * y.pieces : 0;
   y.part_o = masks_layout(nullptr, S, L).bytes;
   y.part_ml = y.part_o + align_up(units * d * 4, 256);
@@ -157,8 +161,8 @@ static BwdLayout bwd_layout(int H, int G, int S, int L, int d, bool tiles) {
   b.n_q_norms = int(ceil_div(int64_t(H) * G * S, kNormRows));
   b.n_k_norms = int(ceil_div(int64_t(H) * L, kNormRows));
   b.part = b.norms + align_up(size_t(2 * b.n_q_norms + b.n_k_norms) * 4, 256);
-  b.splits = tiles ? dkv_splits(H, G, S, L) : f32_splits(H, G, S, L);
-  b.dq_pieces = tiles ? sweep_pieces(H, G, S, L) : f32_pieces(H, G, S, L);
+  b.splits = tiles ? dkv_splits(H, G, S, L) : f32_splits(H, G, S, L, d);
+  b.dq_pieces = tiles ? sweep_pieces(H, G, S, L) : f32_pieces(H, G, S, L, d);
   b.part_dq = b.part + (b.splits > 1 ? size_t(b.splits) * 2 * H * L * d * 4 : 0);
   b.total = b.part_dq + (b.dq_pieces > 1 ? size_t(b.dq_pieces) * H * G * S * d * 4 : 0);
   return b;

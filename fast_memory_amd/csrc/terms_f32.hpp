@@ -69,14 +69,17 @@ __device__ __forceinline__ void f32_resident(float (&x)[16 * NDT], const T* row,
   }
 }
 
-// The resident operand of a product, 4 NDT quads of a lane: registers, or LDS where there are two operands of 32 NDT = 256 dimensions
-// beside a sum of as many (registers for all spilled 455: 8 heads x 1024 d = 256, forward and backward, 2.86 ms against 2.56).  A row in
-// LDS has four words more than dimensions, so that eight neighbouring rows lie on different banks.
+// The resident operand of a product, 4 NDT quads of a lane: registers, or LDS at 32 NDT = 256, where two operands and a sum take three
+// quarters of a wave's registers: with them in LDS, and the waves' sums meeting there 128 dimensions at a time, two waves run on a SIMD
+// (8 x 8 heads x 512, fp32, d = 256, forward and backward: 895 us in registers, of which 455 spilled, 774 in LDS at one wave, 665 at
+// two).  A row in LDS has four words more than dimensions, so that eight neighbouring rows lie on different banks.
 template <int NDT>
 struct F32Regs {
   const float (&x)[16 * NDT];
   __device__ __forceinline__ float4 quad(int j) const { return make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]); }
 };
+template <int NDT>
+constexpr bool kF32Lds = NDT == 8;
 template <int NDT>
 struct F32Lds {
   static constexpr int kRow = 32 * NDT + 4;
@@ -98,21 +101,21 @@ struct F32Lds {
 template <typename T, bool VEC, int NDT, class Resident>
 __device__ __forceinline__ f32_acc f32_products_of(const T* row, const Resident& x, int d, int hb) {
   f32_acc s = f32_zero();
-  float4 v[2][4], u[2][4];
+  float4 v[2][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[0][i] = f32_load4<T, VEC>(row, 8 * i + 4 * hb, d), u[0][i] = x.quad(i);
+  for (int i = 0; i < 4; ++i) v[0][i] = f32_load4<T, VEC>(row, 8 * i + 4 * hb, d);
 #pragma unroll
   for (int g = 0; g < NDT; ++g) {
+    float4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = x.quad(4 * g + i);
     if (g + 1 < NDT)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[(g + 1) & 1][i] = f32_load4<T, VEC>(row, 32 * (g + 1) + 8 * i + 4 * hb, d);
-        u[(g + 1) & 1][i] = x.quad(4 * (g + 1) + i);
-      }
+      for (int i = 0; i < 4; ++i) v[(g + 1) & 1][i] = f32_load4<T, VEC>(row, 32 * (g + 1) + 8 * i + 4 * hb, d);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 a = v[g & 1][i], b = u[g & 1][i];
+      const float4 a = v[g & 1][i], b = u[i];
       s = mfma_f32(a.x, b.x, s);
       s = mfma_f32(a.y, b.y, s);
       s = mfma_f32(a.z, b.z, s);
@@ -219,28 +222,61 @@ __device__ __forceinline__ int2 f32_query_info(const F32Args& a, int i) {  // {l
   return make_int2(i < a.f.S ? seen_limit(i + (a.f.L - a.f.S), a.f.L, a.f.t.causal, 0) : 0, 0);
 }
 
+// The waves' sums meet in LDS, 128 dimensions at a time at most.
+constexpr int kMeetBlocks = 4;
 template <int NDT>
-constexpr size_t f32_lds_bytes(int sums) {
-  return 256 + size_t(sums) * 4 * 32 * (32 * NDT + 4) * 4 + 4 * 32 * 8;
+constexpr int meet_blocks() { return NDT < kMeetBlocks ? NDT : kMeetBlocks; }
+template <int NDT>
+constexpr int kMeetRow = 32 * meet_blocks<NDT>() + 4;
+template <int NDT>
+constexpr int kMeetFloats = 4 * 32 * kMeetRow<NDT>;  // (two operands of 256 dimensions in LDS take 260 x 64 of these 264 x 64)
+
+template <int NDT>
+constexpr size_t f32_lds_bytes() {
+  return 256 + size_t(kMeetFloats<NDT>) * 4 + 4 * 32 * 8;
 }
 
-// A wave's sums into LDS ([wave][32][Dp + 4]), then `dims` of a row summed over the waves with weights f
+// Part h of a wave's sums into LDS ([wave][32][dimensions + 4]), then dimension c of a row's part summed over the waves with weights f
 template <int NDT>
-__device__ __forceinline__ void f32_put(float* lds, const f32_acc (&acc)[NDT], int w, int col, int hb) {
-  float* mine = lds + (w * 32 + col) * (32 * NDT + 4) + 4 * hb;
+__device__ __forceinline__ void f32_put(float* lds, const f32_acc (&acc)[NDT], int h, int w, int col, int hb) {
+  float* mine = lds + (w * 32 + col) * kMeetRow<NDT> + 4 * hb;
 #pragma unroll
-  for (int dt = 0; dt < NDT; ++dt)
+  for (int dt = 0; dt < meet_blocks<NDT>(); ++dt)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<float4*>(mine + 32 * dt + 8 * q) = make_float4(acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]);
+    for (int q = 0; q < 4; ++q) {
+      const f32_acc& x = acc[meet_blocks<NDT>() * h + dt];
+      *reinterpret_cast<float4*>(mine + 32 * dt + 8 * q) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+    }
 }
 template <int NDT>
 __device__ __forceinline__ float f32_get(const float* lds, int row, int c, const float (&f)[4]) {
   float s = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) s = fmaf(lds[(w * 32 + row) * (32 * NDT + 4) + c], f[w], s);
+  for (int w = 0; w < 4; ++w) s = fmaf(lds[(w * 32 + row) * kMeetRow<NDT> + c], f[w], s);
   return s;
 }
+// All rows' sums over the waves, part 0 of which is in LDS already: write(row, dimension, value) a wave a row, dims of rows [0, n).
+// weights(row, f): what the waves weigh.
+template <int NDT, class Weights, class Write>
+__device__ __forceinline__ void f32_meet_all(float* lds, const f32_acc (&acc)[NDT], int w, int col, int hb, int n, int d, const Weights& weights,
+                                             const Write& write) {
+  constexpr int kDims = 32 * meet_blocks<NDT>();
+#pragma unroll
+  for (int h = 0; h < NDT / meet_blocks<NDT>(); ++h) {
+    if (h > 0) {
+      if (kDims * h >= d) return;
+      __syncthreads();
+      f32_put<NDT>(lds, acc, h, w, col, hb);
+      __syncthreads();
+    }
+    for (int i = w; i < n; i += 4) {
+      float f[4];
+      weights(i, f);
+      for (int c = lane_id(); c < kDims && kDims * h + c < d; c += 64) write(i, kDims * h + c, f32_get<NDT>(lds, i, c, f));
+    }
+  }
+}
+__device__ __forceinline__ void f32_ones(int, float (&f)[4]) { f[0] = f[1] = f[2] = f[3] = 1.f; }
 
 // what wave k's sums of a query weigh under the maximum m, and the query's {maximum, sum} over the waves
 __device__ __forceinline__ float f32_weight(const float2* ml, int i, int k, float m) {
@@ -255,10 +291,18 @@ __device__ __forceinline__ float2 f32_meet(const float2* ml, int i) {
   return make_float2(m, l);
 }
 
+// the waves' weights in a query's result, which is divided by its sum where it is whole
+__device__ __forceinline__ void f32_weights(const float2* ml, int i, bool whole, float (&g)[4]) {
+  const float2 st = f32_meet(ml, i);
+  const float inv = !whole ? 1.f : st.y == 0.f ? 0.f : 1.f / st.y;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) g[k] = f32_weight(ml, i, k, st.x) * inv;
+}
+
 // The sweep of a wave over tiles of 32 keys t = first, first + step, .. < t_end of one head.  row_of(j): where key j's row
 // begins, the same function for keys and values.  FLAT: rows follow one another.
-template <typename T, bool VEC, int NDT, bool FLAT, class RowOf, class Docs>
-__device__ __forceinline__ void f32_forward(const float (&qf)[16 * NDT], int pos, int lim, float slope2, int lim_lo, const T* K,
+template <typename T, bool VEC, int NDT, bool FLAT, class Resident, class RowOf, class Docs>
+__device__ __forceinline__ void f32_forward(const Resident& q, int pos, int lim, float slope2, int lim_lo, const T* K,
                                             const T* V, const RowOf& row_of, int n, int first, int step, int t_end, int d,
                                             const F32Score& score, const Docs& docs, f32_acc (&O)[NDT], float& m, float& sum,
                                             bool& dirty) {
@@ -275,7 +319,7 @@ __device__ __forceinline__ void f32_forward(const float (&qf)[16 * NDT], int pos
     bool masked = kp0 + 32 > lim_lo;
     if (!docs.meets(t, masked)) continue;
     masked = wave_any(masked);
-    const f32_acc s = f32_products<T, VEC, NDT>(K + at, qf, d, hb);
+    const f32_acc s = f32_products_of<T, VEC, NDT>(K + at, q, d, hb);
     float x[16], slack[16], mx = -INFINITY;
     f32_scores<false>(x, slack, s, score, slope2, pos - kp0 - 4 * hb, -1);
     if (masked) {
@@ -339,11 +383,11 @@ struct F32Docs {
 };
 
 template <typename T, bool VEC, int NDT>
-__global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
+__global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_fwd_kernel(F32Args a) {
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   int* flag = reinterpret_cast<int*>(f32_lds);
   float* lds = f32_lds + 64;
-  float2* ml = reinterpret_cast<float2*>(lds + 4 * 32 * (32 * NDT + 4));
+  float2* ml = reinterpret_cast<float2*>(lds + kMeetFloats<NDT>);
   const FwdArgs& f = a.f;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
   const int heads = f.H * f.G, bx = int(blockIdx.x) % heads;
@@ -356,8 +400,14 @@ __global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
   const int2 qi = f32_query_info(a, iq);
   const int4 qm = f32_query_meta(a, i0);
   const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
-  float qf[16 * NDT];
-  f32_resident<T, VEC, NDT>(qf, (const T*)f.q + (int64_t(hq) * f.S + (ok ? iq : 0)) * d, ok, d, hb);
+  constexpr bool kLds = kF32Lds<NDT>;
+  float qf[kLds ? 1 : 16 * NDT];
+  if constexpr (kLds) {
+    F32Lds<NDT>::template fill<T, VEC>(lds, (const T*)f.q + (int64_t(hq) * f.S + i0) * d, f.S - i0, d);
+    __syncthreads();
+  } else {
+    f32_resident<T, VEC, NDT>(qf, (const T*)f.q + (int64_t(hq) * f.S + (ok ? iq : 0)) * d, ok, d, hb);
+  }
   const T* K = (const T*)f.k + int64_t(hk) * f.L * d;
   const T* V = (const T*)f.v + int64_t(hk) * f.L * d;
   const F32Docs docs{a.m.kmeta, a.m.dock, qm.z, qm.w, qi.y, f.t.doc_q != nullptr};
@@ -366,11 +416,18 @@ __global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
   bool dirty = false;
   int t0 = 0, t1 = (qm.y + 31) / 32;
   tile_piece(t0, t1, piece, a.pieces);
-  f32_forward<T, VEC, NDT, true>(qf, iq + (f.L - f.S), qi.x, slope2, qm.x, K, V, [&](int j) { return int64_t(j) * d; }, f.L, t0 + w, 4,
-                           t1, d, a.score, docs, O, m, sum, dirty);
+  auto sweep = [&](const auto& q) {
+    f32_forward<T, VEC, NDT, true>(q, iq + (f.L - f.S), qi.x, slope2, qm.x, K, V, [&](int j) { return int64_t(j) * d; }, f.L, t0 + w, 4,
+                                   t1, d, a.score, docs, O, m, sum, dirty);
+  };
+  if constexpr (kLds)
+    sweep(F32Lds<NDT>(lds, col, hb));
+  else
+    sweep(F32Regs<NDT>{qf});
   if (dirty) *flag = 1;
   sum += __shfl_xor(sum, 32);
-  f32_put<NDT>(lds, O, w, col, hb);
+  if constexpr (kLds) __syncthreads();
+  f32_put<NDT>(lds, O, 0, w, col, hb);
   if (hb == 0) ml[w * 32 + col] = make_float2(m, sum);
   __syncthreads();
   if (*flag) {  // values that are not finite, in tiles with masked places: a row at a time (terms.hpp)
@@ -393,23 +450,22 @@ __global__ __launch_bounds__(256, 1) void terms_f32_fwd_kernel(F32Args a) {
     }
     return;
   }
-  for (int i = w; i < 32 && i0 + i < f.S; i += 4) {  // a wave a query
-    const float2 st = f32_meet(ml, i);
-    float g[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) g[k] = f32_weight(ml, i, k, st.x);
-    const int64_t r = int64_t(hq) * f.S + i0 + i;
-    if (a.pieces > 1) {
-      const int64_t at = r * a.pieces + piece;
-      for (int c = l; c < d; c += 64) a.part_o[at * d + c] = f32_get<NDT>(lds, i, c, g);
-      if (l == 0) a.part_ml[at] = st;
-      continue;
+  const int n = min(32, f.S - i0);
+  const int64_t r0 = int64_t(hq) * f.S + i0;
+  if (l == 0)
+    for (int i = w; i < n; i += 4) {
+      const float2 st = f32_meet(ml, i);
+      if (a.pieces > 1)
+        a.part_ml[(r0 + i) * a.pieces + piece] = st;
+      else
+        f.lse[r0 + i] = st.y == 0.f ? -FLT_MAX : (st.x + __builtin_amdgcn_logf(st.y)) * kLn2;
     }
-    const bool none = st.y == 0.f;
-    const float inv = none ? 0.f : 1.f / st.y;
-    for (int c = l; c < d; c += 64) Elem<T>::store((T*)f.out + r * d + c, f32_get<NDT>(lds, i, c, g) * inv);
-    if (l == 0) f.lse[r] = none ? -FLT_MAX : (st.x + __builtin_amdgcn_logf(st.y)) * kLn2;
-  }
+  f32_meet_all<NDT>(lds, O, w, col, hb, n, d, [&](int i, float (&g)[4]) { f32_weights(ml, i, a.pieces == 1, g); }, [&](int i, int c, float x) {
+    if (a.pieces > 1)
+      a.part_o[((r0 + i) * a.pieces + piece) * d + c] = x;
+    else
+      Elem<T>::store((T*)f.out + (r0 + i) * d + c, x);
+  });
 }
 
 // the pieces of a query row, in order: a wave a row
@@ -473,7 +529,7 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
   const int4 qm = f32_query_meta(a, i0);
   const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
   const int64_t row = int64_t(hq) * f.S + (ok ? iq : 0);
-  constexpr bool kLds = NDT == 8;  // both in LDS, where the waves' sums go at the end
+  constexpr bool kLds = kF32Lds<NDT>;
   float qf[kLds ? 1 : 16 * NDT], df[kLds ? 1 : 16 * NDT];
   if constexpr (kLds) {
     F32Lds<NDT>::template fill<T, VEC>(lds + 32 * F32Lds<NDT>::kRow, (const T*)f.q + (int64_t(hq) * f.S + i0) * d, f.S - i0, d);
@@ -523,7 +579,7 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
   }
   if (dirty) *flag = 1;
   if constexpr (kLds) __syncthreads();
-  f32_put<NDT>(lds, O, w, col, hb);
+  f32_put<NDT>(lds, O, 0, w, col, hb);
   __syncthreads();
   if (*flag) {
     const KeyRows<T> KR{K, nullptr, 0, 0, 0, d}, VR{V, nullptr, 0, 0, 0, d};
@@ -544,15 +600,13 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
     }
     return;
   }
-  const float one[4] = {1.f, 1.f, 1.f, 1.f};
-  for (int i = w; i < 32 && i0 + i < f.S; i += 4)
-    for (int c = l; c < d; c += 64) {
-      const float x = f32_get<NDT>(lds, i, c, one) * f.sm_scale;
-      if (part)
-        part[int64_t(i0 + i) * d + c] = x;
-      else
-        Elem<T>::store((T*)a.dq + (int64_t(hq) * f.S + i0 + i) * d + c, x);
-    }
+  f32_meet_all<NDT>(lds, O, w, col, hb, min(32, f.S - i0), d, f32_ones, [&](int i, int c, float x) {
+    x *= f.sm_scale;
+    if (part)
+      part[int64_t(i0 + i) * d + c] = x;
+    else
+      Elem<T>::store((T*)a.dq + (int64_t(hq) * f.S + i0 + i) * d + c, x);
+  });
 }
 
 // dk and dv of 32 keys; PART as in terms_bwd.hpp (both sums and both operands of a padded dimension of 256 are 512 registers)
@@ -572,12 +626,12 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
   const int doc = has_docs ? a.m.dock[j] : 0;
   const int2 km = has_docs ? a.m.kmeta[j0 / 32] : make_int2(0, 0);
   const int64_t row = (int64_t(hk) * f.L + (ok ? j : 0)) * d;
-  constexpr bool kLds = kDk && NDT == 8;  // keys and values in LDS, as q and dout above
+  constexpr bool kLds = kF32Lds<NDT>;
   float kf[kLds ? 1 : 16 * NDT], vf[kDk && !kLds ? 16 * NDT : 1];
   if constexpr (!kLds) f32_resident<T, VEC, NDT>(kf, (const T*)f.k + row, ok, d, hb);
   if constexpr (kLds) {
     F32Lds<NDT>::template fill<T, VEC>(lds + 32 * F32Lds<NDT>::kRow, (const T*)f.k + (int64_t(hk) * f.L + j0) * d, f.L - j0, d);
-    F32Lds<NDT>::template fill<T, VEC>(lds, (const T*)f.v + (int64_t(hk) * f.L + j0) * d, f.L - j0, d);
+    if constexpr (kDk) F32Lds<NDT>::template fill<T, VEC>(lds, (const T*)f.v + (int64_t(hk) * f.L + j0) * d, f.L - j0, d);
     __syncthreads();
   } else if constexpr (kDk) {
     f32_resident<T, VEC, NDT>(vf, (const T*)f.v + row, ok, d, hb);
@@ -657,10 +711,9 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
   }
   if (dirty) *flag = 1;
   if constexpr (kLds) __syncthreads();
-  if constexpr (kDk) f32_put<NDT>(lds, dK, w, col, hb);
+  if constexpr (kDk) f32_put<NDT>(lds, dK, 0, w, col, hb);
   __syncthreads();
   const int last = min(32, f.L - j0);
-  const float one[4] = {1.f, 1.f, 1.f, 1.f};
   // element c of key jj's gradients, x of dk (times sm_scale here) and of dv
   const int64_t plane = int64_t(f.H) * f.L * d;
   auto put = [&](bool dv, int jj, int c, float x) {
@@ -696,16 +749,12 @@ __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float
     }
     return;
   }
-  if constexpr (kDk) {
-    for (int i = w; i < last; i += 4)
-      for (int c = l; c < d; c += 64) put(false, j0 + i, c, f32_get<NDT>(lds, i, c, one));
-  }
+  if constexpr (kDk) f32_meet_all<NDT>(lds, dK, w, col, hb, last, d, f32_ones, [&](int i, int c, float x) { put(false, j0 + i, c, x); });
   if constexpr (kDv) {
     if constexpr (kDk) __syncthreads();
-    f32_put<NDT>(lds, dV, w, col, hb);
+    f32_put<NDT>(lds, dV, 0, w, col, hb);
     __syncthreads();
-    for (int i = w; i < last; i += 4)
-      for (int c = l; c < d; c += 64) put(true, j0 + i, c, f32_get<NDT>(lds, i, c, one));
+    f32_meet_all<NDT>(lds, dV, w, col, hb, last, d, f32_ones, [&](int i, int c, float x) { put(true, j0 + i, c, x); });
   }
 }
 
@@ -725,7 +774,7 @@ __global__ __launch_bounds__(256) void terms_f32_bwd_join_kernel(F32Args a, int6
 }
 
 template <typename T, bool VEC, int NDT>
-__global__ __launch_bounds__(256, 1) void terms_f32_bwd_kernel(F32Args a, int dkv_blocks) {
+__global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_bwd_kernel(F32Args a, int dkv_blocks) {
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   const int block = blockIdx.x;
   if constexpr (NDT == 8) {
@@ -740,9 +789,9 @@ __global__ __launch_bounds__(256, 1) void terms_f32_bwd_kernel(F32Args a, int dk
 
 template <typename T, bool VEC, int NDT>
 static int launch_f32_fwd(const F32Args& a, hipStream_t st) {
-  FM_ALLOW_LDS((terms_f32_fwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_local_attn_terms_fwd(lds)");
+  FM_ALLOW_LDS((terms_f32_fwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(), "fm_local_attn_terms_fwd(lds)");
   hipLaunchKernelGGL((terms_f32_fwd_kernel<T, VEC, NDT>), dim3(unsigned(a.f.H * a.f.G * ceil_div(a.f.S, 32) * a.pieces)), dim3(256),
-                     f32_lds_bytes<NDT>(1), st, a);
+                     f32_lds_bytes<NDT>(), st, a);
   return launch_status("fm_local_attn_terms_fwd(f32)");
 }
 template <typename T>
@@ -755,10 +804,10 @@ static int launch_delta(const BwdArgs& a, float2* rd, hipStream_t st) {
 
 template <typename T, bool VEC, int NDT>
 static int launch_f32_bwd(const F32Args& a, hipStream_t st) {
-  FM_ALLOW_LDS((terms_f32_bwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(1), "fm_local_attn_terms_bwd(lds)");
+  FM_ALLOW_LDS((terms_f32_bwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(), "fm_local_attn_terms_bwd(lds)");
   const int dkv = int(a.f.H * ceil_div(a.f.L, 32) * a.splits), dq = int(a.f.H * a.f.G * ceil_div(a.f.S, 32) * a.pieces);
   hipLaunchKernelGGL((terms_f32_bwd_kernel<T, VEC, NDT>), dim3(unsigned((NDT == 8 ? 2 : 1) * dkv + dq)), dim3(256),
-                     f32_lds_bytes<NDT>(1), st, a, dkv);
+                     f32_lds_bytes<NDT>(), st, a, dkv);
   return launch_status("fm_local_attn_terms_bwd(f32)");
 }
 

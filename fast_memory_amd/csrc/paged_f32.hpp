@@ -13,14 +13,14 @@ namespace fm {
 
 constexpr int kF32Rows = 32;  // query rows of a workgroup
 
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 __global__ __launch_bounds__(256, 1) void paged_f32_kernel(PagedTileArgs a, F32Score score) {
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   int* flag = reinterpret_cast<int*>(f32_lds);
   float* lds = f32_lds + 64;
   float2* ml = reinterpret_cast<float2*>(lds + kMeetFloats<NDT>);
   const PagedArgs& p = a.p;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = p.d;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f32_dims<VEC, NDT>(p.d);
   const int units = p.H * a.many_slots * a.many_pieces;
   if (int(blockIdx.x) >= units) return paged_nobody<T>(a, int(blockIdx.x) - units, int(gridDim.x) - units);
   const int hk = int(blockIdx.x) % p.H, rest = int(blockIdx.x) / p.H;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void paged_f32_join_kernel(PagedTileArgs a) {
                a.p.lse + t * a.p.l_token + hq * a.p.l_head);
 }
 
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 static int launch_paged_f32(const PagedTileArgs& a, hipStream_t st) {
   FM_ALLOW_LDS((paged_f32_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(), "fm_paged_attn_fwd(lds)");
   hipLaunchKernelGGL((paged_f32_kernel<T, VEC, NDT>), dim3(unsigned(a.p.H * a.many_slots * a.many_pieces + nobody_groups(a.p))), dim3(256),
@@ -116,7 +116,7 @@ static int launch_paged_f32(const PagedTileArgs& a, hipStream_t st) {
 
 template <typename T>
 int paged_f32(const PagedTileArgs& a, const PagedPlan& y, hipStream_t st) {
-  const bool vec = f32_vec<T>(a.p.d, {a.p.q, a.p.k, a.p.v}) && a.p.q_token % 4 == 0 && a.p.q_head % 4 == 0;
+  const int vec = a.p.q_token % 4 == 0 && a.p.q_head % 4 == 0 ? f32_vec<T>(a.p.d, {a.p.q, a.p.k, a.p.v}) : kOne;
 #define FM_F(V, N) launch_paged_f32<T, V, N>(a, st)
   const int rc = FM_F32_BY_DIM(a.p.d, vec, FM_F);
 #undef FM_F

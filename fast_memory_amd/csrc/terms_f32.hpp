@@ -39,10 +39,16 @@ __device__ __forceinline__ f32_acc f32_zero() {
 // the row of register r of a block, without the half's 4 hb
 __device__ __forceinline__ constexpr int f32_row(int r) { return 8 * (r >> 2) + (r & 3); }
 
+// VEC: how rows are read.  kOne: an element at a time; kFour: four (d a multiple of 4, rows aligned to four elements); kWhole: four,
+// and d is the instance's 32 NDT, so that no load asks where its row ends (every offset is then a constant of its instruction)
+constexpr int kOne = 0, kFour = 1, kWhole = 2;
+template <int VEC, int NDT>
+__device__ __forceinline__ int f32_dims(int d) { return VEC == kWhole ? 32 * NDT : d; }
+
 // four elements of a row from dimension c, zero behind the row's d
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __device__ __forceinline__ float4 f32_load4(const T* __restrict__ row, int c, int d) {
-  if constexpr (VEC) {  // d a multiple of 4, rows aligned to four elements
+  if constexpr (VEC != kOne) {
     if (c >= d) return make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (std::is_same<T, float>::value) {
       return *reinterpret_cast<const float4*>(row + c);
@@ -60,7 +66,7 @@ __device__ __forceinline__ float4 f32_load4(const T* __restrict__ row, int c, in
 }
 
 // this lane's half of a row (dimensions 8 j + 4 hb ..), to stay in registers
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 __device__ __forceinline__ void f32_resident(float (&x)[16 * NDT], const T* row, bool ok, int d, int hb) {
 #pragma unroll
   for (int j = 0; j < 4 * NDT; ++j) {
@@ -87,7 +93,7 @@ struct F32Lds {
   __device__ __forceinline__ F32Lds(const float* lds, int col, int hb) : at(lds + col * kRow + 4 * hb) {}
   __device__ __forceinline__ float4 quad(int j) const { return *reinterpret_cast<const float4*>(at + 8 * j); }
   // 32 rows from `rows`, of which the first n are there; all threads of the workgroup
-  template <typename T, bool VEC>
+  template <typename T, int VEC>
   __device__ static __forceinline__ void fill(float* lds, const T* rows, int n, int d) {
     for (int i = threadIdx.x; i < 32 * 8 * NDT; i += 256) {
       const int r = i / (8 * NDT), c = 4 * (i % (8 * NDT));
@@ -98,7 +104,7 @@ struct F32Lds {
 
 // products of 32 streamed rows (this lane's is `row`) with the resident ones.  Sixteen elements are in flight while the
 // products of the sixteen before them run (1024 cycles); the barriers keep the compiler from loading everything at once.
-template <typename T, bool VEC, int NDT, class Resident>
+template <typename T, int VEC, int NDT, class Resident>
 __device__ __forceinline__ f32_acc f32_products_of(const T* row, const Resident& x, int d, int hb) {
   f32_acc s = f32_zero();
   float4 v[2][4];
@@ -125,7 +131,7 @@ __device__ __forceinline__ f32_acc f32_products_of(const T* row, const Resident&
   }
   return s;
 }
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 __device__ __forceinline__ f32_acc f32_products(const T* row, const float (&x)[16 * NDT], int d, int hb) {
   return f32_products_of<T, VEC, NDT>(row, F32Regs<NDT>{x}, d, hb);
 }
@@ -301,7 +307,7 @@ __device__ __forceinline__ void f32_weights(const float2* ml, int i, bool whole,
 
 // The sweep of a wave over tiles of 32 keys t = first, first + step, .. < t_end of one head.  row_of(j): where key j's row
 // begins, the same function for keys and values.  FLAT: rows follow one another.
-template <typename T, bool VEC, int NDT, bool FLAT, class Resident, class RowOf, class Docs>
+template <typename T, int VEC, int NDT, bool FLAT, class Resident, class RowOf, class Docs>
 __device__ __forceinline__ void f32_forward(const Resident& q, int pos, int lim, float slope2, int lim_lo, const T* K,
                                             const T* V, const RowOf& row_of, int n, int first, int step, int t_end, int d,
                                             const F32Score& score, const Docs& docs, f32_acc (&O)[NDT], float& m, float& sum,
@@ -382,14 +388,14 @@ struct F32Docs {
   }
 };
 
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 __global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_fwd_kernel(F32Args a) {
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   int* flag = reinterpret_cast<int*>(f32_lds);
   float* lds = f32_lds + 64;
   float2* ml = reinterpret_cast<float2*>(lds + kMeetFloats<NDT>);
   const FwdArgs& f = a.f;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f32_dims<VEC, NDT>(f.d);
   const int heads = f.H * f.G, bx = int(blockIdx.x) % heads;
   const int hk = bx % f.H, hq = hk * f.G + bx / f.H;
   const int rest = int(blockIdx.x) / heads, piece = rest % a.pieces;
@@ -512,12 +518,12 @@ __global__ __launch_bounds__(256) void terms_delta_kernel(const T* __restrict__ 
   if (lane_id() == 0) rd[row] = make_float2(lse[row] * kLog2e, s - (dlse ? dlse[row] : 0.f));
 }
 
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float* f32_lds) {
   int* flag = reinterpret_cast<int*>(f32_lds);
   float* lds = f32_lds + 64;
   const FwdArgs& f = a.f;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f32_dims<VEC, NDT>(f.d);
   const int heads = f.H * f.G, bx = block % heads;
   const int hk = bx % f.H, hq = hk * f.G + bx / f.H;
   const int rest = block / heads, piece = rest % a.pieces;
@@ -612,13 +618,13 @@ __device__ __forceinline__ void f32_dq_block(const F32Args& a, int block, float*
 // dk and dv of 32 keys; PART as in terms_bwd.hpp (both sums and both operands of a padded dimension of 256 are 512 registers)
 constexpr int kF32Both = 0, kF32Dv = 1, kF32Dk = 2;
 
-template <typename T, bool VEC, int NDT, int PART>
+template <typename T, int VEC, int NDT, int PART>
 __device__ __forceinline__ void f32_dkv_block(const F32Args& a, int block, float* f32_lds) {
   constexpr bool kDk = PART != kF32Dv, kDv = PART != kF32Dk;
   int* flag = reinterpret_cast<int*>(f32_lds);
   float* lds = f32_lds + 64;
   const FwdArgs& f = a.f;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f.d;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, col = l & 31, hb = l >> 5, d = f32_dims<VEC, NDT>(f.d);
   const int hk = block % f.H, part = block / f.H, split = part % a.splits, j0 = part / a.splits * 32, j = j0 + col;
   if (tid == 0) *flag = 0;
   __syncthreads();
@@ -773,7 +779,7 @@ __global__ __launch_bounds__(256) void terms_f32_bwd_join_kernel(F32Args a, int6
   Elem<T>::store(is_q ? (T*)a.dq + i : i < plane ? (T*)a.dk + i : (T*)a.dv + (i - plane), x);
 }
 
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 __global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_bwd_kernel(F32Args a, int dkv_blocks) {
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   const int block = blockIdx.x;
@@ -787,7 +793,7 @@ __global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_bwd_kerne
   }
 }
 
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 static int launch_f32_fwd(const F32Args& a, hipStream_t st) {
   FM_ALLOW_LDS((terms_f32_fwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(), "fm_local_attn_terms_fwd(lds)");
   hipLaunchKernelGGL((terms_f32_fwd_kernel<T, VEC, NDT>), dim3(unsigned(a.f.H * a.f.G * ceil_div(a.f.S, 32) * a.pieces)), dim3(256),
@@ -802,7 +808,7 @@ static int launch_delta(const BwdArgs& a, float2* rd, hipStream_t st) {
   return launch_status("fm_local_attn_terms_bwd(delta)");
 }
 
-template <typename T, bool VEC, int NDT>
+template <typename T, int VEC, int NDT>
 static int launch_f32_bwd(const F32Args& a, hipStream_t st) {
   FM_ALLOW_LDS((terms_f32_bwd_kernel<T, VEC, NDT>), f32_lds_bytes<NDT>(), "fm_local_attn_terms_bwd(lds)");
   const int dkv = int(a.f.H * ceil_div(a.f.L, 32) * a.splits), dq = int(a.f.H * a.f.G * ceil_div(a.f.S, 32) * a.pieces);
@@ -811,21 +817,20 @@ static int launch_f32_bwd(const F32Args& a, hipStream_t st) {
   return launch_status("fm_local_attn_terms_bwd(f32)");
 }
 
-// rows of d elements that can be read four at a time
+// how rows of d elements are read
 template <typename T>
-static bool f32_vec(int d, std::initializer_list<const void*> ptrs) {
+static int f32_vec(int d, std::initializer_list<const void*> ptrs) {
   bool ok = d % 4 == 0;
   for (const void* p : ptrs) ok = ok && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0;
-  return ok;
+  return !ok ? kOne : d == 64 || d == 128 || d == 256 ? kWhole : kFour;
 }
-#define FM_F32_BY_DIM(d, vec, F)             \
-  ((d) <= 64    ? ((vec) ? F(true, 2) : F(false, 2)) \
-   : (d) <= 128 ? ((vec) ? F(true, 4) : F(false, 4)) \
-                : ((vec) ? F(true, 8) : F(false, 8)))
+#define FM_F32_BY_VEC(vec, F, N) ((vec) == kWhole ? F(kWhole, N) : (vec) == kFour ? F(kFour, N) : F(kOne, N))
+#define FM_F32_BY_DIM(d, vec, F) \
+  ((d) <= 64 ? FM_F32_BY_VEC(vec, F, 2) : (d) <= 128 ? FM_F32_BY_VEC(vec, F, 4) : FM_F32_BY_VEC(vec, F, 8))
 
 template <typename T>
 int terms_f32_fwd(const F32Args& a, hipStream_t st) {
-  const bool vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v});
+  const int vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v});
 #define FM_F(V, N) launch_f32_fwd<T, V, N>(a, st)
   const int rc = FM_F32_BY_DIM(a.f.d, vec, FM_F);
 #undef FM_F
@@ -837,7 +842,7 @@ template <typename T>
 int terms_f32_bwd(const F32Args& a, const BwdArgs& b, float2* rd, hipStream_t st) {
   int rc = launch_delta<T>(b, rd, st);
   if (rc) return rc;
-  const bool vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v, a.dout});
+  const int vec = f32_vec<T>(a.f.d, {a.f.q, a.f.k, a.f.v, a.dout});
 #define FM_F(V, N) launch_f32_bwd<T, V, N>(a, st)
   rc = FM_F32_BY_DIM(a.f.d, vec, FM_F);
 #undef FM_F

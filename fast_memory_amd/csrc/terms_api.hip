@@ -41,10 +41,10 @@ static bool tiles_take(int d, int dtype) {
 // Into how many pieces the keys of a block of 128 queries are cut: until there are 512 workgroups, two a compute unit, none of
 // less than 8 tiles of 64 keys.  Measured, whole and in pieces, bf16: 2 heads x 4096, d = 256: forward 220 and 64 us, backward
 // 606 and 280; 8 heads x 128 over 4096 keys, d = 128: 122 and 28, 193 and 48; 16 x 2048: 66 and 52, 150 and 131; 32 x 1024
-// (256 blocks): 37 and 37, 93 and 88.
+// (256 blocks): 37 and 37, 93 and 88.  At most 64 pieces: one token over 2^20 keys, d = 128, forward 344 us (16 pieces: 1271).
 static int sweep_pieces(int H, int G, int S, int L) {
   const int64_t blocks = int64_t(H) * G * ceil_div(S, kTQ);
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / blocks, ceil_div(L, 512)), 16)));
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / blocks, ceil_div(L, 512)), 64)));
 }
 
 // Workgroups that the fp32 products' kernels are cut for: one a compute unit, three for every two where two fit one (d > 128).
@@ -55,14 +55,14 @@ static int64_t f32_want(int d) { return d > 128 ? 384 : 256; }
 // Into how many pieces theirs are cut: a block of 32 queries over tiles of 32 keys, of which a piece has four at least, one a wave ..
 static int f32_pieces(int H, int G, int S, int L, int d) {
   const int64_t blocks = int64_t(H) * G * ceil_div(S, 32);
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), ceil_div(L, 32) / 4), 16)));
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), ceil_div(L, 32) / 4), 64)));
 }
 // .. and a block of 32 keys over the tiles of 32 queries of its heads.  Measured, forward and backward in fp32, whole, in pieces for
 // 256 workgroups and for 512: 1 x 512 tokens d = 64: 65, 44 and 43 us; 1 x 8 heads x 1024, d = 64: 500, 124, 134; d = 128: 898, 209,
 // 220; 8 heads x 512, d = 128: 105, 98, 132; 8 x 8 heads x 512, d = 64: 295, 209, 213.
 static int f32_splits(int H, int G, int S, int L, int d) {
   const int64_t blocks = int64_t(H) * ceil_div(L, 32), steps = int64_t(G) * ceil_div(S, 32);
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), steps / 4), 16)));
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), steps / 4), 64)));
 }
 
 // The workspace of a forward: masks | partial sums.  `tiles`: of the 16-bit products' kernels.
@@ -146,12 +146,13 @@ struct BwdLayout {
 
 // Into how many pieces the sweeps over the queries are cut: two workgroups a compute unit at least (512 in all), and four
 // where a piece still has 64 tiles of queries (under a causal mask the first keys' sweeps are twice the average, and more
-// pieces end more evenly); none of less than 4 tiles.  Measured, 512 against 1024 workgroups: 32 heads x 2048 tokens,
+// pieces end more evenly); none of less than 4 tiles, 64 at most (2^18 queries over 64 keys, d = 128, forward and backward: 304 us, with
+// 16 at most 882).  Measured, 512 against 1024 workgroups: 32 heads x 2048 tokens,
 // d = 128: 0.153 and 0.198 ms (the pieces' partial sums are written and read); 64 x 4096, five documents: 0.59 and 0.48.
 static int dkv_splits(int H, int G, int S, int L) {
   const int64_t blocks = int64_t(H) * ceil_div(L, kDkvKeys), steps = int64_t(G) * ceil_div(S, kDkvQ);
   const int64_t want = std::max(ceil_div(512, blocks), std::min(ceil_div(1024, blocks), steps / 64));
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min(want, steps / 4), 16)));
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min(want, steps / 4), 64)));
 }
 
 static BwdLayout bwd_layout(int H, int G, int S, int L, int d, bool tiles) {

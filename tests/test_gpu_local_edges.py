@@ -307,3 +307,11 @@ def test_pieces_of_queries_with_masked_places_that_are_not_finite(dtype, d, bad)
     again = ops.local_attn_terms_bwd(gdo, gq, gk, gv, out, lse, scale, False, on_gpu(t), gdl)
     for x, y in zip(got, again):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("S,L,t", [(9000, 40, {}), (6000, 129, dict(softcap=20.0)), (1, 40000, {}), (3, 33000, dict(softcap=20.0))])
+def test_a_single_block_in_many_pieces(dtype, d, S, L, t):
+    """One block of keys under many queries, and of queries over many keys: up to 64 pieces."""
+    check(131, 1, 1, S, L, d, dtype, S < L, t)

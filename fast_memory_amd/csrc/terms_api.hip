@@ -47,23 +47,19 @@ static int sweep_pieces(int H, int G, int S, int L) {
   return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / blocks, ceil_div(L, 512)), 64)));
 }
 
-// Workgroups that the fp32 products' kernels are cut for: one a compute unit, three for every two where two fit one (d > 128).
-// Measured at d = 256, forward and backward, 256, 384, 512 workgroups: 8 query heads on one KV head x 1024: 470, 403, 414 us; 8 heads
-// x 1024: 452, 416, 419; 4 x 4 heads x 1024: 645, 706, 701; x 2048: 2295, 2085, 2089.
-static int64_t f32_want(int d) { return d > 128 ? 384 : 256; }
-
-// Into how many pieces theirs are cut: a block of 32 queries over tiles of 32 keys, of which a piece has four at least, one a wave ..
-static int f32_pieces(int H, int G, int S, int L, int d) {
-  const int64_t blocks = int64_t(H) * G * ceil_div(S, 32);
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), ceil_div(L, 32) / 4), 64)));
+// Into how many pieces the sweep of a block is cut in the fp32 products' kernels, whose workgroups take 32 queries (or keys) and a tile
+// of 32 on the other side a wave: until there is a workgroup for every compute unit, three for every two between d = 128 and 256 (where two
+// fit one), none of less than four tiles, one a wave.  At d = 256 two for every one where a piece keeps 16 tiles.  Measured in fp32, causal,
+// forward and backward, whole, in pieces for 256 workgroups and for 512: one head x 512, d = 64: 65, 44 and 43 us; 8 query heads on one KV
+// head x 1024, d = 64: 500, 124, 134; d = 128: 898, 209, 220; 8 heads x 512, d = 128: 105, 98, 132; d = 256: 205, 142, 203; 4 heads on one
+// x 2248 without a mask, d = 256: 2174, 1251, 1103.
+static int f32_cut(int64_t blocks, int64_t tiles, int d) {
+  const int64_t few = std::min(ceil_div(d > 128 && d < 256 ? 384 : 256, blocks), tiles / 4);
+  const int64_t many = d == 256 ? std::min(ceil_div(512, blocks), tiles / 16) : 1;
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::max(few, many), 64)));
 }
-// .. and a block of 32 keys over the tiles of 32 queries of its heads.  Measured, forward and backward in fp32, whole, in pieces for
-// 256 workgroups and for 512: 1 x 512 tokens d = 64: 65, 44 and 43 us; 1 x 8 heads x 1024, d = 64: 500, 124, 134; d = 128: 898, 209,
-// 220; 8 heads x 512, d = 128: 105, 98, 132; 8 x 8 heads x 512, d = 64: 295, 209, 213.
-static int f32_splits(int H, int G, int S, int L, int d) {
-  const int64_t blocks = int64_t(H) * ceil_div(L, 32), steps = int64_t(G) * ceil_div(S, 32);
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(f32_want(d), blocks), steps / 4), 64)));
-}
+static int f32_pieces(int H, int G, int S, int L, int d) { return f32_cut(int64_t(H) * G * ceil_div(S, 32), ceil_div(L, 32), d); }
+static int f32_splits(int H, int G, int S, int L, int d) { return f32_cut(int64_t(H) * ceil_div(L, 32), int64_t(G) * ceil_div(S, 32), d); }
 
 // The workspace of a forward: masks | partial sums.  `tiles`: of the 16-bit products' kernels.
 struct FwdLayout {

@@ -75,10 +75,12 @@ __device__ __forceinline__ void f32_resident(float (&x)[16 * NDT], const T* row,
   }
 }
 
-// The resident operand of a product, 4 NDT quads of a lane: registers, or LDS at 32 NDT = 256, where two operands and a sum take three
-// quarters of a wave's registers: with them in LDS, and the waves' sums meeting there 128 dimensions at a time, two waves run on a SIMD
-// (8 x 8 heads x 512, fp32, d = 256, forward and backward: 895 us in registers, of which 455 spilled, 774 in LDS at one wave, 665 at
-// two).  A row in LDS has four words more than dimensions, so that eight neighbouring rows lie on different banks.
+// The resident operand of a product, 4 NDT quads of a lane: registers, or LDS in the backward at 32 NDT = 256, where two operands and a
+// sum would take three quarters of a wave's registers and 455 spilled (16 heads x 1024, fp32, d = 256: 606 us, with LDS 378).  The waves'
+// sums meet in LDS 128 dimensions at a time, so that two workgroups of such a kernel fit a compute unit: with loads that ask where a row
+// ends, two waves a SIMD (and the forward's operand in LDS as well) are the faster (2 x 4 heads x 900, d = 192: forward 87 against 96 us,
+// backward 268 against 295), without one (16 heads x 1024, d = 256: 112 against 168, 378 against 478).
+// A row in LDS has four words more than dimensions, so that eight neighbouring rows lie on different banks.
 template <int NDT>
 struct F32Regs {
   const float (&x)[16 * NDT];
@@ -86,6 +88,9 @@ struct F32Regs {
 };
 template <int NDT>
 constexpr bool kF32Lds = NDT == 8;
+// whether two waves are to run on a SIMD there: where the loads have their bounds to ask for
+template <int VEC, int NDT>
+constexpr bool f32_two_waves() { return kF32Lds<NDT> && VEC != kWhole; }
 template <int NDT>
 struct F32Lds {
   static constexpr int kRow = 32 * NDT + 4;
@@ -389,7 +394,7 @@ struct F32Docs {
 };
 
 template <typename T, int VEC, int NDT>
-__global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_fwd_kernel(F32Args a) {
+__global__ __launch_bounds__(256, (f32_two_waves<VEC, NDT>() ? 2 : 1)) void terms_f32_fwd_kernel(F32Args a) {
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   int* flag = reinterpret_cast<int*>(f32_lds);
   float* lds = f32_lds + 64;
@@ -406,7 +411,7 @@ __global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_fwd_kerne
   const int2 qi = f32_query_info(a, iq);
   const int4 qm = f32_query_meta(a, i0);
   const float slope2 = f.t.slopes ? f.t.slopes[hq] * kLog2e : 0.f;
-  constexpr bool kLds = kF32Lds<NDT>;
+  constexpr bool kLds = f32_two_waves<VEC, NDT>();
   float qf[kLds ? 1 : 16 * NDT];
   if constexpr (kLds) {
     F32Lds<NDT>::template fill<T, VEC>(lds, (const T*)f.q + (int64_t(hq) * f.S + i0) * d, f.S - i0, d);
@@ -780,7 +785,7 @@ __global__ __launch_bounds__(256) void terms_f32_bwd_join_kernel(F32Args a, int6
 }
 
 template <typename T, int VEC, int NDT>
-__global__ __launch_bounds__(256, kF32Lds<NDT> ? 2 : 1) void terms_f32_bwd_kernel(F32Args a, int dkv_blocks) {
+__global__ __launch_bounds__(256, (f32_two_waves<VEC, NDT>() ? 2 : 1)) void terms_f32_bwd_kernel(F32Args a, int dkv_blocks) {
   extern __shared__ __attribute__((aligned(256))) float f32_lds[];
   const int block = blockIdx.x;
   if constexpr (NDT == 8) {

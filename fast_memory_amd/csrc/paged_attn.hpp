@@ -172,7 +172,7 @@ struct FewTile {  // a wave's 32 keys in registers
   uint2 v[8][D / 64];   // keys 4 (l / 16) + r, then 16 + those; dimensions 64 j + 4 (l % 16) ..
 };
 
-template <int D, int NQ>
+template <int D>
 constexpr size_t few_lds_bytes() {
   return 256 + 4 * 16 * (D + 4) * 4 + 4 * 16 * 8;
 }
@@ -606,9 +606,9 @@ inline PagedPlan paged_f32_plan(int rows, int T, int H, int G, int d, int64_t ke
 
 template <bool F16, int D, int NQ>
 static int launch_few(const PagedTileArgs& a, int extra, hipStream_t st) {
-  FM_ALLOW_LDS((paged_few_kernel<F16, D, NQ>), (few_lds_bytes<D, NQ>()), "fm_paged_attn_fwd(lds)");
+  FM_ALLOW_LDS((paged_few_kernel<F16, D, NQ>), few_lds_bytes<D>(), "fm_paged_attn_fwd(lds)");
   hipLaunchKernelGGL((paged_few_kernel<F16, D, NQ>), dim3(unsigned(std::min(a.p.R, a.p.T) * a.p.H * a.few_pieces + extra)), dim3(256),
-                     (few_lds_bytes<D, NQ>()), st, a);
+                     few_lds_bytes<D>(), st, a);
   return launch_status("fm_paged_attn_fwd(few)");
 }
 

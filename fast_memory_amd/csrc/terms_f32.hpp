@@ -1,10 +1,10 @@
 // Attention with score terms in fp32 products: fp32 inputs at any head dimension up to 256, and the 16-bit types at the
 // dimensions and page sizes that the 16-bit matrix instructions are not laid out for.  v_mfma_f32_32x32x2_f32.
 //
-// These instructions take 16 times as long as the 16-bit ones for the same product, so that the operands can come straight
-// from global memory (L1 and L2 serve the repeats): no LDS in the sweep, no barriers, every wave on its own.  A workgroup
+// These instructions take 16 times as long as the 16-bit ones for the same product, so that the streamed operands can come
+// straight from global memory (L1 and L2 serve the repeats): no barriers in the sweep, every wave on its own.  A workgroup
 // owns 32 queries (or 32 keys) and its four waves take the tiles of 32 on the other side in turn; their sums meet in LDS
-// at the end, in wave order.  Short rows are spread over four waves this way, which is what bounds them.
+// at the end, in wave order.  Short rows are spread over four waves this way; too few blocks are cut into pieces (terms_api.hip).
 //
 //   operand of 32 rows   lane (row l % 32, half l / 32) holds half of the row's dimensions, four of eight: the order of a
 //                        contraction is free, a lane then reads 16 consecutive bytes for four products, and both halves the
@@ -12,7 +12,10 @@
 //   scores               as in terms_tile.hpp: lane column = query (key), register r = row 8 (r / 4) + 4 (l / 32) + r % 4
 //   second product       register r of both halves is the operand of one instruction: rows k and k + 4; its partner is
 //                        one element per lane of those two rows, 32 neighbouring dimensions
-// Head dimensions are padded with zeros to Dp = 32 NDT in registers only.
+// Head dimensions are padded with zeros to Dp = 32 NDT in registers and LDS only.
+//
+// Masked places are cleared by selects on bits that are formed beforehand (F32Docs::seen), never by an assignment inside a branch on
+// the mask: with such a branch around the array of scores the compiler left the store of one of them out (documents were ignored).
 //
 // Measured in fp32 (a product of 8192 reaches 154 TFLOP/s): 16 heads x 2048 causal, d = 64 0.13 ms forward = 67 TFLOP/s and 0.45
 // backward, d = 128 0.26 and 0.79, d = 256 (1024 tokens) 0.14 and 0.58; one head of 512 tokens 24 and 39 us.  Bound: the loads'

@@ -1,6 +1,6 @@
 // The tiled forward of the attention with score terms (bf16 / fp16, head dimension 64, 128 or 256): 128 query rows per
-// workgroup, 32 per wave, over tiles of keys.  The training forward (terms_fwd.hip) and the chunks over a paged cache
-// (paged_attn.hip) run it; they differ in where a key's row lies and in what a query row is.
+// workgroup, 32 per wave, over tiles of keys.  The training forward (terms_fwd.hpp) and the chunks over a paged cache
+// (paged_attn.hpp) run it; they differ in where a key's row lies and in what a query row is.
 //
 //   S^T = K.Q^T   v_mfma_f32_32x32x16: A = 32 keys of the tile from LDS, B = this wave's queries, in registers for the
 //                 whole sweep.  Lane (query l % 32, half l / 32) ends up with the scores of keys 8 (r / 4) + 4 (l / 32) +

@@ -18,7 +18,8 @@ REFUSALS = {1: "the pool has fewer free pages than the call needs",
 
 class PagedCache:
     """Keys and values of ``n_rows`` sequences in pages of ``page_size`` tokens (a power of two), out of a pool of
-    ``n_pages`` pages ``k_pages, v_pages [n_pages, n_heads, page_size, d]``.
+    ``n_pages`` pages ``k_pages, v_pages [n_pages, n_heads, page_size, d]``.  ``max_tokens``: the most a row may hold
+    (the whole pool without it); :meth:`attend` takes rows of up to 2^24.
 
     All bookkeeping is one int32 tensor, ``book``, on the device; ``length [n_rows]``, ``refs [n_pages]`` (rows that
     hold a page, 0 = free) and ``table [n_rows, width]`` are views of it.  No call reads anything back, so all of them
@@ -31,7 +32,9 @@ class PagedCache:
 
     def __init__(self, n_rows: int, n_pages: int, page_size: int, n_heads: int, d: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda", max_tokens: Optional[int] = None):
-        width = n_pages if max_tokens is None else -(-int(max_tokens) // page_size)
+        if int(page_size) < 1:
+            raise ValueError(f"PagedCache: page_size={page_size}")
+        width = n_pages if max_tokens is None else -(-int(max_tokens) // int(page_size))
         words = _lib.load().fm_cache_book_ints(int(n_pages), int(n_rows), int(width))
         if words == 0:
             raise ValueError(f"PagedCache: n_rows={n_rows} n_pages={n_pages} max_tokens={max_tokens}")

@@ -406,8 +406,10 @@ int fm_cache_compact(void* k_pages, void* v_pages, int32_t* book, int n_pages, i
  * lse = -FLT_MAX.  What is not seen touches no result, NaN and infinities included.
  * The backward takes the forward's out and lse (or the ones merged with the memory's:
  * the gradients are then the local keys' share), dlse [H*G,S] fp32 or NULL, and writes
- * dq, dk, dv in the inputs' type, each rounded once; the same bits every time.
- * H*G <= 65535, S and L <= 2^24. */
+ * dq, dk, dv in the inputs' type, each rounded once; the same bits every time.  (fp16:
+ * the gradients share one power of two, from the largest |dout| and |v| of the rows that
+ * are finite and no padding; a document that no query belongs to counts among them.)
+ * H*G <= 65535, S and L <= 2^24, H*G*S and H*L < 2^31. */
 size_t fm_local_attn_terms_fwd_workspace(int H, int G, int S, int L, int d, int dtype);
 int fm_local_attn_terms_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
                             float softcap, const float* slopes, const int32_t* doc_q,
@@ -430,7 +432,8 @@ int fm_local_attn_terms_bwd(const void* q, const void* k, const void* v, const v
  * of their own; lse is the natural-log LSE for fm_lse_merge with the memory's attention.
  * A token of no row, or with nothing to see, gets out = 0, lse = -FLT_MAX.  Page numbers
  * outside the pool are clamped into it, never dereferenced.  max_new: no row has more
- * new tokens than that (it shapes the launch only; 0 = unknown).  width * page <= 2^24. */
+ * new tokens than that (it shapes the launch only; 0 = unknown).  H*G <= 65535,
+ * rows and width * page <= 2^24, T*H*G < 2^31. */
 size_t fm_paged_attn_fwd_workspace(int rows, int T, int max_new, int H, int G, int d, int width,
                                    int page, int dtype);
 int fm_paged_attn_fwd(const void* q, int64_t q_token, int64_t q_head, const void* k_pages,

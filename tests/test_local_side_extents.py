@@ -32,3 +32,10 @@ def test_pieces_need_no_large_workspace(dt, d):
             assert 0 < lib.fm_local_attn_terms_fwd_workspace(H, G, S, L, d, dt) <= small + 2 * (512 + H * G) * 128 * (d + 2) * 4
             assert 0 < lib.fm_local_attn_terms_bwd_workspace(H, G, S, L, d, dt) <= \
                 small + 2 * (512 + H * G) * 128 * d * 4 + 2 * (1024 + H) * 2 * 128 * d * 4
+
+
+def test_a_page_of_no_tokens_is_refused():
+    from fast_memory_amd import PagedCache
+    for page in (0, -4):
+        with pytest.raises(ValueError):
+            PagedCache(1, 4, page, 1, 64, device="cpu", max_tokens=8)

@@ -16,8 +16,8 @@
 //
 // Measured, 64 heads x 4096 causal, bf16: d = 128 1.23 ms = 560 TFLOP/s (of 10 d a pair), bias 1.16, cap 1.37, five documents
 // 0.40; d = 64 0.77; d = 256 4.6 (an accumulator is 128 registers: the scores are formed twice and one wave runs on a SIMD).
-// Bound at d = 128: LDS and matrix pipes are asked for the same 1280 cycles a 32 x 32 block of the dk dv sweep (40 KB at 128 bytes
-// a cycle for four waves; 40 MFMAs), the VALU for about 800 more, and two waves a SIMD do not overlap them fully.
+// Bound at d = 128 (counters of 64 heads x 4096 with a bias and a prefix): the matrix pipes are busy 52 % of the time, the VALU 50 %, LDS
+// 26 % without a bank conflict: two waves a SIMD take turns at products and arithmetic more than they overlap them.
 //
 // fp16: p and g of a long row lie below fp16's normal numbers.  p is held times 2^12; g times 2^e, e from the largest
 // |do_i|_2 max_j |v_j|_2 + |D_i| of the call (a bound of |g|), such that |g| 2^e <= 2^13.  bf16 has fp32's range: e = 0.

@@ -17,10 +17,11 @@
 // Masked places are cleared by selects on bits that are formed beforehand (F32Docs::seen), never by an assignment inside a branch on
 // the mask: with such a branch around the array of scores the compiler left the store of one of them out (documents were ignored).
 //
-// Measured in fp32 (a product of 8192 reaches 154 TFLOP/s): 16 heads x 2048 causal, d = 64 0.13 ms forward = 67 TFLOP/s and 0.45
-// backward, d = 128 0.26 and 0.79, d = 256 (1024 tokens) 0.14 and 0.58; one head of 512 tokens 24 and 39 us.  Bound: the loads'
-// latency between the products, at one wave a SIMD (d > 64) or two.  Eight waves a workgroup instead of four: 20 and 54 us for
-// 8 heads x 512, where four take 22 and 42 (the backward's registers no longer hold).
+// Measured in fp32 (a product of 8192 reaches 154 TFLOP/s): 16 heads x 2048 causal, d = 64 130 us forward = 66 TFLOP/s and 356
+// backward, d = 128 199 = 86 and 612, d = 256 (1024 tokens) 109 = 79 and 377; one head of 512 tokens 16 and 24 us, 8 query heads on one
+// KV head x 1024, d = 128, 49 and 104.  bf16 at d = 96, 32 heads x 2048: 768 and 2420 us.  Bound: the loads' latency between the
+// products, at one wave a SIMD (d > 64) or two.  Eight waves a workgroup instead of four: 20 and 54 us for 8 heads x 512, where four
+// take 18 and 36 (the backward's registers no longer hold).
 #pragma once
 #include <type_traits>
 

@@ -8,7 +8,8 @@
 //
 // Measured, 64 heads x 4096 causal, bf16, d = 128: no terms 0.31 ms = 890 TFLOP/s, distance bias 0.33, cap 0.38, both 0.40, five
 // packed documents 0.11; a matrix product of 8192 reaches 1155 here.  Bound: the VALU beside the matrix pipes (a 32 x 32 block is
-// 16 MFMAs of 32 cycles and about 100 vector instructions of 4, the cap 112 more).  Tiles of 32 keys instead of 64: 0.30 ms
+// 16 MFMAs of 32 cycles and about 100 vector instructions of 4, the cap 112 more; counters with a bias and a prefix: VALU busy 64 % of the
+// time, matrix pipes 36 %, LDS 18 %).  Tiles of 32 keys instead of 64: 0.30 ms
 // without terms, but 0.070 against 0.063 at 32 heads x 2048 with a bias, where the barrier a tile shows.
 //
 // Where the blocks are too few for the card (sweep_pieces, terms_api.hip) the tiles that a block sees are cut into pieces, each of

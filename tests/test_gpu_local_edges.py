@@ -315,3 +315,61 @@ def test_pieces_of_queries_with_masked_places_that_are_not_finite(dtype, d, bad)
 def test_a_single_block_in_many_pieces(dtype, d, S, L, t):
     """One block of keys under many queries, and of queries over many keys: up to 64 pieces."""
     check(131, 1, 1, S, L, d, dtype, S < L, t)
+
+
+# ------------------------------------------------------------------ replays
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_replays_follow_which_rows_have_tokens(dtype):
+    """attend recorded once over a cache of 70 rows: every replay finds the rows that have tokens then, and the padding."""
+    R, H, G, d, P, T = 70, 2, 4, 64, 16, 40
+    g = gen(141)
+    n = 40
+    k, v = (torch.randn(n, H, P, d, generator=g).to(dtype).cuda() for _ in range(2))
+    c = PagedCache.over(k, v, torch.zeros(16 + R + n + R * 30, dtype=torch.int32, device="cuda"), R)
+    c.length.copy_(i32([(53 * r) % 480 + 1 for r in range(R)]))
+    c.table.copy_(torch.randint(0, n, (R, 30), generator=g).int())
+    q = torch.randn(T, H * G, d, generator=g).to(dtype).cuda()
+    new = [{3: 1, 69: 2}, {0: 40}, {r: 1 for r in range(0, 40)}, {10: 9, 11: 1, 50: 20, 68: 3}, {}, {69: 1}]
+    cus = [cu_of([x.get(r, 0) for r in range(R)]) for x in new]
+    cu = cus[0].clone()
+    c.attend(q, cu, 0.125)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = c.attend(q, cu, 0.125)
+    for at in (1, 2, 3, 4, 5, 0, 3):
+        cu.copy_(cus[at])
+        graph.replay()
+        torch.cuda.synchronize()
+        o, l = c.attend(q, cus[at], 0.125)
+        assert torch.equal(out, o) and torch.equal(lse, l), at
+        # a token sees something if it is some row's and lies at a position of 0 or more (row 0 holds one key under 40 new tokens)
+        sees = [p >= 0 for r in range(R) for p in range((53 * r) % 480 + 1 - new[at].get(r, 0), (53 * r) % 480 + 1)]
+        sees = torch.tensor(sees + [False] * (T - len(sees)), device="cuda")
+        assert (out[~sees] == 0).all() and (lse[~sees] == O.EMPTY).all() and (lse[sees] > -1e30).all(), at
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float32, 256), (torch.bfloat16, 96), (torch.float16, 64)], ids=str)
+def test_replays_of_a_step_in_pieces(dtype, d):
+    H, G, S, L = 1, 4, 300, 420
+    data = [tuple(x.cuda() for x in inputs(151 + i, H, G, S, L, d, dtype)) for i in range(3)]
+    terms = on_gpu(terms_of(16, H, G, S, L, 15.0, True, 3, 30))
+
+    def step(q, k, v, do, dl):
+        out, lse = ops.local_attn_terms_fwd(q, k, v, 0.09, True, terms)
+        return (out, lse) + ops.local_attn_terms_bwd(do, q, k, v, out, lse, 0.09, True, terms, dl)
+    held = tuple(x.clone() for x in data[0])
+    step(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held)
+    for i in (1, 2, 0, 1):
+        for h, x in zip(held, data[i]):
+            h.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, step(*data[i])):
+            assert torch.equal(x, y)
+        torch.cuda.synchronize()

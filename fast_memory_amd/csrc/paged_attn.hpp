@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256, (few_waves<D, NQ>())) void paged_few_kernel(Pa
           if (a.few_pieces > 1)
             a.part_ml[at] = make_float2(mt, lt);
           else
-            a.p.lse[t * a.p.l_token + hq * a.p.l_head] = none ? -FLT_MAX : (mt + __builtin_amdgcn_logf(lt)) * kLn2;
+            a.p.lse[t * a.p.l_token + hq * a.p.l_head] = none ? -FLT_MAX : tile_lse<F16>(mt, lt);
         }
       }
       __syncthreads();

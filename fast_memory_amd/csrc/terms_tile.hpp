@@ -41,6 +41,12 @@ constexpr float kPUp = F16 ? 12.f : 0.f;
 template <bool F16>
 constexpr float kPLazy = F16 ? 3.f : 8.f;
 
+// The log-sum-exp of sums against m.  (m + kPUp and the scaled l are exact; a logarithm of about 12 would cost bits of a small result.)
+template <bool F16>
+__device__ __forceinline__ float tile_lse(float m, float l) {
+  return ((m + kPUp<F16>) + __builtin_amdgcn_logf(F16 ? l * 0x1p-12f : l)) * kLn2;
+}
+
 // what the scores have, beside the product: bit 0 the cap, bit 1 the distance bias
 constexpr int kModeCap = 1, kModeBias = 2;
 
@@ -509,7 +515,7 @@ __device__ __forceinline__ void tile_write(const typename Mma<F16>::f16v (&O)[D 
       o.y = Mma<F16>::pack2(O[dt][4 * rq + 2] * inv, O[dt][4 * rq + 3] * inv);
       *reinterpret_cast<uint2*>(out + dt * 32 + 8 * rq + 4 * hb) = o;
     }
-  if (hb == 0) *lse = none ? -FLT_MAX : (st.m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (hb == 0) *lse = none ? -FLT_MAX : tile_lse<F16>(st.m, l);
 }
 
 // A piece's state of a query, in fp32 and not yet divided.
@@ -555,7 +561,7 @@ __device__ __forceinline__ void tile_join(const float* __restrict__ po, const fl
   for (int u = 0; u < D / 64; ++u)
     *reinterpret_cast<uint2*>(out + 64 * u + 4 * part) =
         make_uint2(M::pack2(o[4 * u] * inv, o[4 * u + 1] * inv), M::pack2(o[4 * u + 2] * inv, o[4 * u + 3] * inv));
-  if (part == 0) *lse = none ? -FLT_MAX : (mt + __builtin_amdgcn_logf(lt)) * kLn2;
+  if (part == 0) *lse = none ? -FLT_MAX : tile_lse<F16>(mt, lt);
 }
 
 }  // namespace fm

@@ -373,3 +373,24 @@ def test_replays_of_a_step_in_pieces(dtype, d):
         for x, y in zip(got, step(*data[i])):
             assert torch.equal(x, y)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("size", [1e-3, 3e-2])
+def test_the_log_sum_exp_of_small_scores(dtype, d, size):
+    """Scores near 0 over one key: the log-sum-exp is the score.  Beside its bound an exponent against the maximum is rounded once, which
+    fp16 holds 12 off (half a step of 12 is 2^-21), and the logarithm of the sum by as much again."""
+    S = 64
+    g = gen(161)
+    q, k, v = ((torch.randn(1, n, d, generator=g) * s).to(dtype) for n, s in ((S, size), (1, 1.0), (1, 1.0)))
+    f = O.attention(q[0], k[0], v[0], d ** -0.5, torch.ones(S, 1, dtype=torch.bool), t=dtype)
+    more = 2 * 2.0 ** -21 if dtype == torch.float16 else 0.0
+    out, lse = ops.local_attn_terms_fwd(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, False)
+    close(lse[0], f["lse"], f["lse_tol"] + more, "lse")
+    close(out[0], f["out"], f["out_tol"], "out")
+    c = PagedCache(S, S, 16, 1, d, dtype)
+    c.append(k[0, 0].expand(S, 1, d).contiguous().cuda(), v[0, 0].expand(S, 1, d).contiguous().cuda(), i32(list(range(S + 1))))
+    out, lse = c.attend(q[0][:, None].cuda(), i32(list(range(S + 1))), d ** -0.5, max_new=1)
+    close(lse[:, 0], f["lse"], f["lse_tol"] + more, "lse")
+    close(out[:, 0], f["out"], f["out_tol"], "out")

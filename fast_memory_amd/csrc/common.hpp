@@ -29,13 +29,17 @@ static inline int allow_lds(const void* fn, size_t bytes, const char* what) {
     return launch_status(what);
   return FM_OK;
 }
+// (once a device: the attribute is the current device's)
 #define FM_ALLOW_LDS(kernel, bytes, what)                                              \
   do {                                                                                 \
-    static bool done_ = false;                                                         \
-    if (!done_) {                                                                      \
+    static std::atomic<uint64_t> done_{0};                                             \
+    int dev_ = 0;                                                                      \
+    if (hipGetDevice(&dev_) != hipSuccess) return ::fm::launch_status(what);           \
+    const uint64_t bit_ = uint64_t(1) << (dev_ & 63);                                  \
+    if (!(done_.load(std::memory_order_relaxed) & bit_)) {                             \
       int rc_ = ::fm::allow_lds(reinterpret_cast<const void*>(kernel), (bytes), what); \
       if (rc_ != FM_OK) return rc_;                                                    \
-      done_ = true;                                                                    \
+      done_.fetch_or(bit_, std::memory_order_relaxed);                                 \
     }                                                                                  \
   } while (0)
 
